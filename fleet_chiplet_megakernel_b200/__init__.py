@@ -12,8 +12,9 @@ from .qwen3_graph import Qwen3Geometry, build_qwen3_graph, Qwen3Decoder, shard_q
 from . import dsl, fleet
 from .mpk import MPK, MPKMetadata, MirageModelConfig
 from .qwen3_moe_graph import Qwen3MoeGeometry, build_qwen3_moe_graph, Qwen3MoeDecoder
+from .serving import StepPlan, plan_step, rotate_append, chunk_attention, sample_tokens
 
 __all__ = ["PersistentKernel", "DTensor", "bfloat16", "float16", "float32", "int32", "int64", "uint64",
            "valid_persistent_kernel_modes", "get_configurations_from_gpu", "Qwen3Geometry", "build_qwen3_graph",
            "Qwen3Decoder", "shard_qwen3_weights", "dsl", "fleet", "MPK", "MPKMetadata", "MirageModelConfig", "Qwen3MoeGeometry", "build_qwen3_moe_graph",
-           "Qwen3MoeDecoder"]
+           "Qwen3MoeDecoder", "StepPlan", "plan_step", "rotate_append", "chunk_attention", "sample_tokens"]

@@ -24,6 +24,35 @@ class MkConfig(C.Structure):
     ]
 
 
+_P, _I, _L, _F = C.c_void_p, C.c_int32, C.c_int64, C.c_float
+
+
+class MkStepPlanArgs(C.Structure):
+    _fields_ = [(n, _P) for n in ("lengths", "new_tokens", "block_table", "free_pages", "free_range_in", "qo_indptr", "kv_indptr", "kv_indices",
+                                  "last_page_len", "slots", "positions", "granted", "free_range_out")] + \
+        [("table_stride", _L)] + [(n, _I) for n in ("requests", "table_width", "ring_size", "max_indices", "max_tokens", "page_size")]
+
+
+class MkRotateAppendArgs(C.Structure):
+    _fields_ = [(n, _P) for n in ("q", "k", "v", "cos", "sin", "q_norm", "k_norm", "positions", "slots", "k_cache", "v_cache", "out")] + \
+        [(n, _L * 2) for n in ("q_stride", "k_stride", "v_stride", "out_stride", "table_stride")] + \
+        [("k_cache_stride", _L * 3), ("v_cache_stride", _L * 3), ("eps", _F)] + \
+        [(n, _I) for n in ("dtype", "table_dtype", "tokens", "q_heads", "kv_heads", "page_size", "pages", "table_rows")]
+
+
+class MkChunkAttentionArgs(C.Structure):
+    _fields_ = [(n, _P) for n in ("q", "k_cache", "v_cache", "qo_indptr", "kv_indptr", "kv_indices", "last_page_len", "out", "lse", "workspace")] + \
+        [("workspace_bytes", _L), ("q_stride", _L * 2), ("out_stride", _L * 2), ("lse_stride", _L * 2), ("k_cache_stride", _L * 3),
+         ("v_cache_stride", _L * 3), ("scale", _F)] + \
+        [(n, _I) for n in ("dtype", "requests", "tokens", "q_heads", "kv_heads", "page_size", "pages", "num_indices", "window", "sinks", "max_new")]
+
+
+class MkSampleArgs(C.Structure):
+    _fields_ = [(n, _P) for n in ("logits", "qo_indptr", "u", "temperature", "top_p", "min_p", "top_k", "tokens", "logprobs")] + \
+        [("row_stride", _L), ("temperature_value", _F), ("top_p_value", _F), ("min_p_value", _F)] + \
+        [(n, _I) for n in ("top_k_value", "dtype", "requests", "rows", "vocab")]
+
+
 # name -> (restype, argtypes); every symbol the header declares
 SIGNATURES = {
     "mk_create": (C.c_void_p, [C.POINTER(MkConfig)]),
@@ -59,6 +88,12 @@ SIGNATURES = {
     "mk_tensor_ptr": (C.c_void_p, [C.c_void_p, C.c_int]),
     "mk_tensor_read": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int64]),
     "mk_linear_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "mk_op_error": (C.c_int, [C.c_char_p, C.c_int]),
+    "mk_plan_step": (C.c_int, [C.POINTER(MkStepPlanArgs), C.c_void_p]),
+    "mk_rotate_append": (C.c_int, [C.POINTER(MkRotateAppendArgs), C.c_void_p]),
+    "mk_chunk_attention_workspace": (C.c_int64, [C.POINTER(MkChunkAttentionArgs)]),
+    "mk_chunk_attention": (C.c_int, [C.POINTER(MkChunkAttentionArgs), C.c_void_p]),
+    "mk_sample_tokens": (C.c_int, [C.POINTER(MkSampleArgs), C.c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,592 @@
+// mk_chunk_attention: entry point, the kernel for few rows and the merge of its pieces.  (The kernel for many rows: mk_chunk_attention_tiles.cu.)
+//
+// Few rows (one new token per request up to short chunks).  The rows of a kv head (new tokens x its q heads) are cut into groups
+// of 8 or 16; a group has to walk over all K and V rows that it sees, 512 bytes and 4 x 128 x 8 multiplications a position:
+// bound by HBM as long as all SMs stream evenly.  So the unit of work is a tile of 16 positions of a group, and all units of
+// the batch are dealt out as contiguous ranges of equal length to warps, whatever the requests' lengths are: no CTA-wide
+// synchronisation, and one long request among short ones takes no longer than the sum says.  A warp that holds a group's whole
+// range writes its outputs; pieces of a group leave (max, sum, weighted V) in the workspace, and a second kernel merges them
+// in the order of the positions.  K and V tiles come by 16-byte cp.async into a ring of the warp's own, three deep.
+//
+// S = Q K^T with the rows on the M side of mma.m16n8k16, then O^T += V^T P^T with 16 dims on M, for which the scores are the B
+// operand as they are.  P enters as the sum of two 16-bit values (their product with V is cheap here, and the rounding of P would
+// otherwise be as large as that of the output).  A product with P = 0 is not 0 where V is not finite, so a piece whose sums are not
+// finite is done again one row and position at a time, with the positions alone that the row sees.
+#include "mk_chunk_attention.cuh"
+
+namespace mk_serving {
+namespace {
+
+constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps;
+constexpr int kPos = 16;                          // positions of a tile
+constexpr int kTileBytes = kPos * kHeadDim * 2;   // of K, and of V behind it
+constexpr int kRing = 3;
+constexpr int kWarpRing = kRing * 2 * kTileBytes;
+constexpr int kMaxRequests = MK_STEP_MAX_REQUESTS / 2;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <typename T> __device__ __forceinline__ void mma(float4& c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<__nv_bfloat16>(float4& c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c.x), "+f"(c.y), "+f"(c.z), "+f"(c.w) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma<__half>(float4& c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c.x), "+f"(c.y), "+f"(c.z), "+f"(c.w) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The groups of ROWS rows of a request and how many tiles each is counted as (the longest one's).
+template <int ROWS> struct Groups {
+  int groups, tiles;
+  __device__ __forceinline__ Groups(const AttnParams& p, const Request& q) {
+    const long long rows = (long long)q.n * p.per_kv;
+    const bool mine = q.n > 0 && rows <= p.few_rows;
+    groups = mine ? (int)((rows + ROWS - 1) / ROWS) : 0;
+    tiles = 0;
+    if (!mine) return;
+    // A group without a window sees up to len positions; with one, its tokens span at most `span` positions more than the window.
+    const long long span = (ROWS + p.per_kv - 1) / p.per_kv + 1;
+    long long t = ((long long)q.len + kPos - 1) / kPos;
+    if (p.a.window) {
+      const long long w = ((long long)p.a.window + span + kPos - 1) / kPos + 2 + ((long long)p.a.sinks + kPos - 1) / kPos;
+      t = t < w ? t : w;
+    }
+    tiles = (int)(t < 1 ? 1 : t);
+  }
+};
+
+// sums of one group's rows over some positions, as the fragments that the mma leave: lane (g, t) = (lane / 4, lane % 4) holds, for the
+// 16 dims of m-tile i, dims g and g + 8 of rows 2 t and 2 t + 1 (and of the rows 8 further on)
+__host__ __device__ constexpr int part_floats(int rows) { return rows * kHeadDim + 2 * rows; }
+
+template <typename T, int NT> struct RowWarp {
+  static constexpr int ROWS = 8 * NT;
+  const AttnParams& p;
+  const long long* first;  // first unit of every request (shared memory)
+  int lane, warp;
+
+  __device__ __forceinline__ RowWarp(const AttnParams& p_, const long long* f, int w) : p(p_), first(f), lane(threadIdx.x & 31), warp(w) {}
+
+  // A piece: tiles k .. k_end of one group of one kv head; u units are behind this warp, it goes on to u_end.
+  struct Cursor {
+    long long u, u_end;
+    Request q;
+    int r, kv_head, group, k, k_end, tiles, row0, rows, p0, p1, sink, start, count;
+    bool from_start, to_end;  // the piece has the group's first tile, its last
+    __device__ __forceinline__ int position(int i) const { return i < sink ? i * kPos : start + (i - sink) * kPos; }
+  };
+  // the piece that begins at unit c.u
+  __device__ __forceinline__ void open(Cursor& c) const {
+    c.r = find_owner(p.a.requests, c.u, [&](int i) { return first[i]; });
+    c.q = request_of(p.a, c.r);
+    const Groups<ROWS> g(p, c.q);
+    const long long in = c.u - first[c.r];
+    const int item = (int)(in / g.tiles);
+    c.tiles = g.tiles;
+    c.k = (int)(in - (long long)item * g.tiles);
+    c.from_start = c.k == 0;
+    c.k_end = (int)min((long long)g.tiles, c.k + (c.u_end - c.u));
+    c.to_end = c.k_end == g.tiles;
+    c.kv_head = item / g.groups;
+    c.group = item - c.kv_head * g.groups;
+    c.row0 = c.group * ROWS;
+    c.rows = (int)min((long long)ROWS, (long long)c.q.n * p.per_kv - c.row0);
+    c.p0 = c.q.len - c.q.n + c.row0 / p.per_kv;
+    c.p1 = c.q.len - c.q.n + (c.row0 + c.rows - 1) / p.per_kv;
+    const Span<kPos> s(p.a, c.p0, c.p1);
+    c.sink = s.sink;
+    c.start = s.start;
+    c.count = s.count;
+  }
+
+  // K and V rows of tile i of the cursor's piece -> stage; rows that are not there become zeros
+  __device__ __forceinline__ void load(const Cursor& c, int i, uint32_t stage) const {
+    const int pos = c.position(i) + (lane & 15);
+    int page, in_page;
+    locate(p, c.q, i < c.count ? pos : c.q.len, &page, &in_page);
+    const mk_chunk_attention_args& a = p.a;
+    const T* kc = (const T*)a.k_cache + c.kv_head * a.k_cache_stride[2] + (lane & 7) * 8;
+    const T* vc = (const T*)a.v_cache + c.kv_head * a.v_cache_stride[2] + (lane & 7) * 8;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int row = (lane >> 3) + 4 * j;
+      const int pg = __shfl_sync(kAll, page, row), in = __shfl_sync(kAll, in_page, row);
+      const bool there = pg >= 0;
+      const T* kr = kc + (there ? (long long)pg * a.k_cache_stride[0] + (long long)in * a.k_cache_stride[1] : 0);
+      const T* vr = vc + (there ? (long long)pg * a.v_cache_stride[0] + (long long)in * a.v_cache_stride[1] : 0);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t dst = stage + (uint32_t)(row * 256 + ((((lane & 7) + 8 * half) ^ (row & 7)) << 4));
+        cp_async16(dst, kr + 64 * half, there);
+        cp_async16(dst + kTileBytes, vr + 64 * half, there);
+      }
+    }
+  }
+
+  __device__ __forceinline__ float* slot_of(const Cursor& c) const {
+    return p.partial + (size_t)(2 * warp + (c.from_start ? 1 : 0)) * part_floats(ROWS);
+  }
+  __device__ __forceinline__ long long row_token(const Cursor& c, int row, int* head) const {
+    const int x = c.row0 + row, tok = x / p.per_kv;
+    *head = c.kv_head * p.per_kv + (x - tok * p.per_kv);
+    return c.q.q0 + tok;
+  }
+
+  // The piece again, a row and a position at a time: sums that are not finite reach only the rows that see their cause.
+  __device__ __noinline__ void exactly(const Cursor& c, int k0) const {
+    const mk_chunk_attention_args& a = p.a;
+    for (int row = 0; row < c.rows; ++row) {
+      int head;
+      const long long tok = row_token(c, row, &head);
+      const int at = c.q.len - c.q.n + (c.row0 + row) / p.per_kv;
+      const T* qr = (const T*)a.q + tok * a.q_stride[0] + head * a.q_stride[1] + 4 * lane;
+      float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) q[d] = to_float(qr[d]);
+      for (int i = k0; i < min(c.k_end, c.count); ++i)
+        for (int j = c.position(i); j < c.position(i) + kPos; ++j) {
+          if (!sees(a, j, at)) continue;
+          int page, in;
+          locate(p, c.q, j, &page, &in);
+          float s = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+          if (page >= 0) {
+            const T* kr = (const T*)a.k_cache + (long long)page * a.k_cache_stride[0] + (long long)in * a.k_cache_stride[1] + c.kv_head * a.k_cache_stride[2] + 4 * lane;
+            const T* vr = (const T*)a.v_cache + (long long)page * a.v_cache_stride[0] + (long long)in * a.v_cache_stride[1] + c.kv_head * a.v_cache_stride[2] + 4 * lane;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              s += q[d] * to_float(kr[d]);
+              v[d] = to_float(vr[d]);
+            }
+          }
+#pragma unroll
+          for (int o2 = 16; o2 > 0; o2 >>= 1) s += __shfl_xor_sync(kAll, s, o2);
+          s *= p.scale_log2;
+          if (s == -INFINITY) continue;
+          const float mn = s > m ? s : m;  // (a NaN score leaves the maximum and enters the weight)
+          const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - (mn == -INFINITY ? 0.f : mn));
+          l = l * alpha + w;
+#pragma unroll
+          for (int d = 0; d < 4; ++d) o[d] = o[d] * alpha + w * v[d];
+          m = mn;
+        }
+      if (c.from_start && c.to_end) {
+        T* dst = (T*)a.out + tok * a.out_stride[0] + head * a.out_stride[1] + 4 * lane;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) dst[d] = from_float<T>(l == 0.f ? 0.f : o[d] / l);
+        if (a.lse && lane == 0) a.lse[tok * a.lse_stride[0] + head * a.lse_stride[1]] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      } else {
+        float* part = slot_of(c);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const int dim = 4 * lane + d, i = dim >> 4, half = (dim >> 3) & 1, g = dim & 7, nt = row >> 3, t = (row & 7) >> 1;
+          part[(((nt * 8 + i) * 32) + g * 4 + t) * 4 + half * 2 + (row & 1)] = o[d];
+        }
+        if (lane == 0) {
+          part[ROWS * kHeadDim + row] = m;
+          part[ROWS * kHeadDim + ROWS + row] = l;
+        }
+      }
+    }
+  }
+
+  __device__ void run(long long u0, long long u1, uint32_t ring) {
+    const mk_chunk_attention_args& a = p.a;
+    const int g = lane >> 2, t = lane & 3;
+    Cursor ld, c;
+    ld.u = c.u = u0;
+    ld.u_end = c.u_end = u1;
+    open(ld);
+    c = ld;
+    // The loader is kRing - 1 tiles ahead of the sums, across the border between two pieces.
+    auto load_next = [&](int stage) {
+      if (ld.u < ld.u_end) {
+        load(ld, ld.k, ring + (uint32_t)(stage * 2 * kTileBytes));
+        ++ld.u;
+        if (++ld.k == ld.k_end && ld.u < ld.u_end) open(ld);
+      }
+      cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i) load_next(i);
+    int stage = 0;
+    while (c.u < c.u_end) {
+      // q rows as the A operand: rows g and g + 8
+      uint32_t qf[8][4];
+      int pos[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = g + 8 * h;
+        pos[h] = -1;
+        const T* qr = nullptr;
+        if (h < NT && row < c.rows) {
+          int head;
+          const long long tok = row_token(c, row, &head);
+          qr = (const T*)a.q + tok * a.q_stride[0] + head * a.q_stride[1];
+          pos[h] = c.q.len - c.q.n + (c.row0 + row) / p.per_kv;
+        }
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          qf[ks][h] = qr ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 2 * t) : 0u;
+          qf[ks][h + 2] = qr ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8 + 2 * t) : 0u;
+        }
+      }
+      float4 o[NT][8];
+      float m[NT], l[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[n][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const int k0 = c.k;
+      for (; c.k < c.k_end; ++c.k, ++c.u) {
+        cp_async_wait<kRing - 2>();
+        __syncwarp();
+        const uint32_t ks_ = ring + (uint32_t)(stage * 2 * kTileBytes), vs = ks_ + kTileBytes;
+        const int fill = stage == 0 ? kRing - 1 : stage - 1;
+        stage = stage == kRing - 1 ? 0 : stage + 1;
+        load_next(fill);  // (the stage that the last tile left: every lane is past its reads)
+        if (c.k >= c.count) continue;
+        const int start = c.position(c.k);
+        const uint32_t lrow = (uint32_t)((lane & 7) + ((lane >> 4) << 3)), lchunk = (uint32_t)((lane >> 3) & 1);
+        float4 s[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t kf[4];
+          ldmatrix4(ks_ + lrow * 256 + (((2 * ks + lchunk) ^ (lrow & 7)) << 4), kf);
+          mma<T>(s[0], qf[ks], kf[0], kf[1]);
+          mma<T>(s[1], qf[ks], kf[2], kf[3]);
+        }
+        float sc[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          sc[n][0] = (n ? s[0].z : s[0].x) * p.scale_log2;
+          sc[n][1] = (n ? s[0].w : s[0].y) * p.scale_log2;
+          sc[n][2] = (n ? s[1].z : s[1].x) * p.scale_log2;
+          sc[n][3] = (n ? s[1].w : s[1].y) * p.scale_log2;
+        }
+        // every live row sees the whole tile, or each its own part
+        if (!(start + kPos - 1 <= c.p0 && (a.window == 0 || start > (long long)c.p1 - a.window || start + kPos <= a.sinks))) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int j = start + (e >> 1) * 8 + 2 * t + (e & 1);
+              if (!sees(a, j, pos[n])) sc[n][e] = -INFINITY;
+            }
+        }
+        uint32_t hi[NT][2], lo[NT][2];
+        float alpha[NT];
+        bool moved = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float mx = fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3]));
+          mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(kAll, mx, 2));
+          const float mn = fmaxf(m[n], mx), base = mn == -INFINITY ? 0.f : mn;
+          alpha[n] = m[n] == mn ? 1.f : exp2f(m[n] - base);
+          moved = moved || m[n] != mn;
+          m[n] = mn;
+          float w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = exp2f(sc[n][e] - base);
+          l[n] = l[n] * alpha[n] + ((w[0] + w[1]) + (w[2] + w[3]));
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            hi[n][e] = pack2<T>(w[2 * e], w[2 * e + 1]);
+            const float2 back = unpack2<T>(hi[n][e]);
+            lo[n][e] = pack2<T>(w[2 * e] - back.x, w[2 * e + 1] - back.y);
+          }
+        }
+        if (__any_sync(kAll, moved)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float a0 = __shfl_sync(kAll, alpha[n], 8 * t), a1 = __shfl_sync(kAll, alpha[n], 8 * t + 4);  // rows 2 t and 2 t + 1
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              o[n][i].x *= a0; o[n][i].y *= a1;
+              o[n][i].z *= a0; o[n][i].w *= a1;
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t vf[4];
+          ldmatrix4t(vs + lrow * 256 + (((2 * i + lchunk) ^ (lrow & 7)) << 4), vf);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            mma<T>(o[n][i], vf, hi[n][0], hi[n][1]);
+            mma<T>(o[n][i], vf, lo[n][0], lo[n][1]);
+          }
+        }
+        __syncwarp();
+      }
+      // the piece is done
+      bool bad = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        l[n] += __shfl_xor_sync(kAll, l[n], 1);
+        l[n] += __shfl_xor_sync(kAll, l[n], 2);
+        bad = bad || !isfinite(l[n]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) bad = bad || !isfinite((o[n][i].x + o[n][i].y) + (o[n][i].z + o[n][i].w));
+      }
+      if (__any_sync(kAll, bad)) {
+        const Cursor copy = c;  // (so that the cursor itself can stay in registers)
+        exactly(copy, k0);
+      } else if (c.from_start && c.to_end) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+          const float i0 = __shfl_sync(kAll, inv, 8 * t), i1 = __shfl_sync(kAll, inv, 8 * t + 4);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int row = 8 * n + 2 * t + e;
+            if (row >= c.rows) continue;
+            int head;
+            const long long tok = row_token(c, row, &head);
+            T* dst = (T*)a.out + tok * a.out_stride[0] + head * a.out_stride[1] + g;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              dst[16 * i] = from_float<T>((e ? o[n][i].y : o[n][i].x) * (e ? i1 : i0));
+              dst[16 * i + 8] = from_float<T>((e ? o[n][i].w : o[n][i].z) * (e ? i1 : i0));
+            }
+          }
+          const int row = 8 * n + g;
+          if (a.lse && t == 0 && row < c.rows) {
+            int head;
+            const long long tok = row_token(c, row, &head);
+            a.lse[tok * a.lse_stride[0] + head * a.lse_stride[1]] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+          }
+        }
+      } else {
+        float* part = slot_of(c);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(part)[(n * 8 + i) * 32 + lane] = o[n][i];
+          if (t == 0) {
+            part[ROWS * kHeadDim + 8 * n + g] = m[n];
+            part[ROWS * kHeadDim + ROWS + 8 * n + g] = l[n];
+          }
+        }
+      }
+      if (c.u < c.u_end) open(c);
+    }
+    cp_async_wait<0>();
+  }
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(kRowThreads, 1) chunk_attention_rows(const __grid_constant__ AttnParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  long long* first = reinterpret_cast<long long*>(smem + kRowWarps * kWarpRing);
+  __shared__ long long carry[kRowWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = p.a.requests;
+  long long total = 0;
+  for (int r0 = 0; r0 < R; r0 += kRowThreads) {
+    const int r = r0 + threadIdx.x;
+    long long v = 0;
+    if (r < R) {
+      const Groups<8 * NT> g(p, request_of(p.a, r));
+      v = (long long)g.groups * g.tiles * p.a.kv_heads;
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(kAll, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) carry[warp] = v;
+    __syncthreads();
+    long long before = total;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      if (w < warp) before += carry[w];
+      total += carry[w];
+    }
+    if (r < R) first[r + 1] = before + v;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) first[0] = 0;
+  __syncthreads();
+  long long per = (total + p.warps - 1) / p.warps;
+  per = per > p.min_tiles ? per : p.min_tiles;
+  if (blockIdx.x == 0) {
+    for (int r = threadIdx.x; r <= R; r += kRowThreads) p.plan[1 + r] = first[r];
+    if (threadIdx.x == 0) p.plan[0] = per;
+  }
+  // ranges that follow each other go to different SMs
+  const int w = warp * gridDim.x + blockIdx.x;
+  const long long u0 = w * per, u1 = min(total, u0 + per);
+  if (u0 >= u1) return;
+  RowWarp<T, NT>(p, first, w).run(u0, u1, (uint32_t)__cvta_generic_to_shared(smem + warp * kWarpRing));
+}
+
+// One CTA per group and kv head; warp i has the 16 dims of m-tile i.
+template <typename T, int NT>
+__global__ void __launch_bounds__(256) chunk_attention_merge(const __grid_constant__ AttnParams p) {
+  constexpr int ROWS = 8 * NT;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const mk_chunk_attention_args& a = p.a;
+  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  // request r has the slots from floor(first row / ROWS) + r on: as many as its groups at least
+  auto base = [&](int r) { return (long long)min(max(__ldg(a.qo_indptr + r), 0), a.tokens) * p.per_kv / ROWS + r; };
+  const int r = find_owner_warp(a.requests, blockIdx.x, base);
+  const Request q = request_of(a, r);
+  const Groups<ROWS> gr(p, q);
+  const long long group = blockIdx.x - base(r);
+  if (group < 0 || group >= gr.groups) return;
+  const long long per = p.plan[0], u0 = p.plan[1 + r] + ((long long)blockIdx.y * gr.groups + group) * gr.tiles, u1 = u0 + gr.tiles - 1;
+  const int w0 = (int)(u0 / per), w1 = (int)(u1 / per);
+  if (w0 == w1) return;  // the warp has written the outputs
+  // a warp's slot 1 holds the piece that begins a group, slot 0 the one that does not
+  auto part = [&](int w) { return p.partial + (size_t)(2 * w + (w * per <= u0 ? 1 : 0)) * part_floats(ROWS); };
+  float m[NT], l[NT];
+  float4 o[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    m[n] = -INFINITY;
+    for (int w = w0 + t; w <= w1; w += 4) m[n] = fmaxf(m[n], part(w)[ROWS * kHeadDim + 8 * n + g]);
+    m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 1));
+    m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 2));
+    l[n] = 0.f;
+    o[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+#pragma unroll 4
+  for (int w = w0; w <= w1; ++w) {
+    const float* pt = part(w);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float mw = pt[ROWS * kHeadDim + 8 * n + g], lw = pt[ROWS * kHeadDim + ROWS + 8 * n + g];
+      const float4 ow = reinterpret_cast<const float4*>(pt)[(n * 8 + i) * 32 + lane];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - m[n]);
+      l[n] += f * lw;
+      const float f0 = __shfl_sync(kAll, f, 8 * t), f1 = __shfl_sync(kAll, f, 8 * t + 4);
+      // (a piece that saw nothing of a row has weight 0 and finite sums)
+      o[n].x += f0 * ow.x; o[n].y += f1 * ow.y;
+      o[n].z += f0 * ow.z; o[n].w += f1 * ow.w;
+    }
+  }
+  const int row0 = (int)group * ROWS, rows = (int)min((long long)ROWS, (long long)q.n * p.per_kv - row0);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+    const float i0 = __shfl_sync(kAll, inv, 8 * t), i1 = __shfl_sync(kAll, inv, 8 * t + 4);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = 8 * n + 2 * t + e;
+      if (row >= rows) continue;
+      const int x = row0 + row, tok = x / p.per_kv, head = blockIdx.y * p.per_kv + (x - tok * p.per_kv);
+      T* dst = (T*)a.out + (long long)(q.q0 + tok) * a.out_stride[0] + head * a.out_stride[1] + 16 * i + g;
+      dst[0] = from_float<T>((e ? o[n].y : o[n].x) * (e ? i1 : i0));
+      dst[8] = from_float<T>((e ? o[n].w : o[n].z) * (e ? i1 : i0));
+    }
+    const int row = 8 * n + g;
+    if (a.lse && i == 0 && t == 0 && row < rows) {
+      const int x = row0 + row, tok = x / p.per_kv, head = blockIdx.y * p.per_kv + (x - tok * p.per_kv);
+      a.lse[(long long)(q.q0 + tok) * a.lse_stride[0] + head * a.lse_stride[1]] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+    }
+  }
+}
+
+template <typename T, int NT> int launch_rows(const AttnParams& p, cudaStream_t s) {
+  const int smem = kRowWarps * kWarpRing + (p.a.requests + 1) * 8;
+  cudaError_t e = cudaFuncSetAttribute(chunk_attention_rows<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: %s", cudaGetErrorString(e));
+  chunk_attention_rows<T, NT><<<p.warps / kRowWarps, kRowThreads, smem, s>>>(p);
+  if (int rc = launched("chunk_attention")) return rc;
+  // the merge may be set up while the rows are still being done; it waits for them itself
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((long long)p.a.tokens * p.per_kv / (8 * NT) + p.a.requests), (unsigned)p.a.kv_heads);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, chunk_attention_merge<T, NT>, p);
+  return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "chunk_attention: launch failed: %s", cudaGetErrorString(e));
+}
+
+// What a call needs of the workspace; the host's choices of kernels stand here once.
+struct Layout {
+  int nt, warps;
+  size_t plan, partial, bytes;
+};
+Layout layout_of(const mk_chunk_attention_args& a) {
+  Layout l;
+  const int per_kv = a.q_heads / a.kv_heads;
+  const long long most = a.max_new > 0 ? a.max_new : a.tokens;
+  l.nt = most * per_kv <= 8 ? 1 : 2;
+  l.warps = sm_count() * kRowWarps;
+  l.plan = 0;
+  l.partial = ((size_t)(a.requests + 2) * 8 + 255) / 256 * 256;
+  l.bytes = l.partial + (size_t)2 * l.warps * part_floats(8 * l.nt) * sizeof(float);
+  return l;
+}
+
+int check(const mk_chunk_attention_args& a) {
+  if (!a.q || !a.k_cache || !a.v_cache || !a.qo_indptr || !a.kv_indptr || !a.kv_indices || !a.last_page_len || !a.out)
+    return fail(MK_E_INVALID, "chunk_attention: null pointer");
+  if (a.dtype != MK_BF16 && a.dtype != MK_F16) return fail(MK_E_INVALID, "chunk_attention: rows and caches are bf16 or fp16");
+  if (a.tokens < 0 || a.q_heads < 1 || a.kv_heads < 1 || a.page_size < 1 || a.pages < 1 || a.num_indices < 0 || a.window < 0 || a.sinks < 0 || a.max_new < 0)
+    return fail(MK_E_INVALID, "chunk_attention: negative or zero size");
+  if (a.q_heads % a.kv_heads) return fail(MK_E_INVALID, "chunk_attention: %d q heads on %d kv heads", a.q_heads, a.kv_heads);
+  if (a.requests < 1 || a.requests > kMaxRequests)
+    return fail(a.requests < 1 ? MK_E_INVALID : MK_E_TOO_LARGE, "chunk_attention: %d requests (1 to %d)", a.requests, kMaxRequests);
+  if ((long long)a.tokens * a.q_heads > 0x3fffffffll || a.kv_heads > 65535) return fail(MK_E_TOO_LARGE, "chunk_attention: too many rows");
+  if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out)) return fail(MK_E_INVALID, "chunk_attention: pointers must be 16-byte aligned");
+  for (int i = 0; i < 3; ++i)
+    if ((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7) return fail(MK_E_INVALID, "chunk_attention: rows of the caches must start at multiples of 16 bytes");
+  for (int i = 0; i < 2; ++i)
+    if ((a.q_stride[i] | a.out_stride[i]) & 7) return fail(MK_E_INVALID, "chunk_attention: rows of q and out must start at multiples of 16 bytes");
+  return 0;
+}
+
+}  // namespace
+}  // namespace mk_serving
+
+extern "C" int64_t mk_chunk_attention_workspace(const mk_chunk_attention_args* args) {
+  using namespace mk_serving;
+  if (!args) return fail(MK_E_INVALID, "chunk_attention: null arguments");
+  if (int rc = check(*args)) return rc;
+  return (int64_t)layout_of(*args).bytes;
+}
+
+extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* stream) {
+  using namespace mk_serving;
+  if (!args) return fail(MK_E_INVALID, "chunk_attention: null arguments");
+  const mk_chunk_attention_args& a = *args;
+  if (int rc = check(a)) return rc;
+  if (a.tokens == 0) return 0;
+  const Layout l = layout_of(a);
+  if (!a.workspace || a.workspace_bytes < (int64_t)l.bytes || (((uintptr_t)a.workspace) & 15))
+    return fail(MK_E_INVALID, "chunk_attention: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)l.bytes);
+  AttnParams p = {};
+  p.a = a;
+  p.per_kv = a.q_heads / a.kv_heads;
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.page_size == 1 << s) p.page_shift = s;
+  p.scale_log2 = a.scale * kLog2e;
+  p.warps = l.warps;
+  p.min_tiles = 4;
+  p.plan = reinterpret_cast<long long*>((char*)a.workspace + l.plan);
+  p.partial = reinterpret_cast<float*>((char*)a.workspace + l.partial);
+  p.few_rows = 0x7fffffff;
+  const cudaStream_t s = (cudaStream_t)stream;
+  if (a.dtype == MK_BF16) return l.nt == 1 ? launch_rows<__nv_bfloat16, 1>(p, s) : launch_rows<__nv_bfloat16, 2>(p, s);
+  return l.nt == 1 ? launch_rows<__half, 1>(p, s) : launch_rows<__half, 2>(p, s);
+}

@@ -1,0 +1,78 @@
+// Attention of the new tokens of a batch over a paged K/V cache: what its kernels share.
+//
+// Request r has the n new rows qo_indptr[r] <= t < qo_indptr[r + 1] and, with its new tokens, `len` positions: its pages are
+// kv_indices[kv_indptr[r] .. kv_indptr[r + 1]), the last of them filled up to last_page_len[r].  Row i of the n sits at
+// position p = len - n + i and sees position j where
+//     0 <= j <= p   and   (no window, or j > p - window, or j < sinks).
+// out = sum_j w_j v_j / sum_j w_j with w_j = exp(scale q.k_j); a row that sees nothing is zero, its lse minus infinity.
+// What the index arrays say is held against the sizes of the tensors before it is used: a page that does not exist reads as zeros.
+#ifndef MK_CHUNK_ATTENTION_CUH
+#define MK_CHUNK_ATTENTION_CUH
+
+#include "mk_serving.cuh"
+
+namespace mk_serving {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+struct AttnParams {
+  mk_chunk_attention_args a;
+  int per_kv;           // q heads of a kv head
+  int page_shift;       // log2 of the page size, -1 if it is no power of two
+  float scale_log2;     // scale * log2(e): scores and maxima are kept in base 2
+  int few_rows;         // requests with at most so many rows (new tokens x q heads of a kv head) are the row kernel's, others the tile kernel's
+  int min_tiles;        // a warp's share of the row kernel is no shorter
+  int warps;            // of the row kernel
+  long long* plan;      // row kernel -> merge: [tiles a warp][first tile of request 0 .. R]
+  float* partial;       // of the row kernel's pieces
+  int splits;           // of the tile kernel: pieces of every row's positions
+  float* tile_partial;  // [splits][tokens][q heads][130]
+};
+
+struct Request {
+  int q0, n, len, kv0;  // first row, rows, positions, first entry of the page index
+};
+__device__ __forceinline__ Request request_of(const mk_chunk_attention_args& a, int r) {
+  Request q;
+  const int q0 = __ldg(a.qo_indptr + r), q1 = __ldg(a.qo_indptr + r + 1), k0 = __ldg(a.kv_indptr + r), k1 = __ldg(a.kv_indptr + r + 1), last = __ldg(a.last_page_len + r);
+  q.q0 = min(max(q0, 0), a.tokens);
+  q.n = min(max(q1, q.q0), a.tokens) - q.q0;
+  q.kv0 = min(max(k0, 0), a.num_indices);
+  const int pages = min(max(k1, q.kv0), a.num_indices) - q.kv0;
+  q.len = pages > 0 ? (int)min((long long)(pages - 1) * a.page_size + min(max(last, 0), a.page_size), 0x7fffff00ll) : 0;
+  return q;
+}
+__device__ __forceinline__ bool sees(const mk_chunk_attention_args& a, int j, int p) {
+  return j <= p && (a.window == 0 || j > p - a.window || j < a.sinks);
+}
+// Page and row in the page of a position; the page is -1 where it does not exist.
+__device__ __forceinline__ void locate(const AttnParams& p, const Request& q, int pos, int* page, int* in_page) {
+  const int k = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.a.page_size;
+  *in_page = pos - k * p.a.page_size;
+  const int pg = pos < q.len ? __ldg(p.a.kv_indices + q.kv0 + k) : -1;
+  *page = (unsigned)pg < (unsigned)p.a.pages ? pg : -1;
+}
+
+// The tiles of `TILE` positions that rows at positions p0 <= p <= p1 see: `sink` tiles from position 0, the others from `start` on.
+template <int TILE> struct Span {
+  int sink, start, count;
+  __device__ __forceinline__ Span(const mk_chunk_attention_args& a, int p0, int p1) {
+    if (p1 < 0) {
+      sink = start = count = 0;
+      return;
+    }
+    // (64 bits: the window may be as long as an int)
+    const long long w0 = a.window == 0 ? 0 : (long long)max(p0, 0) - a.window + 1;
+    start = w0 > 0 ? (int)(w0 / TILE) * TILE : 0;
+    sink = min((int)(((long long)a.sinks + TILE - 1) / TILE), start / TILE);
+    if (a.window == 0) sink = 0;
+    count = sink + (p1 - start) / TILE + 1;
+  }
+  __device__ __forceinline__ int position(int k) const { return k < sink ? k * TILE : start + (k - sink) * TILE; }
+};
+
+int launch_tile_attention(const AttnParams& p, cudaStream_t s);  // mk_chunk_attention_tiles.cu
+
+}  // namespace mk_serving
+
+#endif

@@ -1,0 +1,207 @@
+// mk_plan_step: page allocation, block tables, index pointers and slot map of a serving step, from the requests' lengths.
+//
+// With held(r) = ceil(length / page) and need(r) = ceil((length + new) / page) - held(r), everything that the step needs is a
+// prefix sum over the requests (pages taken from the ring, pages given back, token rows, pages in the index) and a lookup in
+// it.  The sums are short (a few hundred to a few thousand requests) and the lookups many (a page each, a token each), so
+// every CTA works out all the sums for itself in shared memory and then takes its share of the lookups: one launch, no
+// CTA waits for another, no atomics.  What is read and written is about 8 bytes a page and 12 a token; bound by latency.
+#include "mk_serving.cuh"
+
+namespace mk_serving {
+namespace {
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanWarps = kPlanThreads / 32;
+
+struct PlanParams {
+  mk_step_plan_args a;
+};
+
+// Inclusive sum over the block, and the block's total; `carry` holds kPlanWarps + 1 values and is free again on return.
+__device__ __forceinline__ long long block_scan(long long v, long long* carry, long long* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long u = __shfl_up_sync(kAll, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) carry[warp] = v;
+  __syncthreads();
+  if (warp == 0) {
+    long long c = lane < kPlanWarps ? carry[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long u = __shfl_up_sync(kAll, c, o);
+      if (lane >= o) c += u;
+    }
+    if (lane < kPlanWarps) carry[lane] = c;
+  }
+  __syncthreads();
+  const long long before = warp ? carry[warp - 1] : 0;
+  *total = carry[kPlanWarps - 1];
+  __syncthreads();
+  return before + v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_constant__ PlanParams p) {
+  const mk_step_plan_args& a = p.a;
+  extern __shared__ int table[];  // three tables of R + 1 first entries: token rows, pages of the index, pages given back
+  __shared__ long long carry[kPlanWarps];
+  const int R = a.requests, page = a.page_size;
+  int* tok0 = table;
+  int* kv0 = tok0 + R + 1;
+  int* need0 = kv0 + R + 1;
+  int* back0 = need0 + R + 1;
+  const long long head = a.free_range_in[0], tail = a.free_range_in[1];
+  const long long longest = min((long long)a.table_width * page, 0x7fffffffll);  // what a row of the block table can hold
+  auto length_of = [&](int r) { return (int)min((long long)max(0, a.lengths[r]), longest); };
+  auto pages_of = [&](long long n) { return (n + page - 1) / page; };
+
+  // pages that ended requests give back: they count as free in this step already
+  long long back = 0, total;
+  for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
+    const int r = r0 + threadIdx.x;
+    const long long mine = r < R && a.new_tokens[r] < 0 ? pages_of(length_of(r)) : 0;
+    const long long upto = back + block_scan(mine, carry, &total);
+    if (r < R) back0[r + 1] = (int)upto;
+    back += total;
+  }
+  const long long free_pages = tail - head + back;
+
+  long long wanted = 0, rows = 0, kv = 0, taken = 0, tokens = 0;
+  for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
+    const int r = r0 + threadIdx.x;
+    const int len = r < R ? length_of(r) : 0, want = r < R ? a.new_tokens[r] : 0;
+    const long long held = pages_of(len), after = pages_of((long long)len + max(0, want));
+    const bool valid = want > 0 && after <= a.table_width;
+    const long long need = valid ? after - held : 0;
+    const long long upto = wanted + block_scan(need, carry, &total);
+    wanted += total;
+    const bool fits = valid && (need == 0 || upto <= free_pages);
+    const long long row_end = rows + block_scan(fits ? want : 0, carry, &total);
+    rows += total;
+    const int granted = fits && row_end <= a.max_tokens ? want : 0;
+    const long long take = granted > 0 ? need : 0;
+    // (want < 0: ended.  A request that gets nothing keeps the pages that it has.)
+    const long long pages = want < 0 ? 0 : held + take;
+    const long long tok_end = tokens + block_scan(granted, carry, &total);
+    tokens += total;
+    const long long need_end = taken + block_scan(take, carry, &total);
+    taken += total;
+    const long long kv_end = kv + block_scan(pages, carry, &total);
+    kv += total;
+    if (r < R) {
+      tok0[r + 1] = (int)tok_end;
+      need0[r + 1] = (int)need_end;
+      kv0[r + 1] = (int)kv_end;
+      if (blockIdx.x == 0) {
+        a.granted[r] = granted;
+        a.qo_indptr[r + 1] = (int)tok_end;
+        a.kv_indptr[r + 1] = (int)kv_end;
+        a.last_page_len[r] = pages > 0 ? (int)(len + granted - (pages - 1) * page) : 0;
+      }
+    }
+  }
+  if (threadIdx.x == 0) {
+    tok0[0] = kv0[0] = need0[0] = back0[0] = 0;
+    if (blockIdx.x == 0) {
+      a.qo_indptr[0] = a.kv_indptr[0] = 0;
+      a.free_range_out[0] = head + taken;
+      a.free_range_out[1] = tail + back;
+    }
+  }
+  __syncthreads();
+
+  const long long ring = a.ring_size;
+  const long long head_at = ring > 0 ? ((head % ring) + ring) % ring : 0, tail_at = ring > 0 ? ((tail % ring) + ring) % ring : 0;
+  // page i of those that the step takes, ring first; what ended requests give back in this launch comes from their own rows
+  auto taken_page = [&](long long i) -> int {
+    const long long in_ring = tail - head;
+    if (i < in_ring) {
+      const long long at = head_at + i;
+      return a.free_pages[at < ring ? at : at % ring];
+    }
+    const int b = (int)(i - in_ring);
+    const int r = find_owner(R, b, [&](int k) { return (long long)back0[k]; });
+    return a.block_table[(long long)r * a.table_stride + (b - back0[r])];
+  };
+  auto page_at = [&](int r, int k) -> int {  // page k of request r, held or taken
+    const int held = (int)pages_of(length_of(r));
+    return k < held ? a.block_table[(long long)r * a.table_stride + k] : taken_page((long long)need0[r] + k - held);
+  };
+
+  const long long n_kv = min(kv, (long long)a.max_indices);
+  const long long n_back = ring > 0 ? back : 0;
+  const long long all = n_kv + a.max_tokens + n_back;
+  for (long long e = (long long)blockIdx.x * kPlanThreads + threadIdx.x; e < all; e += (long long)gridDim.x * kPlanThreads) {
+    if (e < n_kv) {  // an entry of the page index; a new page enters its request's table as well
+      const int r = find_owner(R, e, [&](int k) { return (long long)kv0[k]; });
+      const int k = (int)e - kv0[r], held = (int)pages_of(length_of(r));
+      const int pg = page_at(r, k);
+      a.kv_indices[e] = pg;
+      if (k >= held) a.block_table[(long long)r * a.table_stride + k] = pg;
+    } else if (e < n_kv + a.max_tokens) {  // a token row: its position and cache slot
+      const int t = (int)(e - n_kv);
+      long long slot = -1;
+      int pos = 0;
+      if (t < tokens) {
+        const int r = find_owner(R, t, [&](int k) { return (long long)tok0[k]; });
+        pos = length_of(r) + t - tok0[r];
+        const int k = pos / page;
+        slot = (long long)page_at(r, k) * page + (pos - k * page);
+      }
+      a.slots[t] = slot;
+      a.positions[t] = pos;
+    } else {  // a page given back
+      const int b = (int)(e - n_kv - a.max_tokens);
+      const int r = find_owner(R, b, [&](int k) { return (long long)back0[k]; });
+      a.free_pages[(tail_at + b) % ring] = a.block_table[(long long)r * a.table_stride + (b - back0[r])];
+    }
+  }
+}
+
+}  // namespace
+
+int sm_count() {
+  static int count[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (count[dev] == 0 && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return count[dev];
+}
+char* error_text() {
+  static thread_local char text[kErrorBytes];
+  return text;
+}
+
+}  // namespace mk_serving
+
+extern "C" int mk_op_error(char* buf, int n) {
+  if (!buf || n <= 0) return MK_E_INVALID;
+  snprintf(buf, n, "%s", mk_serving::error_text());
+  return 0;
+}
+
+extern "C" int mk_plan_step(const mk_step_plan_args* args, void* stream) {
+  using namespace mk_serving;
+  if (!args) return fail(MK_E_INVALID, "plan_step: null arguments");
+  const mk_step_plan_args& a = *args;
+  if (!a.lengths || !a.new_tokens || !a.block_table || !a.free_pages || !a.free_range_in || !a.qo_indptr || !a.kv_indptr || !a.kv_indices ||
+      !a.last_page_len || !a.slots || !a.positions || !a.granted || !a.free_range_out)
+    return fail(MK_E_INVALID, "plan_step: null pointer");
+  if (a.requests < 1 || a.requests > MK_STEP_MAX_REQUESTS)
+    return fail(a.requests < 1 ? MK_E_INVALID : MK_E_TOO_LARGE, "plan_step: %d requests (1 to %d)", a.requests, MK_STEP_MAX_REQUESTS);
+  if (a.page_size < 1 || a.table_width < 1 || a.table_stride < a.table_width || a.max_tokens < 1 || a.max_indices < 1 || a.ring_size < 1)
+    return fail(MK_E_INVALID, "plan_step: sizes must be positive and table rows may not overlap");
+  if ((long long)a.requests * a.table_width > 0x7fffffffll) return fail(MK_E_TOO_LARGE, "plan_step: block table of over 2^31 entries");
+  const size_t smem = 4 * (size_t)(a.requests + 1) * sizeof(int);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return fail(MK_E_CUDA, "plan_step: %s", cudaGetErrorString(e));
+  }
+  const long long entries = (long long)a.max_indices + a.max_tokens;
+  const int ctas = (int)((entries + kPlanThreads - 1) / kPlanThreads);
+  PlanParams p{a};
+  step_plan_kernel<<<ctas < sm_count() ? ctas : sm_count(), kPlanThreads, smem, (cudaStream_t)stream>>>(p);
+  return launched("plan_step");
+}

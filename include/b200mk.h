@@ -198,6 +198,102 @@ int mk_tensor_read(mk_handle* h, int tensor_id, void* host_buf, int64_t bytes); 
 int mk_linear_static(const void* x, const void* w, const void* residual, void* out, int tokens, int n, int k,
                      void* stream);
 
+/* Operators of a serving step for hosts that keep the paging metadata themselves (mode online_notoken): what stands around the
+ * layers, and attention of chunks that are longer than a megakernel iteration.  No handle; every call enqueues its work on `stream`
+ * of the current device, allocates nothing and keeps nothing between calls, so calls on different streams and captured ones do not
+ * meet (each needs outputs and a workspace of its own).  Structures are read during the call only.  Strides count elements; the
+ * last dimension is contiguous.  Returns 0 or MK_E_*; mk_op_error gives the text of this thread's last refused call.  What device arrays
+ * say (index pointers, pages, slots) is not visible to the checks: the kernels hold it against the sizes given here. */
+int mk_op_error(char* buf, int n);
+
+#define MK_STEP_MAX_REQUESTS 8192
+
+/* Page allocation, block tables, index pointers and slot map of a step.  Request r has lengths[r] tokens in the cache, on the pages
+ * block_table[r, 0 .. ceil(length / page)), and is to be fed new_tokens[r]: 0 idle, -1 ended (its pages go back behind the ring's
+ * tail, first of all).  Free pages are free_pages[i % ring_size] for free_range[0] <= i < free_range[1].  Requests take pages and
+ * token rows in their order; one that cannot get all of them, or whose row of the table is too short, is granted nothing, and
+ * those behind it that need pages (or rows) neither.  Written: granted[r] (new tokens or 0), new pages into block_table, the
+ * index pointers, pages and last page lengths as the attention layers read them, cache slot (page * page_size + row) and
+ * position of every token row (-1 and 0 behind the last), and the free range behind the step.  lengths, new_tokens and
+ * free_range_in are left as they are: the same call again gives the same step. */
+typedef struct mk_step_plan_args {
+  const int32_t* lengths;        /* [requests] */
+  const int32_t* new_tokens;     /* [requests] */
+  int32_t* block_table;          /* [requests, table_width], rows table_stride apart */
+  int32_t* free_pages;           /* [ring_size] */
+  const int64_t* free_range_in;  /* [2] */
+  int32_t* qo_indptr;            /* [requests + 1] */
+  int32_t* kv_indptr;            /* [requests + 1] */
+  int32_t* kv_indices;           /* [max_indices] */
+  int32_t* last_page_len;        /* [requests] */
+  int64_t* slots;                /* [max_tokens] */
+  int32_t* positions;            /* [max_tokens] */
+  int32_t* granted;              /* [requests] */
+  int64_t* free_range_out;       /* [2], not free_range_in */
+  int64_t table_stride;
+  int32_t requests, table_width, ring_size, max_indices, max_tokens, page_size;
+} mk_step_plan_args;
+int mk_plan_step(const mk_step_plan_args* args, void* stream);
+
+/* QK norm (where q_norm / k_norm are given) and rotary embedding of rows q [tokens, q_heads, 128] and k [tokens, kv_heads, 128];
+ * q goes to out, k and v to the cache rows slots[t].  cos and sin: [table_rows, 128], row positions[t].  A token whose slot or
+ * position is outside is left out.  Slots may not repeat (two tokens would write one row). */
+typedef struct mk_rotate_append_args {
+  const void *q, *k, *v, *cos, *sin, *q_norm, *k_norm;
+  const int32_t* positions;
+  const int64_t* slots;
+  void *k_cache, *v_cache, *out;
+  int64_t q_stride[2], k_stride[2], v_stride[2], out_stride[2];  /* token, head */
+  int64_t table_stride[2];                                       /* row of cos, of sin */
+  int64_t k_cache_stride[3], v_cache_stride[3];                  /* page, row, head */
+  float eps;
+  int32_t dtype, table_dtype;                                    /* MK_BF16 or MK_F16; tables of the same type or MK_F32 */
+  int32_t tokens, q_heads, kv_heads, page_size, pages, table_rows;
+} mk_rotate_append_args;
+int mk_rotate_append(const mk_rotate_append_args* args, void* stream);
+
+/* Causal attention of the new tokens qo_indptr[r] <= t < qo_indptr[r + 1] of every request over its pages (the new tokens' K and V
+ * among them, as the last positions), head dimension 128.  window > 0: a row at position p sees positions above p - window and the
+ * first `sinks`.  Rows behind the last request are left as they are; a row that sees nothing is zero with lse minus infinity.
+ * lse (natural logarithm of the sum of weights) may be NULL.  max_new, if not 0, is the largest number of new tokens of a
+ * request as far as the host knows it: it chooses kernels, results do not depend on it.  mk_chunk_attention_workspace gives the
+ * bytes of the workspace of such a call, whatever its pointers are, or MK_E_*. */
+typedef struct mk_chunk_attention_args {
+  const void *q, *k_cache, *v_cache;
+  const int32_t *qo_indptr, *kv_indptr, *kv_indices, *last_page_len;
+  void* out;
+  float* lse;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_stride[2], out_stride[2], lse_stride[2];  /* token, head */
+  int64_t k_cache_stride[3], v_cache_stride[3];       /* page, row, head */
+  float scale;
+  int32_t dtype;                                      /* MK_BF16 or MK_F16 */
+  int32_t requests, tokens, q_heads, kv_heads, page_size, pages, num_indices, window, sinks, max_new;
+} mk_chunk_attention_args;
+int64_t mk_chunk_attention_workspace(const mk_chunk_attention_args* args);
+int mk_chunk_attention(const mk_chunk_attention_args* args, void* stream);
+
+/* A token per request from logits [rows, vocab] (row r, or with qo_indptr the request's last row; -1 where it has none or where no
+ * token can be chosen) and u[r] in [0, 1).  temperature 0: the largest logit, the lowest index on ties.  Otherwise top_k (0: off),
+ * then top_p (1: off) of what top_k leaves, and min_p (0: off) relative to the largest weight; the token is the first by
+ * index at which the running sum of kept weights exceeds u times their sum.  Settings are per request, or the values where the
+ * pointer is NULL.  logprobs (may be NULL): logarithm of the probability with which the token was drawn. */
+typedef struct mk_sample_args {
+  const void* logits;
+  const int32_t* qo_indptr;
+  const float *u, *temperature, *top_p, *min_p;
+  const int32_t* top_k;
+  int64_t* tokens;
+  float* logprobs;
+  int64_t row_stride;
+  float temperature_value, top_p_value, min_p_value;
+  int32_t top_k_value;
+  int32_t dtype;                                      /* MK_BF16, MK_F16 or MK_F32 */
+  int32_t requests, rows, vocab;
+} mk_sample_args;
+int mk_sample_tokens(const mk_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
