@@ -21,7 +21,7 @@ REPORT = os.path.join(OBJDIR, "instances.json")  # what ptxas made of every kern
 # is compiled once per linear path that its programs take (MK_NC, see mk_launch.cu)
 SOURCES = {"mk_kernel.cu": (0, 8, 16, 32), "mk_kernel_tp.cu": (0, 8, 16, 32), "mk_kernel_hier.cu": (0, 8, 16, 32), "mk_kernel_moe.cu": (0,),
            "mk_launch.cu": None, "mk_runtime.cpp": None, "mk_noalloc.cu": None,
-           "mk_step_plan.cu": None, "mk_rotate_append.cu": None, "mk_chunk_attention.cu": None, "mk_sample.cu": None}
+           "mk_step_plan.cu": None, "mk_rotate_append.cu": None, "mk_chunk_attention.cu": None, "mk_chunk_attention_tiles.cu": None, "mk_sample.cu": None}
 HEADERS = ["mk_types.h", "mk_wide.cuh", "mk_serving.cuh", "mk_chunk_attention.cuh", os.path.join("..", "..", "include", "b200mk.h")]
 
 

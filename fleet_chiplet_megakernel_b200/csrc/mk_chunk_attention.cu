@@ -142,43 +142,15 @@ template <typename T, int NT> struct RowWarp {
     return c.q.q0 + tok;
   }
 
-  // The piece again, a row and a position at a time: sums that are not finite reach only the rows that see their cause.
+  // The piece again, a row and a position at a time.
   __device__ __noinline__ void exactly(const Cursor& c, int k0) const {
     const mk_chunk_attention_args& a = p.a;
+    Span<kPos> span(a, c.p0, c.p1);
     for (int row = 0; row < c.rows; ++row) {
       int head;
       const long long tok = row_token(c, row, &head);
-      const int at = c.q.len - c.q.n + (c.row0 + row) / p.per_kv;
-      const T* qr = (const T*)a.q + tok * a.q_stride[0] + head * a.q_stride[1] + 4 * lane;
-      float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
-#pragma unroll
-      for (int d = 0; d < 4; ++d) q[d] = to_float(qr[d]);
-      for (int i = k0; i < min(c.k_end, c.count); ++i)
-        for (int j = c.position(i); j < c.position(i) + kPos; ++j) {
-          if (!sees(a, j, at)) continue;
-          int page, in;
-          locate(p, c.q, j, &page, &in);
-          float s = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-          if (page >= 0) {
-            const T* kr = (const T*)a.k_cache + (long long)page * a.k_cache_stride[0] + (long long)in * a.k_cache_stride[1] + c.kv_head * a.k_cache_stride[2] + 4 * lane;
-            const T* vr = (const T*)a.v_cache + (long long)page * a.v_cache_stride[0] + (long long)in * a.v_cache_stride[1] + c.kv_head * a.v_cache_stride[2] + 4 * lane;
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              s += q[d] * to_float(kr[d]);
-              v[d] = to_float(vr[d]);
-            }
-          }
-#pragma unroll
-          for (int o2 = 16; o2 > 0; o2 >>= 1) s += __shfl_xor_sync(kAll, s, o2);
-          s *= p.scale_log2;
-          if (s == -INFINITY) continue;
-          const float mn = s > m ? s : m;  // (a NaN score leaves the maximum and enters the weight)
-          const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - (mn == -INFINITY ? 0.f : mn));
-          l = l * alpha + w;
-#pragma unroll
-          for (int d = 0; d < 4; ++d) o[d] = o[d] * alpha + w * v[d];
-          m = mn;
-        }
+      float o[4], m, l;
+      exact_row<T, kPos>(p, c.q, span, k0, c.k_end, c.q.len - c.q.n + (c.row0 + row) / p.per_kv, tok, head, c.kv_head, o, m, l);
       if (c.from_start && c.to_end) {
         T* dst = (T*)a.out + tok * a.out_stride[0] + head * a.out_stride[1] + 4 * lane;
 #pragma unroll
@@ -520,20 +492,32 @@ template <typename T, int NT> int launch_rows(const AttnParams& p, cudaStream_t 
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "chunk_attention: launch failed: %s", cudaGetErrorString(e));
 }
 
-// What a call needs of the workspace; the host's choices of kernels stand here once.
+// Which kernels a call takes and what it needs of the workspace.
+constexpr int kFewRows = 32;
 struct Layout {
-  int nt, warps;
-  size_t plan, partial, bytes;
+  bool rows, tiles;
+  int nt, few_rows, warps, splits;
+  size_t partial, tile_partial, bytes;
 };
 Layout layout_of(const mk_chunk_attention_args& a) {
-  Layout l;
+  Layout l = {};
   const int per_kv = a.q_heads / a.kv_heads;
-  const long long most = a.max_new > 0 ? a.max_new : a.tokens;
+  const long long most = a.max_new > 0 && a.max_new < a.tokens ? a.max_new : a.tokens;
+  l.tiles = most * per_kv > kFewRows && tiles_take(a);
+  l.rows = !l.tiles || a.requests > 1;
+  l.few_rows = !l.tiles ? 0x7fffffff : l.rows ? kFewRows : 0;
   l.nt = most * per_kv <= 8 ? 1 : 2;
   l.warps = sm_count() * kRowWarps;
-  l.plan = 0;
-  l.partial = ((size_t)(a.requests + 2) * 8 + 255) / 256 * 256;
-  l.bytes = l.partial + (size_t)2 * l.warps * part_floats(8 * l.nt) * sizeof(float);
+  l.splits = 1;
+  if (l.tiles) {
+    const long long tokens = 2 * (128 / per_kv), ctas = (a.tokens + tokens - 1) / tokens * a.kv_heads;
+    while (l.splits < 16 && 2 * l.splits * ctas <= sm_count()) l.splits *= 2;
+  }
+  const size_t plan = ((size_t)(a.requests + 2) * 8 + 255) / 256 * 256;
+  l.partial = l.rows ? plan : 0;
+  l.tile_partial = l.partial + (l.rows ? (size_t)2 * l.warps * part_floats(8 * l.nt) * sizeof(float) : 0);
+  l.bytes = l.tile_partial + (l.splits > 1 ? (size_t)l.splits * a.tokens * a.q_heads * (kHeadDim + 2) * sizeof(float) : 0);
+  if (l.bytes == 0) l.bytes = 16;
   return l;
 }
 
@@ -546,7 +530,7 @@ int check(const mk_chunk_attention_args& a) {
   if (a.q_heads % a.kv_heads) return fail(MK_E_INVALID, "chunk_attention: %d q heads on %d kv heads", a.q_heads, a.kv_heads);
   if (a.requests < 1 || a.requests > kMaxRequests)
     return fail(a.requests < 1 ? MK_E_INVALID : MK_E_TOO_LARGE, "chunk_attention: %d requests (1 to %d)", a.requests, kMaxRequests);
-  if ((long long)a.tokens * a.q_heads > 0x3fffffffll || a.kv_heads > 65535) return fail(MK_E_TOO_LARGE, "chunk_attention: too many rows");
+  if ((long long)a.tokens * a.q_heads > 0x3fffffffll || (long long)a.requests * a.kv_heads > 0x3fffffffll || a.kv_heads > 65535) return fail(MK_E_TOO_LARGE, "chunk_attention: too many rows");
   if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out)) return fail(MK_E_INVALID, "chunk_attention: pointers must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     if ((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7) return fail(MK_E_INVALID, "chunk_attention: rows of the caches must start at multiples of 16 bytes");
@@ -583,10 +567,15 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   p.scale_log2 = a.scale * kLog2e;
   p.warps = l.warps;
   p.min_tiles = 4;
-  p.plan = reinterpret_cast<long long*>((char*)a.workspace + l.plan);
+  p.plan = reinterpret_cast<long long*>(a.workspace);
   p.partial = reinterpret_cast<float*>((char*)a.workspace + l.partial);
-  p.few_rows = 0x7fffffff;
+  p.few_rows = l.few_rows;
+  p.splits = l.splits;
+  p.tile_partial = reinterpret_cast<float*>((char*)a.workspace + l.tile_partial);
   const cudaStream_t s = (cudaStream_t)stream;
+  if (l.tiles)
+    if (int rc = launch_tile_attention(p, s)) return rc;
+  if (!l.rows) return 0;
   if (a.dtype == MK_BF16) return l.nt == 1 ? launch_rows<__nv_bfloat16, 1>(p, s) : launch_rows<__nv_bfloat16, 2>(p, s);
   return l.nt == 1 ? launch_rows<__half, 1>(p, s) : launch_rows<__half, 2>(p, s);
 }

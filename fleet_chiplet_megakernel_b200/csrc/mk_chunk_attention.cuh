@@ -71,7 +71,54 @@ template <int TILE> struct Span {
   __device__ __forceinline__ int position(int k) const { return k < sink ? k * TILE : start + (k - sink) * TILE; }
 };
 
-int launch_tile_attention(const AttnParams& p, cudaStream_t s);  // mk_chunk_attention_tiles.cu
+// One row over the tiles k0 <= k < k1 of a span, a position at a time and only those that the row sees, by a warp: lane l has dims
+// 4 l .. 4 l + 3.  For pieces whose products were not finite: a product with weight 0 is not 0 there, so a value that is not finite
+// would reach rows that do not see it.
+template <typename T, int TILE>
+__device__ __noinline__ void exact_row(const AttnParams& p, const Request& q, const Span<TILE>& span, int k0, int k1, int at, long long tok, int head, int kv_head,
+                                       float (&o)[4], float& m, float& l) {
+  const mk_chunk_attention_args& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const T* qr = (const T*)a.q + tok * a.q_stride[0] + head * a.q_stride[1] + 4 * lane;
+  float x[4];
+#pragma unroll
+  for (int d = 0; d < 4; ++d) {
+    x[d] = to_float(qr[d]);
+    o[d] = 0.f;
+  }
+  m = -INFINITY;
+  l = 0.f;
+  for (int i = k0; i < min(k1, span.count); ++i)
+    for (int j = span.position(i); j < span.position(i) + TILE; ++j) {
+      if (!sees(a, j, at)) continue;
+      int page, in;
+      locate(p, q, j, &page, &in);
+      float s = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+      if (page >= 0) {
+        const T* kr = (const T*)a.k_cache + (long long)page * a.k_cache_stride[0] + (long long)in * a.k_cache_stride[1] + kv_head * a.k_cache_stride[2] + 4 * lane;
+        const T* vr = (const T*)a.v_cache + (long long)page * a.v_cache_stride[0] + (long long)in * a.v_cache_stride[1] + kv_head * a.v_cache_stride[2] + 4 * lane;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          s += x[d] * to_float(kr[d]);
+          v[d] = to_float(vr[d]);
+        }
+      }
+#pragma unroll
+      for (int e = 16; e > 0; e >>= 1) s += __shfl_xor_sync(kAll, s, e);
+      s *= p.scale_log2;
+      if (s == -INFINITY) continue;
+      const float mn = s > m ? s : m;  // (a NaN score leaves the maximum and enters the weight)
+      const float alpha = m == -INFINITY ? 0.f : exp2f(m - mn), w = exp2f(s - (mn == -INFINITY ? 0.f : mn));
+      l = l * alpha + w;
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[d] = o[d] * alpha + w * v[d];
+      m = mn;
+    }
+}
+
+// mk_chunk_attention_tiles.cu: whether the tile kernel takes such tensors at all, and its launch
+bool tiles_take(const mk_chunk_attention_args& a);
+int launch_tile_attention(const AttnParams& p, cudaStream_t s);
 
 }  // namespace mk_serving
 
