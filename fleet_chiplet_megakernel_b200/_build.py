@@ -3,6 +3,7 @@
 ``python -m fleet_chiplet_megakernel_b200._build`` or ``build()`` compiles the
 CUDA sources for sm_100a into ``libb200mk.so`` next to this file.  The built
 library is what the package loads; there is no fallback when it is missing.
+Beside it stands ``_serving_native.so``, the binding of the serving operators.
 """
 import json
 import os
@@ -10,11 +11,14 @@ import re
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libb200mk.so")
+BINDING = os.path.join(HERE, "_serving_native.so")  # the serving operators as Python functions (serving.py)
+BINDING_SOURCE = "mk_binding.cpp"
 OBJDIR = os.path.join(HERE, "build")
 REPORT = os.path.join(OBJDIR, "instances.json")  # what ptxas made of every kernel instance
 # mk_kernel_tp.cu, mk_kernel_hier.cu and mk_kernel_moe.cu include mk_kernel.cu with other build switches (see its header); each
@@ -33,10 +37,10 @@ def _nvcc():
 
 
 def needs_build():
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(BINDING):
         return True
-    t = os.path.getmtime(LIB)
-    deps = [os.path.join(CSRC, s) for s in list(SOURCES) + HEADERS]
+    t = min(os.path.getmtime(LIB), os.path.getmtime(BINDING))
+    deps = [os.path.join(CSRC, s) for s in list(SOURCES) + HEADERS + [BINDING_SOURCE]]
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
@@ -58,6 +62,18 @@ def check_registers(instances):
         raise RuntimeError(f"kernel instances with fewer than {need} registers a thread: {few}")
 
 
+def binding_command():
+    """The binding is compiled against the torch that runs it (its headers, its C++ ABI) and linked with torch alone."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    lib = os.path.join(root, "lib")
+    include = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+               os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] +
+            [f"-I{i}" for i in include] + [os.path.join(CSRC, BINDING_SOURCE), "-o", BINDING, f"-L{lib}"] +
+            [f"-l{n}" for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python")])
+
+
 def build(force=False, verbose=False):
     if not force and not needs_build():
         return LIB
@@ -70,6 +86,7 @@ def build(force=False, verbose=False):
             obj = os.path.join(OBJDIR, stem + ("" if nc is None else f"_{nc}") + ".o")
             define = [] if nc is None else [f"-DMK_NC={nc}"]
             jobs.append(([_nvcc()] + flags + define + ["-c", os.path.join(CSRC, src), "-o", obj], obj))
+    jobs.append((binding_command(), None))
     # one nvcc per object, as many side by side as there are cores, then one link
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as pool:
         done = list(pool.map(lambda job: subprocess.run(job[0], stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True), jobs))
@@ -79,13 +96,15 @@ def build(force=False, verbose=False):
             sys.stdout.write(" ".join(cmd) + "\n" + r.stdout)
         if r.returncode != 0:
             raise subprocess.CalledProcessError(r.returncode, cmd)
+        if obj is None:
+            continue
         name = os.path.splitext(os.path.basename(obj))[0]
         if name.startswith("mk_kernel"):
             instances[name] = resources(r.stdout)
     check_registers(instances)
     with open(REPORT, "w") as f:
         json.dump(instances, f, indent=1)
-    objs = [obj for _, obj in jobs]
+    objs = [obj for _, obj in jobs if obj is not None]
     subprocess.check_call([_nvcc(), "-shared", "-o", LIB] + objs)
     return LIB
 

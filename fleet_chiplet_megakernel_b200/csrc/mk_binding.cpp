@@ -1,0 +1,356 @@
+// The serving operators as Python functions: checks of the tensors, outputs and workspaces from torch's allocator, the C entry point on
+// the current stream of the tensors' device.  A call of these takes a few microseconds of host time where the same checks in
+// Python and ctypes take 30 to 50, several times what the smaller kernels run.
+//
+// The entry points are those of the library that the package has loaded (bind()); this module is linked with none of it.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
+#include <ATen/ops/zeros.h>
+#include <c10/core/GradMode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+
+#include "../../include/b200mk.h"
+
+namespace {
+
+constexpr int64_t kHeadDim = 128;
+constexpr int64_t kMaxInt = 0x7fffffff;
+
+struct {
+  decltype(&mk_plan_step) plan_step;
+  decltype(&mk_rotate_append) rotate_append;
+  decltype(&mk_chunk_attention_workspace) attention_workspace;
+  decltype(&mk_chunk_attention) attention;
+  decltype(&mk_sample_tokens) sample;
+  decltype(&mk_op_error) error;
+} g_lib;
+
+void need(bool ok, const char* what, const char* msg) {
+  if (!ok) TORCH_CHECK_VALUE(false, what, msg);
+}
+// A status of the library as the exceptions of PersistentKernel.
+void status(int64_t rc) {
+  if (rc >= 0) return;
+  char text[512] = "";
+  g_lib.error(text, sizeof text);
+  if (rc == MK_E_UNSUPPORTED || rc == MK_E_TOO_LARGE) TORCH_CHECK_NOT_IMPLEMENTED(false, text);
+  if (rc == MK_E_INVALID) TORCH_CHECK_VALUE(false, text);
+  TORCH_CHECK(false, text);
+}
+
+const at::Tensor& tensor(PyObject* o, const char* what) {
+  need(THPVariable_Check(o), what, ": a tensor is needed");
+  return THPVariable_Unpack(o);
+}
+const at::Tensor* maybe(PyObject* o, const char* what) { return o == Py_None ? nullptr : &tensor(o, what); }
+int64_t number(PyObject* o, const char* what, int64_t lo, int64_t hi) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  if (v < lo || v > hi) TORCH_CHECK_VALUE(false, what, ": ", v, ", ", lo, " to ", hi, " is allowed");
+  return v;
+}
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+
+struct Checks {
+  c10::Device device;
+  explicit Checks(const at::Tensor& t, const char* what) : device(t.device()) {
+    need(t.is_cuda(), what, " must be a CUDA tensor; there is no CPU fallback");
+    no_gradient(t, what);
+  }
+  static void no_gradient(const at::Tensor& t, const char* what) {
+    need(!t.requires_grad() || !c10::GradMode::is_enabled(), what, " requires a gradient and the serving operators have none: call them under torch.no_grad()");
+  }
+  void here(const at::Tensor& t, const char* what) const {
+    if (t.device() != device) TORCH_CHECK_VALUE(false, what, " is on ", t.device(), ", the first tensor on ", device);
+    need(t.layout() == at::kStrided, what, ": a strided tensor is needed");
+    no_gradient(t, what);
+  }
+  void type(const at::Tensor& t, const char* what, at::ScalarType dt) const {
+    here(t, what);
+    if (t.scalar_type() != dt) TORCH_CHECK_VALUE(false, what, ".dtype: ", t.scalar_type(), ", ", dt, " is needed");
+  }
+  // one dimension of n entries (n < 0: of any number), contiguous
+  template <typename P = void> P* list(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t n) const {
+    type(t, what, dt);
+    if (t.dim() != 1 || (n >= 0 && t.size(0) != n)) TORCH_CHECK_VALUE(false, what, ".shape: ", t.sizes(), ", one dimension", n >= 0 ? " of " + std::to_string(n) : std::string(), " is needed");
+    need(t.is_contiguous(), what, " must be contiguous");
+    if (t.size(0) > kMaxInt) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": over 2^31 entries");
+    return static_cast<P*>(t.data_ptr());
+  }
+  // [tokens, heads, 128], any token and head stride
+  void* rows(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t tokens, int64_t heads, int64_t* stride) const {
+    type(t, what, dt);
+    if (t.dim() != 3 || t.size(2) != kHeadDim || (tokens >= 0 && t.size(0) != tokens) || (heads >= 0 && t.size(1) != heads))
+      TORCH_CHECK_VALUE(false, what, ".shape: ", t.sizes(), ", [", tokens >= 0 ? std::to_string(tokens) : "tokens", ", ", heads >= 0 ? std::to_string(heads) : "heads", ", 128] is needed");
+    need(t.stride(2) == 1, what, ": the elements of a row must be contiguous");
+    if (t.size(0) > kMaxInt || t.size(1) > kMaxInt) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": over 2^31 rows");
+    stride[0] = t.stride(0);
+    stride[1] = t.stride(1);
+    return t.data_ptr();
+  }
+  void* cache(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t* stride) const {
+    type(t, what, dt);
+    if (t.dim() != 4 || t.size(3) != kHeadDim || t.numel() == 0) TORCH_CHECK_VALUE(false, what, ".shape: ", t.sizes(), ", [pages, page_size, kv_heads, 128] is needed");
+    need(t.stride(3) == 1, what, ": the elements of a row must be contiguous");
+    for (int i = 0; i < 3; ++i) {
+      if (t.size(i) > kMaxInt) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": over 2^31 pages or rows");
+      stride[i] = t.stride(i);
+    }
+    return t.data_ptr();
+  }
+  // Rows that are written may not share memory, as those of an expanded tensor do.
+  static void apart(const at::Tensor& t, const char* what) {
+    const int n = (int)t.dim() - 1;
+    int64_t reach = kHeadDim;
+    bool done[4] = {};
+    for (int k = 0; k < n; ++k) {
+      int best = -1;
+      for (int i = 0; i < n; ++i)
+        if (!done[i] && (best < 0 || t.stride(i) < t.stride(best))) best = i;
+      done[best] = true;
+      if (t.size(best) <= 1) continue;
+      need(t.stride(best) >= reach, what, ": its rows share memory");
+      reach += t.stride(best) * (t.size(best) - 1);
+    }
+  }
+};
+at::ScalarType row_type(const at::Tensor& t, const char* what) {
+  if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf) TORCH_CHECK_VALUE(false, what, ".dtype: ", t.scalar_type(), ", bf16 or fp16 is needed");
+  return t.scalar_type();
+}
+int code(at::ScalarType t) { return t == at::kBFloat16 ? MK_BF16 : t == at::kHalf ? MK_F16 : MK_F32; }
+at::Tensor new_rows(int64_t tokens, int64_t heads, const at::Tensor& like) { return at::zeros({tokens, heads, kHeadDim}, like.options().requires_grad(false)); }
+void count(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK(n == want, "wrong number of arguments"); }
+
+PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 6);
+  auto at = [&](int i) { return PyLong_AsVoidPtr(v[i]); };
+  g_lib.plan_step = reinterpret_cast<decltype(g_lib.plan_step)>(at(0));
+  g_lib.rotate_append = reinterpret_cast<decltype(g_lib.rotate_append)>(at(1));
+  g_lib.attention_workspace = reinterpret_cast<decltype(g_lib.attention_workspace)>(at(2));
+  g_lib.attention = reinterpret_cast<decltype(g_lib.attention)>(at(3));
+  g_lib.sample = reinterpret_cast<decltype(g_lib.sample)>(at(4));
+  g_lib.error = reinterpret_cast<decltype(g_lib.error)>(at(5));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* plan_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 14);
+  mk_step_plan_args a = {};
+  const at::Tensor& lengths = tensor(v[0], "lengths");
+  const Checks c(lengths, "lengths");
+  a.lengths = c.list<int32_t>(lengths, "lengths", at::kInt, -1);
+  const int64_t R = lengths.size(0);
+  need(R > 0, "lengths", ": a length per request is needed");
+  a.new_tokens = c.list<int32_t>(tensor(v[1], "new_tokens"), "new_tokens", at::kInt, R);
+  const at::Tensor& table = tensor(v[2], "block_table");
+  c.type(table, "block_table", at::kInt);
+  if (table.dim() != 2 || table.size(0) != R || table.size(1) < 1 || table.size(1) > kMaxInt) TORCH_CHECK_VALUE(false, "block_table.shape: ", table.sizes(), ", [", R, ", pages of the longest request] is needed");
+  need(table.stride(1) == 1 && (R == 1 || table.stride(0) >= table.size(1)), "block_table", ": rows must be contiguous and apart");
+  a.block_table = static_cast<int32_t*>(table.data_ptr());
+  a.table_width = (int32_t)table.size(1);
+  a.table_stride = R == 1 ? table.size(1) : table.stride(0);
+  const at::Tensor& ring = tensor(v[3], "free_pages");
+  a.free_pages = c.list<int32_t>(ring, "free_pages", at::kInt, -1);
+  a.free_range_in = c.list<int64_t>(tensor(v[4], "free_range"), "free_range", at::kLong, 2);
+  a.page_size = (int32_t)number(v[5], "page_size", 1, kMaxInt);
+  a.qo_indptr = c.list<int32_t>(tensor(v[6], "plan.qo_indptr"), "plan.qo_indptr", at::kInt, R + 1);
+  a.kv_indptr = c.list<int32_t>(tensor(v[7], "plan.kv_indptr"), "plan.kv_indptr", at::kInt, R + 1);
+  const at::Tensor& indices = tensor(v[8], "plan.kv_indices");
+  a.kv_indices = c.list<int32_t>(indices, "plan.kv_indices", at::kInt, -1);
+  a.last_page_len = c.list<int32_t>(tensor(v[9], "plan.last_page_len"), "plan.last_page_len", at::kInt, R);
+  const at::Tensor& slots = tensor(v[10], "plan.slots");
+  a.slots = c.list<int64_t>(slots, "plan.slots", at::kLong, -1);
+  a.positions = c.list<int32_t>(tensor(v[11], "plan.positions"), "plan.positions", at::kInt, slots.size(0));
+  a.granted = c.list<int32_t>(tensor(v[12], "plan.granted"), "plan.granted", at::kInt, R);
+  a.free_range_out = c.list<int64_t>(tensor(v[13], "plan.free_range"), "plan.free_range", at::kLong, 2);
+  need(a.free_range_out != a.free_range_in, "plan.free_range", " may not be free_range: the call reads one and writes the other");
+  a.requests = (int32_t)std::min(R, kMaxInt);
+  a.ring_size = (int32_t)ring.size(0);
+  a.max_indices = (int32_t)indices.size(0);
+  a.max_tokens = (int32_t)slots.size(0);
+  const c10::cuda::CUDAGuard guard(c.device);
+  status(g_lib.plan_step(&a, at::cuda::getCurrentCUDAStream().stream()));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* rotate_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 13);
+  mk_rotate_append_args a = {};
+  const at::Tensor& q = tensor(v[0], "q");
+  const Checks c(q, "q");
+  const at::ScalarType dt = row_type(q, "q");
+  a.q = c.rows(q, "q", dt, -1, -1, a.q_stride);
+  const at::Tensor& k = tensor(v[1], "k");
+  const int64_t T = q.size(0), n_q = q.size(1);
+  a.k = c.rows(k, "k", dt, T, -1, a.k_stride);
+  const int64_t n_kv = k.size(1);
+  a.v = c.rows(tensor(v[2], "v"), "v", dt, T, n_kv, a.v_stride);
+  const at::Tensor &cos = tensor(v[3], "cos"), &sin = tensor(v[4], "sin");
+  for (const at::Tensor* t : {&cos, &sin}) {
+    const char* what = t == &cos ? "cos" : "sin";
+    c.here(*t, what);
+    if (t->dim() != 2 || t->size(1) != kHeadDim || t->size(0) < 1 || t->size(0) > kMaxInt || t->stride(1) != 1 || t->sizes() != cos.sizes())
+      TORCH_CHECK_VALUE(false, what, ".shape: ", t->sizes(), ", [positions, 128] with contiguous rows, cos and sin alike, is needed");
+    if ((t->scalar_type() != dt && t->scalar_type() != at::kFloat) || t->scalar_type() != cos.scalar_type())
+      TORCH_CHECK_VALUE(false, what, ".dtype: ", t->scalar_type(), ", ", dt, " or fp32, cos and sin alike, is needed");
+  }
+  a.cos = cos.data_ptr();
+  a.sin = sin.data_ptr();
+  a.table_stride[0] = cos.stride(0);
+  a.table_stride[1] = sin.stride(0);
+  a.positions = c.list<int32_t>(tensor(v[5], "positions"), "positions", at::kInt, T);
+  a.slots = c.list<int64_t>(tensor(v[6], "slots"), "slots", at::kLong, T);
+  const at::Tensor &kc = tensor(v[7], "k_cache"), &vc = tensor(v[8], "v_cache");
+  a.k_cache = c.cache(kc, "k_cache", dt, a.k_cache_stride);
+  a.v_cache = c.cache(vc, "v_cache", dt, a.v_cache_stride);
+  if (kc.size(2) != n_kv || vc.sizes() != kc.sizes()) TORCH_CHECK_VALUE(false, "caches of shape ", kc.sizes(), " and ", vc.sizes(), " for ", n_kv, " kv heads");
+  Checks::apart(kc, "k_cache");
+  Checks::apart(vc, "v_cache");
+  if (const at::Tensor* t = maybe(v[9], "q_norm")) a.q_norm = c.list(*t, "q_norm", dt, kHeadDim);
+  if (const at::Tensor* t = maybe(v[10], "k_norm")) a.k_norm = c.list(*t, "k_norm", dt, kHeadDim);
+  a.eps = (float)real(v[11]);
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor out = v[12] == Py_None ? new_rows(T, n_q, q) : tensor(v[12], "out");
+  a.out = c.rows(out, "out", dt, T, n_q, a.out_stride);
+  Checks::apart(out, "out");
+  a.dtype = code(dt);
+  a.table_dtype = code(cos.scalar_type());
+  a.tokens = (int32_t)T;
+  a.q_heads = (int32_t)n_q;
+  a.kv_heads = (int32_t)n_kv;
+  a.pages = (int32_t)kc.size(0);
+  a.page_size = (int32_t)kc.size(1);
+  a.table_rows = (int32_t)cos.size(0);
+  if (T > 0) status(g_lib.rotate_append(&a, at::cuda::getCurrentCUDAStream().stream()));
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* chunk_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 13);
+  mk_chunk_attention_args a = {};
+  const at::Tensor& q = tensor(v[0], "q");
+  const Checks c(q, "q");
+  const at::ScalarType dt = row_type(q, "q");
+  a.q = c.rows(q, "q", dt, -1, -1, a.q_stride);
+  const int64_t T = q.size(0), n_q = q.size(1);
+  const at::Tensor &kc = tensor(v[1], "k_cache"), &vc = tensor(v[2], "v_cache");
+  a.k_cache = c.cache(kc, "k_cache", dt, a.k_cache_stride);
+  a.v_cache = c.cache(vc, "v_cache", dt, a.v_cache_stride);
+  if (vc.sizes() != kc.sizes()) TORCH_CHECK_VALUE(false, "k_cache is ", kc.sizes(), ", v_cache ", vc.sizes());
+  const int64_t n_kv = kc.size(2);
+  if (n_q % n_kv) TORCH_CHECK_VALUE(false, n_q, " q heads on ", n_kv, " kv heads");
+  const at::Tensor& last = tensor(v[6], "last_page_len");
+  a.last_page_len = c.list<int32_t>(last, "last_page_len", at::kInt, -1);
+  const int64_t R = last.size(0);
+  a.qo_indptr = c.list<int32_t>(tensor(v[3], "qo_indptr"), "qo_indptr", at::kInt, R + 1);
+  a.kv_indptr = c.list<int32_t>(tensor(v[4], "kv_indptr"), "kv_indptr", at::kInt, R + 1);
+  const at::Tensor& indices = tensor(v[5], "kv_indices");
+  a.kv_indices = c.list<int32_t>(indices, "kv_indices", at::kInt, -1);
+  a.scale = v[7] == Py_None ? (float)(1.0 / std::sqrt((double)kHeadDim)) : (float)real(v[7]);
+  a.window = (int32_t)number(v[8], "window", 0, kMaxInt);
+  a.sinks = (int32_t)number(v[9], "sinks", 0, kMaxInt);
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor out = v[10] == Py_None ? new_rows(T, n_q, q) : tensor(v[10], "out");
+  a.out = c.rows(out, "out", dt, T, n_q, a.out_stride);
+  Checks::apart(out, "out");
+  need(a.out != a.q || T * n_q == 0, "out", " may not be q");
+  if (const at::Tensor* t = maybe(v[11], "lse")) {
+    c.type(*t, "lse", at::kFloat);
+    if (t->dim() != 2 || t->size(0) != T || t->size(1) != n_q) TORCH_CHECK_VALUE(false, "lse.shape: ", t->sizes(), ", [", T, ", ", n_q, "] is needed");
+    a.lse = static_cast<float*>(t->data_ptr());
+    a.lse_stride[0] = t->stride(0);
+    a.lse_stride[1] = t->stride(1);
+  }
+  a.max_new = (int32_t)number(v[12], "max_new", 0, kMaxInt);
+  a.dtype = code(dt);
+  a.requests = (int32_t)R;
+  a.tokens = (int32_t)T;
+  a.q_heads = (int32_t)n_q;
+  a.kv_heads = (int32_t)n_kv;
+  a.page_size = (int32_t)kc.size(1);
+  a.pages = (int32_t)kc.size(0);
+  a.num_indices = (int32_t)indices.size(0);
+  if (T > 0 && R > 0 && n_q > 0) {
+    a.workspace_bytes = g_lib.attention_workspace(&a);
+    status(a.workspace_bytes);
+    // of the current stream's pool, or of the graph that captures the call
+    const at::Tensor workspace = at::empty({a.workspace_bytes}, q.options().dtype(at::kByte).requires_grad(false));
+    a.workspace = workspace.data_ptr();
+    status(g_lib.attention(&a, at::cuda::getCurrentCUDAStream().stream()));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* sample_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 9);
+  mk_sample_args a = {};
+  const at::Tensor& logits = tensor(v[0], "logits");
+  const Checks c(logits, "logits");
+  const at::ScalarType dt = logits.scalar_type();
+  if (dt != at::kBFloat16 && dt != at::kHalf && dt != at::kFloat) TORCH_CHECK_VALUE(false, "logits.dtype: ", dt, ", bf16, fp16 or fp32 is needed");
+  if (logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > kMaxInt || logits.size(0) > kMaxInt) TORCH_CHECK_VALUE(false, "logits.shape: ", logits.sizes(), ", [rows, vocab] is needed");
+  need(logits.stride(1) == 1 || logits.size(1) == 1, "logits", ": the elements of a row must be contiguous");
+  const at::Tensor& u = tensor(v[1], "u");
+  a.u = c.list<float>(u, "u", at::kFloat, -1);
+  const int64_t R = u.size(0);
+  if (THPVariable_Check(v[2])) a.temperature = c.list<float>(tensor(v[2], "temperature"), "temperature", at::kFloat, R);
+  else a.temperature_value = (float)real(v[2]);
+  if (THPVariable_Check(v[3])) a.top_k = c.list<int32_t>(tensor(v[3], "top_k"), "top_k", at::kInt, R);
+  else a.top_k_value = (int32_t)number(v[3], "top_k", -kMaxInt, kMaxInt);
+  if (THPVariable_Check(v[4])) a.top_p = c.list<float>(tensor(v[4], "top_p"), "top_p", at::kFloat, R);
+  else a.top_p_value = (float)real(v[4]);
+  if (THPVariable_Check(v[5])) a.min_p = c.list<float>(tensor(v[5], "min_p"), "min_p", at::kFloat, R);
+  else a.min_p_value = (float)real(v[5]);
+  if (const at::Tensor* t = maybe(v[6], "qo_indptr")) a.qo_indptr = c.list<int32_t>(*t, "qo_indptr", at::kInt, R + 1);
+  else if (logits.size(0) < R) TORCH_CHECK_VALUE(false, logits.size(0), " rows of logits for ", R, " requests");
+  const c10::cuda::CUDAGuard guard(c.device);
+  at::Tensor out = v[7] == Py_None ? at::empty({R}, logits.options().dtype(at::kLong).requires_grad(false)) : tensor(v[7], "out");
+  a.tokens = c.list<int64_t>(out, "out", at::kLong, R);
+  const bool with_logprobs = v[8] == Py_True;
+  at::Tensor logprobs;
+  if (with_logprobs) {
+    logprobs = at::empty({R}, logits.options().dtype(at::kFloat).requires_grad(false));
+    a.logprobs = static_cast<float*>(logprobs.data_ptr());
+  }
+  a.logits = logits.data_ptr();
+  a.row_stride = logits.stride(0);
+  a.dtype = code(dt);
+  a.requests = (int32_t)R;
+  a.rows = (int32_t)logits.size(0);
+  a.vocab = (int32_t)logits.size(1);
+  if (R > 0) status(g_lib.sample(&a, at::cuda::getCurrentCUDAStream().stream()));
+  if (!with_logprobs) return THPVariable_Wrap(std::move(out));
+  PyObject* pair = PyTuple_New(2);
+  if (!pair) throw python_error();
+  PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+  PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(logprobs)));
+  return pair;
+  END_HANDLE_TH_ERRORS
+}
+
+#define MK_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
+PyMethodDef g_methods[] = {MK_METHOD(bind), MK_METHOD(plan_step), MK_METHOD(rotate_append), MK_METHOD(chunk_attention), MK_METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
+PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_serving_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__serving_native() { return PyModule_Create(&g_module); }
