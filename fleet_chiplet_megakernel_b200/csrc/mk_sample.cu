@@ -9,12 +9,18 @@
 // A token is a whole number: with sums in fp32 one draw in some thousands would fall on the neighbour's side of a border.  Weights
 // and their sums are therefore 64-bit, and every sum has one fixed order (no atomics on anything but counts).
 //
-// A row is taken by a cluster of up to 8 CTAs, as many as leave the SMs busy; each has a contiguous part of the vocabulary and
-// reads it a few times, from L2 after the first.  The border is found by counting: a histogram over bins that fall with the logit
-// (for top_p with bounds of each bin's weight from its edges) leaves one bin or few that the border can be in, what is
-// above is summed, and the few candidates are sorted.  Where they are too many for that (equal logits, flat rows), the histogram is
-// repeated over the candidates' range of (logit, index), which a pass divides by 1024.  Bound by the latency of these steps, below
-// some tens of rows.
+// A row is taken by a cluster of up to 8 CTAs, as many as leave no SM with two; each has a contiguous part of the vocabulary and
+// reads it two to four times in 16-byte words, from L2 after the first.  What is kept is mostly a few tokens, so the usual way is to find a
+// bound that few logits exceed, to list these, and to do the rest of the work on the sorted list in one CTA:
+//   top_k: at least k threads of the first pass hold a logit of at least the k-th largest of the threads' maxima, so a histogram
+//          of these maxima gives the bound;
+//   top_p: a histogram of all logits near the largest, in bins of a factor exp(1/64) of the weight, and the sum of all weights in fp32 say
+//          to 1e-5 where the border is; the list tells whether a place in it lies that close to the border.
+// Where the list would be too long, or the border too close, the border is found step by step with sums in 64 bits: bins that the
+// border can be in, the weights above them, and again over the candidates' range of (logit, index), which a step divides by 1024;
+// the draw then reads the row once more.  CTAs hand each other sums by storing them into their neighbours' shared memory ahead of a
+// cluster barrier.  A weight in 64 bits is 10 operations, 64 a cycle and SM: the rows that keep all tokens are bound by these, the
+// others by the latency of the steps, and from some tens of rows on by the reads.
 #include <cooperative_groups.h>
 
 #include "mk_serving.cuh"
@@ -24,18 +30,22 @@ namespace cg = cooperative_groups;
 namespace mk_serving {
 namespace {
 
-constexpr int kSampleThreads = 1024;
-constexpr int kSampleWarps = kSampleThreads / 32;
-constexpr int kBins = 1024;          // one a thread
-constexpr int kCandidates = 2048;    // sorted at once
+constexpr int kThreads = 1024;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = kThreads;      // one a thread
+constexpr int kCandidates = 2 * kThreads;  // sorted at once, two a thread
 constexpr int kMaxCluster = 8;
 constexpr int kInner = 1024;         // (2^32 / 1024 elements a CTA)
-constexpr double kBinsPerUnit = 32.0;  // linear bins of weights: a factor of exp(1/32) each
+constexpr double kBinsPerUnit = 32.0;
+constexpr int kSlots = 4;
+constexpr float kNearBins = 64.f;    // bins a unit of (largest logit - logit) / temperature, near the largest
+constexpr float kTopBins = 16.f;     // bins a unit of (largest logit - logit) for the bound of the k-th
+constexpr float kSumError = 1e-5f;   // relative, of a sum of weights in fp32: the argument of exp is off by 2^-22 of itself, at most 23 where weights count
 
 // Larger logits are larger keys; -0 and +0 are equal, NaN counts as minus infinity.
+__device__ __forceinline__ float clean(float l) { return fmaxf(l, -INFINITY); }
 __device__ __forceinline__ uint32_t key_of(float l) {
-  l = isnan(l) ? -INFINITY : l + 0.f;
-  const uint32_t u = __float_as_uint(l);
+  const uint32_t u = __float_as_uint(l + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
@@ -46,38 +56,123 @@ struct SampleShared {
   uint32_t hist[kBins];
   uint32_t inner[kBins];            // of linear bins: how far into the bin its logits lie, summed, in units of 1 / kInner
   uint64_t list[kCandidates];       // rank 0's is used
-  double sums[kSampleWarps + 1];
-  uint64_t words[kSampleWarps];
-  double mass;                      // this CTA's share of a sum over the cluster
-  uint64_t best;                    // this CTA's first place
-  uint64_t lo, hi;                  // range of this CTA's candidates
-  uint32_t listed;                  // rank 0's: candidates in the list
+  double weights[kCandidates];      // of the list's
+  double power[64];                 // 2^(i / 64)
+  double sums[kWarps];
+  uint64_t words[kWarps];
+  double slot[kSlots][kMaxCluster];  // sums of the ranks, in turn; a slot comes round again behind three more barriers
+  uint64_t lo[kMaxCluster], hi[kMaxCluster];  // of every rank: first place; the range of its candidates
+  uint32_t counts[kMaxCluster];     // of every rank: candidates that it has listed
+  uint32_t listed[3];               // rank 0's: candidates in the list, of the rounds in turn; the first list's
+  int close;                        // rank 0 -> all: the border is too close to say
   uint64_t border;                  // written by rank 0 into every CTA
   double border_mass;
-  int found;
-  int first_bin, last_bin;
+  int first_bin, last_bin, last_kept;
 };
 
-struct Row {
-  const void* logits;
-  int dtype, vocab, begin, end;
+// A row, as the groups of 16 bytes (aligned) that it lies in: the first and the last may have elements outside.
+template <typename T> struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  const T* logits;
+  int vocab, shift;   // element of a group g: g N - shift + e
+  int g0, g1;         // this CTA's groups
   float top;
-  double inv_t;
-};
-__device__ __forceinline__ float logit_at(const Row& r, int i) {
-  float l;
-  if (r.dtype == MK_F32) l = __ldg((const float*)r.logits + i);
-  else if (r.dtype == MK_BF16) l = __bfloat162float(((const __nv_bfloat16*)r.logits)[i]);
-  else l = __half2float(((const __half*)r.logits)[i]);
-  return isnan(l) ? -INFINITY : l + 0.f;
-}
-__device__ __forceinline__ double weight(const Row& r, float l) {
-  if (l == r.top) return 1.0;  // (both may be infinite)
-  if (l == -INFINITY) return 0.0;
-  return exp(((double)l - (double)r.top) * r.inv_t);
-}
+  double scale;       // 64 log2(e) / temperature
+  double top_scaled;  // top * scale
+  const double* power;
 
-// Sum over the block in a fixed order; every thread gets it.
+  __device__ __forceinline__ int index(int g) const { return g * N - shift; }
+  __device__ __forceinline__ bool inside(int g) const { return index(g) >= 0 && index(g) + N <= vocab; }
+  // The logits of a group that is wholly inside the row.
+  __device__ __forceinline__ void load(int g, float (&l)[N]) const {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(logits + index(g)));
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 4) {
+        l[e] = clean(__uint_as_float(w[e]));
+      } else {
+        const float2 f = unpack2<T>(w[e]);
+        l[2 * e] = clean(f.x);
+        l[2 * e + 1] = clean(f.y);
+      }
+    }
+  }
+  // The same of any group; returns a bit for every element that is outside the row.
+  __device__ __forceinline__ uint32_t load_edge(int g, float (&l)[N]) const {
+    uint32_t outside = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int i = index(g) + e;
+      const bool in = i >= 0 && i < vocab;
+      l[e] = in ? clean(to_float(logits[i])) : -INFINITY;
+      outside |= in ? 0u : 1u << e;
+    }
+    return outside;
+  }
+  // exp((l - top) / temperature): the argument y in units of ln 2 / 64, its whole part by table (P. T. P. Tang's method, 1989), the rest
+  // r (|r| <= 1/2) by the series up to the fourth power; the next term is 4e-14.
+  __device__ __forceinline__ double weight(float l) const {
+    if (l == top) return 1.0;  // (both may be infinite)
+    constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: a sum with it is rounded to a whole number
+    constexpr double c1 = 0.6931471805599453094 / 64.0, c2 = c1 * c1 / 2.0, c3 = c2 * c1 / 3.0, c4 = c3 * c1 / 4.0;
+    const double x = (double)l, y = fma(x, scale, -top_scaled);
+    if (!(y >= -64.0 * 1021.0)) return far_weight(l);
+    const double big = y + kRound;
+    const int n = __double2loint(big);
+    const double r = y - (big - kRound);
+    const double t = power[n & 63];
+    const double e = fma(t * r, fma(r, fma(r, fma(r, c4, c3), c2), c1), t);
+    return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
+  }
+  // next to the smallest numbers, and where infinities meet
+  __device__ __noinline__ double far_weight(float l) const {
+    const double y = ((double)l - (double)top) * scale;
+    return l == -INFINITY || isnan(y) ? 0.0 : exp(y * (0.6931471805599453094 / 64.0));
+  }
+  // f(logits, n, index of the first) for all elements of the CTA: n = N at a time, at the row's two ends one.  DEEP: several loads of a
+  // thread in flight (code that runs once or twice is better short).
+  template <bool DEEP = false, typename F> __device__ __forceinline__ void each_group(const F& f) const {
+    constexpr int U = DEEP ? 16 / N : 1;
+    const int i0 = g0 < g1 && !inside(g0) ? g0 + 1 : g0, i1 = g1 > i0 && !inside(g1 - 1) ? g1 - 1 : g1;
+    int g = i0 + threadIdx.x;
+    if constexpr (U > 1) {
+#pragma unroll 1
+      for (; g + (U - 1) * kThreads < i1; g += U * kThreads) {
+        float l[U][N];
+#pragma unroll
+        for (int k = 0; k < U; ++k) load(g + k * kThreads, l[k]);
+#pragma unroll
+        for (int k = 0; k < U; ++k) f(l[k], N, index(g + k * kThreads));
+      }
+    }
+#pragma unroll 1
+    for (; g < i1; g += kThreads) {
+      float l[N];
+      load(g, l);
+      f(l, N, index(g));
+    }
+    if (threadIdx.x < 2 * N) {  // a thread an element
+      const int edge = threadIdx.x < N ? g0 : g1 - 1, i = index(edge) + (int)threadIdx.x % N;
+      const bool mine = threadIdx.x < N ? i0 > g0 : i1 < g1;
+      if (mine && i >= 0 && i < vocab) {
+        float l[N];
+        l[0] = clean(to_float(logits[i]));
+        f(l, 1, i);
+      }
+    }
+  }
+  // f(logit, index)
+  template <bool DEEP = false, typename F> __device__ __forceinline__ void each(const F& f) const {
+    each_group<DEEP>([&](const float (&l)[N], int n, int i) {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (e < n) f(l[e], i + e);
+    });
+  }
+};
+
+// Sum over the block in a fixed order; thread 0 to kMaxCluster - 1 get it (and all others).
 __device__ __forceinline__ double block_sum(double v, SampleShared& s) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
@@ -90,231 +185,469 @@ __device__ __forceinline__ double block_sum(double v, SampleShared& s) {
   return t;
 }
 // Sum of the values before this thread's, in the order of the threads; *total: of all.
-template <typename N> __device__ __forceinline__ N block_before(N v, N* scratch, N* total) {
+template <typename V> __device__ __forceinline__ V block_before(V v, V* scratch, V* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  N in = v;
+  V in = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const N u = __shfl_up_sync(kAll, in, o);
+    const V u = __shfl_up_sync(kAll, in, o);
     if (lane >= o) in += u;
   }
   __syncthreads();
   if (lane == 31) scratch[warp] = in;
   __syncthreads();
-  N c = scratch[lane];
+  V c = scratch[lane];
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const N u = __shfl_up_sync(kAll, c, o);
+    const V u = __shfl_up_sync(kAll, c, o);
     if (lane >= o) c += u;
   }
   *total = __shfl_sync(kAll, c, 31);
-  const N warps = __shfl_sync(kAll, c, warp > 0 ? warp - 1 : 0);
-  __syncthreads();
-  N before = __shfl_up_sync(kAll, in, 1);  // (not in - v: the sum before a thread must be the inclusive one of its neighbour)
+  const V warps = __shfl_sync(kAll, c, warp > 0 ? warp - 1 : 0);
+  V before = __shfl_up_sync(kAll, in, 1);  // (not in - v: the sum before a thread must be the inclusive one of its neighbour)
   if (lane == 0) before = 0;
-  return (warp > 0 ? warps : N(0)) + before;
+  return (warp > 0 ? warps : V(0)) + before;
 }
 
-struct Sampler {
+template <typename T> struct Sampler {
   cg::cluster_group cluster;
   SampleShared& s;
-  Row r;
-  int ranks, rank;
+  Row<T> r;
+  int ranks, rank, turn;  // turn: of the slots and the list's counters
 
-  template <typename N> __device__ __forceinline__ N* peer(N* p, int k) { return cluster.map_shared_rank(p, k); }
-  // Sum over the cluster, in the order of the ranks.
-  __device__ double cluster_sum(double v) {
+  template <typename V> __device__ __forceinline__ V* peer(V* p, int k) { return cluster.map_shared_rank(p, k); }
+  // A sum over the cluster, in the order of the ranks: give() on this side of a barrier, taken() on the other.
+  __device__ __forceinline__ void give(double v) {
     const double mine = block_sum(v, s);
-    if (threadIdx.x == 0) s.mass = mine;
-    cluster.sync();
+    if ((int)threadIdx.x < ranks) *peer(&s.slot[turn & (kSlots - 1)][rank], threadIdx.x) = mine;
+  }
+  __device__ __forceinline__ double taken() {
     double t = 0.0;
-    for (int k = 0; k < ranks; ++k) t += *peer(&s.mass, k);
-    cluster.sync();
+    for (int k = 0; k < ranks; ++k) t += s.slot[turn & (kSlots - 1)][k];
+    ++turn;
     return t;
   }
+  // Linear bins: the depth below the largest logit in units of a factor exp(1/32) of the weight; the last bin takes all that is deeper.
+  __device__ __forceinline__ float depth(float l) const {
+    if (l == r.top) return 0.f;
+    return fminf((r.top - l) * per_bin, (float)(kBins - 1));  // (infinite differences too)
+  }
+  float per_bin;
+  uint32_t count;         // of this thread's bin, over the cluster
+  double low_w, high_w;   // bounds of the mean weight in it
 
-  // First element in the order that the criterion leaves out is not wanted here but the last that it keeps:
-  // by count: the k-th; by mass: the last with (weights before it) < limit.  Returns its place; *kept: the weights up to and with it.
-  __device__ uint64_t border(bool by_mass, double limit, long long k, double* kept) {
+  // Histogram of the linear bins; with `sum`, *mass: the sum of all weights.
+  __device__ void linear_bins(bool sum, double* mass) {
+    double w = 0.0;
+    r.each([&](float l, int) {
+      const float d = depth(l);
+      const int b = (int)d;
+      atomicAdd(&s.hist[b], 1u);
+      if (b < kBins - 1) atomicAdd(&s.inner[b], (uint32_t)((d - (float)b) * (float)kInner));
+      if (sum) w += r.weight(l);
+    });
+    if (sum) give(w);
+    cluster.sync();
+    if (sum) *mass = taken();
+    count = 0;
+    uint32_t inner = 0;
+    for (int q = 0; q < ranks; ++q) {
+      count += *peer(&s.hist[threadIdx.x], q);
+      inner += *peer(&s.inner[threadIdx.x], q);
+    }
+    // exp is convex: the mean weight is at least the weight at the mean depth and at most the chord's value there.  The depth is
+    // known to 1 / kInner of a bin and to some units of 2^-24 relative.
+    low_w = high_w = 0.0;
+    const double edge = exp(-(double)threadIdx.x / kBinsPerUnit);
+    if (threadIdx.x == kBins - 1) {
+      high_w = edge * (1.0 + 1e-4);
+    } else if (count > 0) {
+      const double f = (double)inner / ((double)count * kInner);
+      low_w = edge * exp(-(f + 1.0 / kInner) / kBinsPerUnit) * (1.0 - 1e-5);
+      high_w = edge * (1.0 - (1.0 - exp(-1.0 / kBinsPerUnit)) * f) * (1.0 + 1e-5);
+    }
+  }
+
+  // List all elements with depth_of(l) < bins (bins <= kBins) at rank 0; returns how many there are, in the whole cluster (kCandidates + 1: more).
+  template <typename F> __device__ int list_above(const F& depth_of, float unit, int bins) {
+    // most are far below: one comparison with a bound that is safely too low
+    float bound = bins < kBins ? r.top - (float)bins / unit * 1.0001f - fabsf(r.top) * 1e-6f : -INFINITY;
+    if (isnan(bound)) bound = -INFINITY;  // (the largest is infinite)
+    r.template each<true>([&](float l, int i) {
+      if (l >= bound && (bins >= kBins || (int)depth_of(l) < bins)) {
+        const uint32_t at = atomicAdd(&s.listed[2], 1u);
+        if (at < kCandidates) s.list[at] = place_of(l, i);
+      }
+    });
+    __syncthreads();
+    const uint32_t mine = s.listed[2];
+    if ((int)threadIdx.x < ranks) *peer(&s.counts[rank], threadIdx.x) = mine;
+    cluster.sync();
+    uint64_t all = 0, before = 0;
+    for (int q = 0; q < ranks; ++q) {
+      if (q == rank) before = all;
+      all += s.counts[q];
+    }
+    if (all > kCandidates) return kCandidates + 1;
+    if (rank > 0) {
+      uint64_t* list = peer(s.list, 0) + before;
+      for (int i = threadIdx.x; i < (int)mine; i += kThreads) list[i] = s.list[i];
+    }
+    cluster.sync();
+    return (int)all;
+  }
+  // Bins 0 .. of which hold at least k of the threads' maxima: what top_k keeps is in them.
+  __device__ int bins_of_top(float mine, bool any, int k) {
+    auto depth_of = [&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * kTopBins, (float)(kBins - 1)); };
+    if (any) atomicAdd(&s.hist[(int)depth_of(mine)], 1u);
+    if (threadIdx.x == 0) s.last_bin = kBins;  // (fewer than k maxima: everything)
+    cluster.sync();
+    uint32_t n = 0;
+    for (int q = 0; q < ranks; ++q) n += *peer(&s.hist[threadIdx.x], q);
+    uint64_t total;
+    const uint64_t before = block_before((uint64_t)n, s.words, &total);
+    if (n > 0 && before < (uint64_t)k && before + n >= (uint64_t)k) s.last_bin = threadIdx.x + 1;
+    __syncthreads();
+    const int bins = s.last_bin;
+    return bins;
+  }
+  // Bins 0 .. that hold what top_p keeps, by sums to kSumError; *mass: the sum of all weights, as exactly.
+  __device__ int bins_of_mass(double top_p, float unit, double* mass) {
+    const float log2_scale = (float)(r.scale / 64.0);
+    auto depth_of = [&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * unit, (float)(kBins - 1)); };
+    const float top = r.top == INFINITY ? 3.4028235e38f : r.top;  // (differences without NaN)
+    const float near = top - (float)(kBins - 1) / unit * 1.0001f - fabsf(top) * 1e-6f;
+    float w = 0.f;
+    double sum = 0.0;
+    int n_w = 0;
+    r.template each_group<true>([&](const float (&l)[Row<T>::N], int n, int) {
+#pragma unroll
+      for (int e = 0; e < Row<T>::N; ++e) {
+        if (e >= n) break;
+        float x;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"((l[e] - top) * log2_scale));
+        w += x;
+        if (l[e] >= near) {
+          const float d = depth_of(l[e]);
+          if (d < (float)(kBins - 1)) atomicAdd(&s.hist[(int)d], 1u);
+        }
+      }
+      if (++n_w == 8) {  // (no more than 64 terms in fp32)
+        sum += (double)w;
+        w = 0.f;
+        n_w = 0;
+      }
+    });
+    give(sum + (double)w);
+    cluster.sync();
+    *mass = taken();
+    uint32_t n = 0;
+    for (int q = 0; q < ranks; ++q) n += *peer(&s.hist[threadIdx.x], q);
+    // at least so much weight is in the bins up to this one
+    double total;
+    const double low = (double)n * (double)exp2f(-(float)(threadIdx.x + 1) * (1.4427f / kNearBins)) * (1.0 - 1e-4);
+    const double before = block_before(threadIdx.x < kBins - 1 ? low : 0.0, s.sums, &total);
+    if (threadIdx.x == 0) s.last_bin = kBins;
+    __syncthreads();
+    const double limit = top_p * *mass * (1.0 + 4.0 * (double)kSumError);
+    if (threadIdx.x < kBins - 1 && before + low >= limit) atomicMin(&s.last_bin, (int)threadIdx.x + 1);
+    __syncthreads();
+    return s.last_bin;
+  }
+  // Histograms anew, for the way in steps.
+  __device__ void clear_bins() {
+    cluster.sync();  // (nobody reads them any more)
+    s.hist[threadIdx.x] = s.inner[threadIdx.x] = 0;
+    __syncthreads();
+  }
+
+  // Which bins can the border be in?  -> s.first_bin, s.last_bin (of the places behind `above` elements with the weights above_mass)
+  __device__ void find_bins(bool by_mass, double limit, long long k, long long above, double above_mass) {
+    if (threadIdx.x == 0) {
+      s.first_bin = kBins - 1;
+      s.last_bin = 0;
+    }
+    if (!by_mass) {
+      uint64_t total;
+      const uint64_t before = block_before((uint64_t)count, s.words, &total);  // (its barriers stand behind the two stores)
+      if (count > 0 && (long long)before + above < k && (long long)(before + count) + above >= k) s.first_bin = s.last_bin = threadIdx.x;
+    } else {
+      double total;
+      const double low_before = above_mass + block_before(count * low_w, s.sums, &total);
+      const double high_before = above_mass + block_before(count * high_w, s.sums, &total);
+      // kept for certain: all of a bin whose weights with those before it stay below the limit; left out for certain: low_before >= limit
+      if (count > 0 && low_before * (1.0 - 1e-9) < limit) {
+        if ((high_before + count * high_w) * (1.0 + 1e-9) >= limit) atomicMin(&s.first_bin, (int)threadIdx.x);
+        atomicMax(&s.last_bin, (int)threadIdx.x);
+      }
+    }
+    __syncthreads();
+  }
+
+  // Sorts s.list[0 .. n), the largest first, zeros last; all of it is there on return, up to the power of two.
+  __device__ __noinline__ void sort_list(int n_list) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (n_list <= kThreads / 8) {
+      // few: eight threads count how many of the others are larger than one of them (no two are equal but zeros)
+      const uint64_t mine = (t >> 3) < n_list ? s.list[t >> 3] : 0;
+      int larger = 0;
+      for (int j = t & 7; j < n_list; j += 8) larger += s.list[j] > mine;
+#pragma unroll
+      for (int o = 1; o < 8; o <<= 1) larger += __shfl_xor_sync(kAll, larger, o);
+      __syncthreads();
+      if (t < kThreads / 8) s.list[t] = 0;
+      __syncthreads();
+      if ((t & 7) == 0 && mine) s.list[larger] = mine;
+      __syncthreads();
+      return;
+    }
+    int n = kThreads / 4;
+    while (n < n_list) n <<= 1;
+    uint64_t x0 = t < n_list ? s.list[t] : 0, x1 = t + kThreads < n_list ? s.list[t + kThreads] : 0;
+    if (n <= kThreads) {
+      sort_steps<false>(x0, x1, n);
+    } else {
+      sort_steps<true>(x0, x1, n);
+    }
+    __syncthreads();
+    s.list[t] = x0;
+    if (n > kThreads) s.list[t + kThreads] = x1;
+    __syncthreads();
+  }
+  template <bool BOTH> __device__ __forceinline__ void sort_steps(uint64_t& x0, uint64_t& x1, int n) {
+    const int t = threadIdx.x;
+    // the earlier of two places takes the larger where the run falls, else the smaller
+    auto pick = [](uint64_t x, uint64_t y, bool larger) { return larger == (x > y) ? x : y; };
+#pragma unroll 1
+    for (int size = 2; size <= n; size <<= 1) {
+      const bool down0 = (t & size) == 0, down1 = ((t + kThreads) & size) == 0;
+#pragma unroll 1
+      for (int step = size >> 1; step > 0; step >>= 1) {
+        const bool first = (t & step) == 0;
+        uint64_t y0, y1 = 0;
+        if (step == kThreads) {  // (both are this thread's)
+          const uint64_t a = max(x0, x1);
+          x1 = min(x0, x1);
+          x0 = a;
+          continue;
+        }
+        if (step >= 32) {
+          __syncthreads();
+          s.list[t] = x0;
+          if (BOTH) s.list[t + kThreads] = x1;
+          __syncthreads();
+          y0 = s.list[t ^ step];
+          if (BOTH) y1 = s.list[(t ^ step) + kThreads];
+        } else {
+          y0 = __shfl_xor_sync(kAll, (unsigned long long)x0, step);
+          if (BOTH) y1 = __shfl_xor_sync(kAll, (unsigned long long)x1, step);
+        }
+        x0 = pick(x0, y0, first == down0);
+        if (BOTH) x1 = pick(x1, y1, first == down1);
+      }
+    }
+  }
+  // Sum of the values ahead of each of a thread's two, in the order of the sorted numbers.
+  __device__ __forceinline__ void before_both(const double (&w)[2], int n, double (&before)[2], double* total) {
+    double first, second = 0.0;
+    before[0] = block_before(w[0], s.sums, &first);
+    if (n > kThreads) {
+      before[1] = first + block_before(w[1], s.sums, &second);
+    } else {
+      before[1] = first;
+    }
+    *total = first + second;
+  }
+
+  // The draw from the sorted list alone (rank 0): it holds all that can be kept.  Without top_k, `mass` is the sum of all weights to
+  // kSumError; false where that leaves the border open.
+  __device__ bool draw(int n_list, bool by_k, int k, bool by_mass, double top_p, double mass, float min_p, double u, int64_t* token, float* logprob) {
+    const int t = threadIdx.x;
+    sort_list(n_list);
+    const uint64_t place[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
+    bool keep[2], open = false;
+    double w[2], before[2], total;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = t + h * kThreads;
+      keep[h] = at < n_list && (!by_k || at < k);
+      w[h] = keep[h] ? r.weight(logit_of((uint32_t)(place[h] >> 32))) : 0.0;
+    }
+    before_both(w, n_list, before, &total);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = t + h * kThreads;
+      if (by_mass) {
+        const double limit = top_p * (by_k ? total : mass), slack = by_k ? 0.0 : (double)kSumError * limit;
+        open = open || (keep[h] && at > 0 && before[h] > limit - slack && before[h] < limit + slack);
+        // (a list that ends below the limit does not hold the border)
+        open = open || (!by_k && at == 0 && total < limit + slack && n_list < r.vocab);
+        keep[h] = keep[h] && (before[h] < limit || at == 0);
+      }
+      keep[h] = keep[h] && w[h] > 0.0 && w[h] >= (double)min_p;
+      s.weights[at] = w[h];
+    }
+    if (__syncthreads_or(open)) return false;
+    // the kept ones in the order of the index
+#pragma unroll
+    for (int h = 0; h < 2; ++h) s.list[t + h * kThreads] = keep[h] ? (place[h] & 0xffffffffu) << 32 | (uint32_t)(t + h * kThreads + 1) : 0;
+    // (what is kept is the beginning of the sorted list)
+    const int kept = __syncthreads_count(keep[0]) + (n_list > kThreads ? __syncthreads_count(keep[1]) : 0);
+    sort_list(kept);
+    const uint64_t by_index[2] = {t < kept ? s.list[t] : 0, t + kThreads < kept ? s.list[t + kThreads] : 0};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) w[h] = t + h * kThreads < kept ? s.weights[(uint32_t)by_index[h] - 1] : 0.0;
+    before_both(w, n_list, before, &total);
+    const double goal = u * total;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (t + h * kThreads < kept && before[h] + w[h] > goal) atomicMin(&s.first_bin, t + h * kThreads);
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (t + h * kThreads == min(s.first_bin, kept - 1)) {
+        *token = (int64_t)(uint32_t)~(uint32_t)(by_index[h] >> 32);
+        if (logprob) *logprob = (float)log(w[h] / total);
+      }
+    return true;
+  }
+
+  // The border among `n_list` sorted candidates, by rank 0; `above` elements with the weights `mass` stand before them.  by_k: the first k
+  // of the order are kept; by_mass: those before which less than `limit` lies, with by_k less than limit times the first k's weights.
+  __device__ void cut(int n_list, bool by_k, long long k, bool by_mass, double limit, long long above, double mass) {
+    const int t = threadIdx.x;
+    sort_list(n_list);
+    const uint64_t place[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
+    if (t == 0) s.last_kept = 0;
+    bool keep[2];
+    double w[2], before[2], total;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = t + h * kThreads;
+      keep[h] = at < n_list && (!by_k || above + at < k);
+      w[h] = keep[h] ? r.weight(logit_of((uint32_t)(place[h] >> 32))) : 0.0;
+    }
+    before_both(w, n_list, before, &total);
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = t + h * kThreads;
+      before[h] += mass;
+      if (by_mass) keep[h] = keep[h] && (before[h] < (by_k ? limit * (mass + total) : limit) || above + at == 0);
+      if (keep[h]) atomicMax(&s.last_kept, at);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (t + h * kThreads == s.last_kept)
+        for (int q = 0; q < ranks; ++q) {
+          *peer(&s.border, q) = place[h];
+          *peer(&s.border_mass, q) = before[h] + w[h];
+        }
+  }
+
+  // The last place that is kept.  Linear bins first; by_k: the k-th, and with by_mass that of top_p = `limit` among them where one list
+  // holds them all (*both says so); by_mass alone: weights before it < limit.  *kept: the weights up to and with it.
+  __device__ uint64_t border(bool by_k, long long k, bool by_mass, double limit, double* kept, bool* both) {
     uint64_t lo = 0, hi = ~0ull;     // places of the candidates
     long long above = 0;             // elements before them
     double above_mass = 0.0;
     long long left = r.vocab;        // candidates
-    bool linear = true;              // bins fall linearly with the logit; later: a shift of the place
-    const float per_bin = by_mass ? (float)(kBinsPerUnit * r.inv_t) : 64.f;
+    bool linear = true;
+    int shift = 0;
+    *both = false;
     for (;;) {
-      const int shift = linear ? 0 : max(0, 64 - (int)__clzll(hi - lo) - 10);
-      auto depth_of = [&](float l) -> float { return l == -INFINITY ? (float)kBins : r.top == l ? 0.f : fminf((r.top - l) * per_bin, (float)kBins); };
-      auto bin_of = [&](float l, uint64_t place) -> int { return linear ? min((int)depth_of(l), kBins - 1) : (int)((hi - place) >> shift); };
-      s.hist[threadIdx.x] = s.inner[threadIdx.x] = 0;
-      __syncthreads();
-      for (int i = r.begin + threadIdx.x; i < r.end; i += kSampleThreads) {
-        const float l = logit_at(r, i);
-        const uint64_t place = place_of(l, i);
-        if (place < lo || place > hi) continue;
-        const int b = bin_of(l, place);
-        atomicAdd(&s.hist[b], 1u);
-        if (by_mass && linear && b < kBins - 1) atomicAdd(&s.inner[b], (uint32_t)((depth_of(l) - (float)b) * (float)kInner));
-      }
-      cluster.sync();
-      uint32_t count = 0;
-      for (int q = 0; q < ranks; ++q) count += *peer(&s.hist[threadIdx.x], q);
-      // Which bins can the border be in?  By mass: the weights before a bin are known up to those of its edges.
-      int first_bin, last_bin;
-      if (threadIdx.x == 0) {
-        s.first_bin = kBins - 1;
-        s.last_bin = 0;
-      }
-      if (!by_mass) {
-        uint64_t total;
-        const uint64_t before = block_before((uint64_t)count, s.words, &total);
-        // (k is at most the number of elements)
-        if (count > 0 && (long long)before + above < k && (long long)(before + count) + above >= k) s.first_bin = s.last_bin = threadIdx.x;
-      } else {
-        double low_w = 0.0, high_w = 0.0;  // bounds of the mean weight in the bin
-        if (linear) {
-          // exp is convex: the mean is at least the weight at the mean depth and at most the chord's value there.  The depth is known
-          // to 1 / kInner of a bin and to some units of 2^-24.
-          uint32_t inner = 0;
-          for (int q = 0; q < ranks; ++q) inner += *peer(&s.inner[threadIdx.x], q);
-          const double edge = exp(-(double)threadIdx.x / kBinsPerUnit), slope = 1.0 - exp(-1.0 / kBinsPerUnit);
-          if (threadIdx.x == kBins - 1) {
-            high_w = edge * (1.0 + 1e-4);
-          } else if (count > 0) {
-            const double f = (double)inner / ((double)count * kInner);
-            low_w = edge * exp(-(f + 1.0 / kInner) / kBinsPerUnit) * (1.0 - 1e-5);
-            high_w = edge * (1.0 - slope * f) * (1.0 + 1e-5);
-          }
-        } else {
-          const uint64_t top = (uint64_t)threadIdx.x << shift, end = top + ((1ull << shift) - 1);
-          const uint64_t a = top <= hi - lo ? hi - top : lo, b = end <= hi - lo ? hi - end : lo;
-          high_w = weight(r, logit_of((uint32_t)(a >> 32))) * (1.0 + 1e-9);
-          low_w = weight(r, logit_of((uint32_t)(b >> 32))) * (1.0 - 1e-9);
-        }
-        double total;
-        const double low_before = above_mass + block_before(count * low_w, s.sums, &total);
-        const double high_before = above_mass + block_before(count * high_w, s.sums, &total);
-        // kept for certain: all of a bin whose weights with those before it stay below the limit; left out for certain: low_before >= limit
-        if (count > 0 && low_before * (1.0 - 1e-9) < limit) {
-          if ((high_before + count * high_w) * (1.0 + 1e-9) >= limit) atomicMin(&s.first_bin, (int)threadIdx.x);
-          atomicMax(&s.last_bin, (int)threadIdx.x);
-        }
-      }
-      __syncthreads();
-      first_bin = min(s.first_bin, s.last_bin);
-      last_bin = s.last_bin;
-      uint64_t candidates, all;
+      find_bins(!by_k, limit, k, above, above_mass);
+      int first_bin = min(s.first_bin, s.last_bin);
+      const int last_bin = s.last_bin;
+      uint64_t candidates, ahead;
       {
-        const uint64_t in = (int)threadIdx.x >= first_bin && (int)threadIdx.x <= last_bin ? count : 0;
-        const uint64_t ahead = (int)threadIdx.x < first_bin ? count : 0;
-        block_before(in, s.words, &candidates);
-        block_before(ahead, s.words, &all);
-        above += (long long)all;
+        // both counts in one sum: 2^32 a half
+        const uint64_t mine = (int)threadIdx.x < first_bin ? (uint64_t)count : (int)threadIdx.x <= last_bin ? (uint64_t)count << 32 : 0;
+        uint64_t total;
+        block_before(mine, s.words, &total);
+        candidates = total >> 32;
+        ahead = total & 0xffffffffu;
       }
+      if (linear && by_k && candidates + ahead <= kCandidates) {  // all of the first k in one list
+        candidates += ahead;
+        ahead = 0;
+        first_bin = 0;
+        *both = true;
+      }
+      above += (long long)ahead;
       // the weights above the candidates, and the candidates themselves or their range
       const bool few = candidates <= kCandidates;
-      if (threadIdx.x == 0) {
-        s.lo = ~0ull;
-        s.hi = 0;
-        s.listed = 0;
-      }
-      cluster.sync();  // (all have read the histograms; rank 0's list is empty)
-      uint32_t* listed = peer(&s.listed, 0);
+      uint32_t* listed = peer(&s.listed[turn & 1], 0);
       uint64_t* list = peer(s.list, 0);
       double mass = 0.0;
       uint64_t my_lo = ~0ull, my_hi = 0;
-      for (int i = r.begin + threadIdx.x; i < r.end; i += kSampleThreads) {
-        const float l = logit_at(r, i);
+      r.each([&](float l, int i) {
         const uint64_t place = place_of(l, i);
-        if (place < lo || place > hi) continue;
-        const int b = bin_of(l, place);
-        if (b < first_bin) mass += weight(r, l);
-        else if (b <= last_bin) {
+        if (place < lo || place > hi) return;
+        const int b = linear ? (int)depth(l) : (int)((hi - place) >> shift);
+        if (b < first_bin) {
+          mass += r.weight(l);
+        } else if (b <= last_bin) {
           if (few) list[atomicAdd(listed, 1u)] = place;
           my_lo = min(my_lo, place);
           my_hi = max(my_hi, place);
         }
+      });
+      give(mass);
+      if (!few) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+          my_lo = min(my_lo, (uint64_t)__shfl_xor_sync(kAll, (unsigned long long)my_lo, o));
+          my_hi = max(my_hi, (uint64_t)__shfl_xor_sync(kAll, (unsigned long long)my_hi, o));
+        }
+        if (threadIdx.x < 2) s.words[threadIdx.x] = threadIdx.x ? 0 : ~0ull;
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) {
+          atomicMin((unsigned long long*)&s.words[0], (unsigned long long)my_lo);
+          atomicMax((unsigned long long*)&s.words[1], (unsigned long long)my_hi);
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < ranks) {
+          *peer(&s.lo[rank], threadIdx.x) = s.words[0];
+          *peer(&s.hi[rank], threadIdx.x) = s.words[1];
+        }
       }
-      above_mass += cluster_sum(mass);
+      cluster.sync();
+      above_mass += taken();
       if (few) {
         if (rank == 0) {
-          // sorted, earliest first (the list's order was that of arrival, the sorted one is not)
-          int n = 32;
-          while (n < (int)candidates) n <<= 1;
-          for (int i = threadIdx.x; i < n; i += kSampleThreads)
-            if (i >= (int)candidates) s.list[i] = 0;
-          __syncthreads();
-          for (int size = 2; size <= n; size <<= 1)
-            for (int step = size >> 1; step > 0; step >>= 1) {
-              for (int i = threadIdx.x; i < n / 2; i += kSampleThreads) {
-                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                const uint64_t x = s.list[a], y = s.list[b];
-                if ((x < y) == ((a & size) == 0)) {
-                  s.list[a] = y;
-                  s.list[b] = x;
-                }
-              }
-              __syncthreads();
-            }
-          // two of them a thread
-          const int at = 2 * threadIdx.x;
-          const uint64_t p0 = at < (int)candidates ? s.list[at] : 0, p1 = at + 1 < (int)candidates ? s.list[at + 1] : 0;
-          const double w0 = at < (int)candidates ? weight(r, logit_of((uint32_t)(p0 >> 32))) : 0.0;
-          const double w1 = at + 1 < (int)candidates ? weight(r, logit_of((uint32_t)(p1 >> 32))) : 0.0;
-          double total;
-          const double before = above_mass + block_before(w0 + w1, s.sums, &total);
-          if (threadIdx.x == 0) s.first_bin = 0;
-          __syncthreads();
-          bool keep0, keep1;
-          if (by_mass) {
-            keep0 = at < (int)candidates && (before < limit || above + at == 0);
-            keep1 = at + 1 < (int)candidates && before + w0 < limit;
-          } else {
-            keep0 = at < (int)candidates && above + at < k;
-            keep1 = at + 1 < (int)candidates && above + at + 1 < k;
-          }
-          const int last = keep1 ? at + 1 : keep0 ? at : -1;
-          if (last >= 0) atomicMax(&s.first_bin, last);
-          __syncthreads();
-          if (last == s.first_bin && last >= 0) {
-            const uint64_t place = keep1 ? p1 : p0;
-            const double up_to = keep1 ? before + w0 + w1 : before + w0;
-            for (int q = 0; q < ranks; ++q) {
-              *peer(&s.border, q) = place;
-              *peer(&s.border_mass, q) = up_to;
-            }
-          }
+          if (threadIdx.x == 0) s.listed[(turn - 1) & 1] = 0;  // (for the round after the next; a barrier stands between)
+          cut((int)candidates, by_k, k, *both ? by_mass : !by_k, limit, above, above_mass);
         }
         cluster.sync();
         *kept = s.border_mass;
         return s.border;
       }
       // too many: their range, in 1024 parts
-      if (my_lo <= my_hi) {
-        atomicMin((unsigned long long*)&s.lo, (unsigned long long)my_lo);
-        atomicMax((unsigned long long*)&s.hi, (unsigned long long)my_hi);
-      }
-      cluster.sync();
       lo = ~0ull;
       hi = 0;
       for (int q = 0; q < ranks; ++q) {
-        lo = min(lo, *peer(&s.lo, q));
-        hi = max(hi, *peer(&s.hi, q));
+        lo = min(lo, s.lo[q]);
+        hi = max(hi, s.hi[q]);
       }
-      cluster.sync();
-      if (by_mass && !linear && 4 * (long long)candidates > 3 * left) {
+      if (!by_k && !linear && 4 * (long long)candidates > 3 * left) {
         // bounds from the edges can leave all bins open, where logits of very different weight share one: halve the range
         const uint64_t mid = lo + ((hi - lo) >> 1);
         double w = 0.0, n = 0.0;
-        for (int i = r.begin + threadIdx.x; i < r.end; i += kSampleThreads) {
-          const float l = logit_at(r, i);
+        r.each([&](float l, int i) {
           const uint64_t place = place_of(l, i);
-          if (place <= mid || place > hi) continue;
-          w += weight(r, l);
+          if (place <= mid || place > hi) return;
+          w += r.weight(l);
           n += 1.0;
-        }
-        w = cluster_sum(w);
-        n = cluster_sum(n);
+        });
+        give(w);
+        cluster.sync();
+        w = taken();
+        give(n);
+        cluster.sync();
+        n = taken();
         if (above_mass + w < limit) {
           above += (long long)n;
           above_mass += w;
@@ -325,15 +658,30 @@ struct Sampler {
       }
       left = (long long)candidates;
       linear = false;
+      shift = max(0, 64 - (int)__clzll(hi - lo) - 10);
+      s.hist[threadIdx.x] = 0;  // (all have read the last one: a barrier stands between)
+      __syncthreads();
+      r.each([&](float l, int i) {
+        const uint64_t place = place_of(l, i);
+        if (place >= lo && place <= hi) atomicAdd(&s.hist[(int)((hi - place) >> shift)], 1u);
+      });
+      cluster.sync();
+      count = 0;
+      for (int q = 0; q < ranks; ++q) count += *peer(&s.hist[threadIdx.x], q);
+      const uint64_t first = (uint64_t)threadIdx.x << shift, last = first + ((1ull << shift) - 1);
+      high_w = r.weight(logit_of((uint32_t)((first <= hi - lo ? hi - first : lo) >> 32))) * (1.0 + 1e-9);
+      low_w = r.weight(logit_of((uint32_t)((last <= hi - lo ? hi - last : lo) >> 32))) * (1.0 - 1e-9);
     }
   }
 };
 
 __device__ __forceinline__ float setting(const float* per_request, float value, int r) { return per_request ? __ldg(per_request + r) : value; }
 
-__global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const __grid_constant__ mk_sample_args a) {
+template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kernel(const __grid_constant__ mk_sample_args a) {
   __shared__ SampleShared s;
+  constexpr int N = Row<T>::N;
   cg::cluster_group cluster = cg::this_cluster();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int req = blockIdx.x / ranks;
   long long row = req;
@@ -342,6 +690,7 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const __grid_
     row = q1 > q0 && q0 >= 0 ? q1 - 1 : -1;
   }
   if (row < 0 || row >= a.rows) {  // (the whole cluster)
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
     if (rank == 0 && threadIdx.x == 0) {
       a.tokens[req] = -1;
       if (a.logprobs) a.logprobs[req] = -INFINITY;
@@ -349,135 +698,222 @@ __global__ void __launch_bounds__(kSampleThreads, 1) sample_kernel(const __grid_
     return;
   }
   const float temperature = setting(a.temperature, a.temperature_value, req);
-  const float top_p = setting(a.top_p, a.top_p_value, req), min_p = setting(a.min_p, a.min_p_value, req);
+  const float top_p = setting(a.top_p, a.top_p_value, req), min_p = fminf(setting(a.min_p, a.min_p_value, req), 1.f);  // (the largest always stays)
   const int top_k = a.top_k ? __ldg(a.top_k + req) : a.top_k_value;
-  Sampler d{cluster, s, {}, ranks, rank};
-  Row& r = d.r;
-  r.dtype = a.dtype;
+  const double u = (double)__ldg(a.u + req);
+  Sampler<T> d{cluster, s, {}, ranks, rank, 0};
+  Row<T>& r = d.r;
   r.vocab = a.vocab;
-  r.logits = (const char*)a.logits + row * a.row_stride * (a.dtype == MK_F32 ? 4 : 2);
-  const int per = (a.vocab + ranks - 1) / ranks;
-  r.begin = min(a.vocab, rank * per);
-  r.end = min(a.vocab, r.begin + per);
+  r.logits = (const T*)a.logits + row * a.row_stride;
+  r.shift = (int)((reinterpret_cast<uintptr_t>(r.logits) & 15) / sizeof(T));
+  r.power = s.power;
+  const int groups = (a.vocab + r.shift + N - 1) / N, per = (groups + ranks - 1) / ranks;
+  r.g0 = min(groups, rank * per);
+  r.g1 = min(groups, r.g0 + per);
 
   // the first place
-  uint64_t best = 0;
-  for (int i = r.begin + threadIdx.x; i < r.end; i += kSampleThreads) best = max(best, place_of(logit_at(r, i), i));
+  s.hist[threadIdx.x] = s.inner[threadIdx.x] = 0;
+  if (threadIdx.x < 64) s.power[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  if (threadIdx.x < 3) s.listed[threadIdx.x] = 0;
+  if (threadIdx.x == 0) s.first_bin = 0x7fffffff;
+  float top = -INFINITY;
+  int top_at = 0x7fffffff;
+  r.template each<true>([&](float l, int i) {  // (a thread's indices rise, but for the row's first elements)
+    if (l > top || top_at == 0x7fffffff || (l == top && i < top_at)) {
+      top = l;
+      top_at = i;
+    }
+  });
+  uint64_t best = top_at == 0x7fffffff ? 0 : place_of(top, top_at);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(kAll, (unsigned long long)best, o));
   if ((threadIdx.x & 31) == 0) s.words[threadIdx.x >> 5] = best;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kSampleWarps; ++w) best = max(best, s.words[w]);
-    s.best = best;
-    s.found = -1;
-  }
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // every CTA has begun before its shared memory is written
+  best = s.words[threadIdx.x & 31];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) best = max(best, (uint64_t)__shfl_xor_sync(kAll, (unsigned long long)best, o));
+  if ((int)threadIdx.x < ranks) *d.peer(&s.hi[rank], threadIdx.x) = best;
   cluster.sync();
   best = 0;
-  for (int q = 0; q < ranks; ++q) best = max(best, *d.peer(&s.best, q));
+  for (int q = 0; q < ranks; ++q) best = max(best, s.hi[q]);
   r.top = logit_of((uint32_t)(best >> 32));
   const bool nothing = r.top == -INFINITY;
-  if (nothing || !(temperature > 0.f)) {  // no token can be chosen, or the greedy one is
+  if (nothing || !(temperature > 0.f)) {  // no token can be chosen, or the greedy one is (no CTA looks into another any more)
     if (rank == 0 && threadIdx.x == 0) {
       a.tokens[req] = nothing ? -1 : (long long)(uint32_t)~(uint32_t)best;
       if (a.logprobs) a.logprobs[req] = nothing ? -INFINITY : 0.f;
     }
-    cluster.sync();  // nobody leaves while another reads its shared memory
     return;
   }
-  r.inv_t = 1.0 / (double)temperature;
+  const double inv_t = 1.0 / (double)temperature;
+  r.scale = inv_t * (64.0 / 0.6931471805599453094);
+  r.top_scaled = (double)r.top * r.scale;
+  d.per_bin = (float)(kBinsPerUnit * inv_t);
 
   uint64_t least = 0;  // the border: places from here on are kept
-  double kept_mass = -1.0;
   const bool cut_k = top_k > 0 && top_k < a.vocab, cut_p = top_p < 1.f;
-  if (cut_k) least = d.border(false, 0.0, top_k, &kept_mass);
-  if (cut_p) {
-    if (!cut_k) {
-      double w = 0.0;
-      for (int i = r.begin + threadIdx.x; i < r.end; i += kSampleThreads) w += weight(r, logit_at(r, i));
-      kept_mass = d.cluster_sum(w);
+  if (cut_k || cut_p) {
+    double mass = 0.0;
+    // the short way: a list of all that can be kept
+    int listed;
+    if (cut_k) {
+      const int bins = d.bins_of_top(top, top_at != 0x7fffffff, top_k);
+      listed = d.list_above([&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * kTopBins, (float)(kBins - 1)); }, kTopBins, bins);
+    } else {
+      const float unit = (float)((double)kNearBins * inv_t);
+      const int bins = d.bins_of_mass((double)top_p, unit, &mass);
+      listed = bins < kBins ? d.list_above([&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * unit, (float)(kBins - 1)); }, unit, bins) : kCandidates + 1;
     }
-    double unused;
-    const uint64_t b = d.border(true, (double)top_p * kept_mass, 0, &unused);
-    least = max(least, b);
+    if (listed <= kCandidates) {
+      bool open = false;
+      if (rank == 0) open = !d.draw(listed, cut_k, top_k, cut_p, (double)top_p, mass, min_p, u, a.tokens + req, a.logprobs ? a.logprobs + req : nullptr);
+      if (cut_k) return;  // (no sum in fp32 is in it: the border is never open, and nobody looks into another CTA any more)
+      if (rank == 0 && (int)threadIdx.x < ranks) *d.peer(&s.close, threadIdx.x) = open;
+      cluster.sync();
+      if (!s.close) return;
+    }
+    // the way in steps
+    d.clear_bins();
+    d.linear_bins(!cut_k, &mass);
+    bool both = false;
+    if (cut_k) {
+      const uint32_t count = d.count;
+      const double low = d.low_w, high = d.high_w;
+      least = d.border(true, top_k, cut_p, (double)top_p, &mass, &both);
+      d.count = count;
+      d.low_w = low;
+      d.high_w = high;
+    }
+    if (cut_p && !both) {
+      double unused;
+      least = max(least, d.border(false, 0, true, (double)top_p * mass, &unused, &both));
+    }
   }
 
   // the kept weights in the order of the index: a warp has a contiguous part of the CTA's
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int part = ((r.end - r.begin + kSampleWarps - 1) / kSampleWarps + 31) / 32 * 32;
-  const int b0 = min(r.end, r.begin + warp * part), b1 = min(r.end, b0 + part);
-  auto kept = [&](int i) -> double {
-    const float l = logit_at(r, i);
-    if (place_of(l, i) < least) return 0.0;
-    const double w = weight(r, l);
-    return w >= (double)min_p ? w : 0.0;
+  const int part = ((r.g1 - r.g0 + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int b0 = min(r.g1, r.g0 + warp * part), b1 = min(r.g1, b0 + part);
+  // (min_p: a bound that is safely too low; the weight itself decides)
+  const float least_logit = fmaxf(least ? logit_of((uint32_t)(least >> 32)) : -INFINITY,
+                                  min_p > 0.f ? r.top + temperature * (logf(min_p) - 1e-3f) * 1.0001f - fabsf(r.top) * 1e-6f : -INFINITY);
+  auto kept = [&](float l, int i) -> double {
+    if (l < least_logit || (least != 0 && place_of(l, i) < least)) return 0.0;
+    const double w = r.weight(l);
+    return min_p > 0.f && w < (double)min_p ? 0.0 : w;
+  };
+  auto kept_group = [&](int g, double (&w)[N]) -> double {  // and their sum, in order
+    float l[N];
+    uint32_t outside = 0;
+    if (r.inside(g)) r.load(g, l);
+    else outside = r.load_edge(g, l);
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      w[e] = outside >> e & 1 ? 0.0 : kept(l[e], r.index(g) + e);
+      sum += w[e];
+    }
+    return sum;
   };
   double mine = 0.0;
-  for (int i = b0 + lane; i < b1; i += 32) mine += kept(i);
+#pragma unroll 2
+  for (int g = b0 + lane; g < b1; g += 32) {
+    double w[N];
+    mine += kept_group(g, w);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kAll, mine, o);
   __syncthreads();
   if (lane == 0) s.sums[warp] = mine;
   __syncthreads();
-  double in_cta = 0.0;
-  for (int w = 0; w < kSampleWarps; ++w) in_cta += s.sums[w];
-  if (threadIdx.x == 0) s.mass = in_cta;
-  cluster.sync();
+  if ((int)threadIdx.x < ranks) {
+    double in_cta = 0.0;
+    for (int w = 0; w < kWarps; ++w) in_cta += s.sums[w];
+    *d.peer(&s.slot[d.turn & (kSlots - 1)][rank], threadIdx.x) = in_cta;
+  }
+  cluster.sync();  // the last time that a CTA touches another
   // the first CTA whose sum exceeds the goal has the token, and of its warps the first; where rounding leaves none, the last that keeps any
+  const double* in_rank = s.slot[d.turn & (kSlots - 1)];
   double total = 0.0;
-  for (int q = 0; q < ranks; ++q) total += *d.peer(&s.mass, q);
-  const double goal = (double)__ldg(a.u + req) * total;
+  for (int q = 0; q < ranks; ++q) total += in_rank[q];
+  const double goal = u * total;
   double end = 0.0, before = 0.0;
   int owner = -1;
   for (int q = 0; q < ranks; ++q) {
-    const double m = *d.peer(&s.mass, q);
+    const double m = in_rank[q];
     if (m > 0.0 && (owner < 0 || goal >= end)) {
       owner = q;
       before = end;
     }
     end += m;
   }
-  if (rank == owner) {
-    double from = before;
-    end = before;
-    owner = -1;
-    for (int w = 0; w < kSampleWarps; ++w) {
-      const double m = s.sums[w];
-      if (m > 0.0 && (owner < 0 || goal >= end)) {
-        owner = w;
-        from = end;
-      }
-      end += m;
+  if (rank != owner) return;
+  double from = before;
+  end = before;
+  owner = -1;
+  for (int w = 0; w < kWarps; ++w) {
+    const double m = s.sums[w];
+    if (m > 0.0 && (owner < 0 || goal >= end)) {
+      owner = w;
+      from = end;
     }
-    if (warp == owner) {
-      double run = from;
-      int token = -1;
-      double w_token = 0.0;
-      for (int i0 = b0; i0 < b1; i0 += 32) {
-        const int i = i0 + lane;
-        const double w = i < b1 ? kept(i) : 0.0;
-        double up = w;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double u = __shfl_up_sync(kAll, up, o);
-          if (lane >= o) up += u;
-        }
-        const unsigned over = __ballot_sync(kAll, w > 0.0 && run + up > goal), any = __ballot_sync(kAll, w > 0.0);
-        if (any) {
-          const int k = over ? __ffs(over) - 1 : 31 - __clz(any);
-          token = i0 + k;
-          w_token = __shfl_sync(kAll, w, k);
-        }
-        if (over) break;
-        run += __shfl_sync(kAll, up, 31);
-      }
-      if (lane == 0) {
-        a.tokens[req] = token;
-        if (a.logprobs) a.logprobs[req] = (float)log(w_token / total);
-      }
-    }
+    end += m;
   }
-  cluster.sync();
+  if (warp != owner) return;
+  int token = -1;
+  double w_token = 0.0, run = from;
+  for (int i0 = b0; i0 < b1; i0 += 32) {
+    double w[N] = {};
+    const double sum = i0 + lane < b1 ? kept_group(i0 + lane, w) : 0.0;
+    double up = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double x = __shfl_up_sync(kAll, up, o);
+      if (lane >= o) up += x;
+    }
+    const unsigned over = __ballot_sync(kAll, sum > 0.0 && run + up > goal), any = __ballot_sync(kAll, sum > 0.0);
+    if (any) {
+      const int k = over ? __ffs(over) - 1 : 31 - __clz(any);
+      double at = __shfl_up_sync(kAll, up, 1);
+      at = run + (lane == 0 ? 0.0 : at);
+      // of that lane's elements the first that exceeds, else its last that is kept
+      int pick = -1;
+      double w_pick = 0.0;
+      bool done = false;
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        if (w[e] > 0.0 && !done) {
+          pick = e;
+          w_pick = w[e];
+        }
+        at += w[e];
+        done = done || (w[e] > 0.0 && at > goal);
+      }
+      token = r.index(i0 + k) + __shfl_sync(kAll, pick, k);
+      w_token = __shfl_sync(kAll, w_pick, k);
+    }
+    if (over) break;
+    run += __shfl_sync(kAll, up, 31);
+  }
+  if (lane == 0) {
+    a.tokens[req] = token;
+    if (a.logprobs) a.logprobs[req] = (float)log(w_token / total);
+  }
+}
+
+template <typename T> cudaError_t launch(const mk_sample_args& a, int ranks, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ranks * a.requests));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a);
 }
 
 }  // namespace
@@ -495,16 +931,7 @@ extern "C" int mk_sample_tokens(const mk_sample_args* args, void* stream) {
   if (a.requests == 0) return 0;
   int ranks = kMaxCluster;
   while (ranks > 1 && ((long long)ranks * a.requests > sm_count() || a.vocab / ranks < 1024)) ranks >>= 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ranks * a.requests));
-  cfg.blockDim = dim3(kSampleThreads);
-  cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, sample_kernel, a);
+  const cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = a.dtype == MK_F32 ? launch<float>(a, ranks, st) : a.dtype == MK_BF16 ? launch<__nv_bfloat16>(a, ranks, st) : launch<__half>(a, ranks, st);
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "sample_tokens: launch failed: %s", cudaGetErrorString(e));
 }
