@@ -136,6 +136,17 @@ template <typename T, int NT> struct RowWarp {
   __device__ __forceinline__ float* slot_of(const Cursor& c) const {
     return p.partial + (size_t)(2 * warp + (c.from_start ? 1 : 0)) * part_floats(ROWS);
   }
+  // A group that begins here and goes on in other warps' ranges: what the merge needs to know of it.
+  __device__ __forceinline__ void leave_merge(const Cursor& c, long long per) const {
+    const int last = (int)((c.u - 1 + c.tiles - c.k_end) / per);  // (c.u: behind the piece)
+    if (lane == 0) {
+      p.merges[warp].last = last;
+      p.merges[warp].kv_head = c.kv_head;
+      p.merges[warp].row0 = c.row0;
+      p.merges[warp].rows = c.rows;
+      p.merges[warp].first_token = c.q.q0;
+    }
+  }
   __device__ __forceinline__ long long row_token(const Cursor& c, int row, int* head) const {
     const int x = c.row0 + row, tok = x / p.per_kv;
     *head = c.kv_head * p.per_kv + (x - tok * p.per_kv);
@@ -171,7 +182,7 @@ template <typename T, int NT> struct RowWarp {
     }
   }
 
-  __device__ void run(long long u0, long long u1, uint32_t ring) {
+  __device__ void run(long long u0, long long u1, long long per, uint32_t ring) {
     const mk_chunk_attention_args& a = p.a;
     const int g = lane >> 2, t = lane & 3;
     Cursor ld, c;
@@ -354,6 +365,7 @@ template <typename T, int NT> struct RowWarp {
           }
         }
       }
+      if (c.from_start && !c.to_end) leave_merge(c, per);
       if (c.u < c.u_end) open(c);
     }
     cp_async_wait<0>();
@@ -366,6 +378,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) chunk_attention_rows(const __g
   long long* first = reinterpret_cast<long long*>(smem + kRowWarps * kWarpRing);
   __shared__ long long carry[kRowWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = p.a.requests;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the merge waits for this grid's end before it reads)
   long long total = 0;
   for (int r0 = 0; r0 < R; r0 += kRowThreads) {
     const int r = r0 + threadIdx.x;
@@ -394,101 +407,153 @@ __global__ void __launch_bounds__(kRowThreads, 1) chunk_attention_rows(const __g
   __syncthreads();
   long long per = (total + p.warps - 1) / p.warps;
   per = per > p.min_tiles ? per : p.min_tiles;
-  if (blockIdx.x == 0) {
-    for (int r = threadIdx.x; r <= R; r += kRowThreads) p.plan[1 + r] = first[r];
-    if (threadIdx.x == 0) p.plan[0] = per;
-  }
   // ranges that follow each other go to different SMs
   const int w = warp * gridDim.x + blockIdx.x;
   const long long u0 = w * per, u1 = min(total, u0 + per);
-  if (u0 >= u1) return;
-  RowWarp<T, NT>(p, first, w).run(u0, u1, (uint32_t)__cvta_generic_to_shared(smem + warp * kWarpRing));
-}
-
-// One CTA per group and kv head; warp i has the 16 dims of m-tile i.
-template <typename T, int NT>
-__global__ void __launch_bounds__(256) chunk_attention_merge(const __grid_constant__ AttnParams p) {
-  constexpr int ROWS = 8 * NT;
+  if (lane == 0) p.merges[w].last = -1;
+  if (u0 < u1) RowWarp<T, NT>(p, first, w).run(u0, u1, per, (uint32_t)__cvta_generic_to_shared(smem + warp * kWarpRing));
+  // (launched while the tile kernel may still run: the stream goes on when both are done)
   asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Joins the pieces of the groups that several warps have worked on, in the order of the positions.  The warp with a group's first piece has
+// left a record of it; a CTA looks at the records blockIdx + k gridDim.  Warp i of a CTA's first, second, ... eight has the 16 dims
+// of m-tile i and every first, second, ... of the pieces: one request with a long context has a hundred of them, and what they cost is
+// the latency of their loads, while with many groups a few pieces each it is the number of CTAs that counts.
+constexpr int kLookAhead = 8;
+template <typename T, int NT, int SHARES>
+__global__ void __launch_bounds__(256 * SHARES) chunk_attention_merge(const __grid_constant__ AttnParams p) {
+  constexpr int ROWS = 8 * NT;
+  __shared__ float4 joined[SHARES > 1 ? (SHARES - 1) * 8 * NT * 32 : 1];
   const mk_chunk_attention_args& a = p.a;
-  const int lane = threadIdx.x & 31, i = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  // request r has the slots from floor(first row / ROWS) + r on: as many as its groups at least
-  auto base = [&](int r) { return (long long)min(max(__ldg(a.qo_indptr + r), 0), a.tokens) * p.per_kv / ROWS + r; };
-  const int r = find_owner_warp(a.requests, blockIdx.x, base);
-  const Request q = request_of(a, r);
-  const Groups<ROWS> gr(p, q);
-  const long long group = blockIdx.x - base(r);
-  if (group < 0 || group >= gr.groups) return;
-  const long long per = p.plan[0], u0 = p.plan[1 + r] + ((long long)blockIdx.y * gr.groups + group) * gr.tiles, u1 = u0 + gr.tiles - 1;
-  const int w0 = (int)(u0 / per), w1 = (int)(u1 / per);
-  if (w0 == w1) return;  // the warp has written the outputs
-  // a warp's slot 1 holds the piece that begins a group, slot 0 the one that does not
-  auto part = [&](int w) { return p.partial + (size_t)(2 * w + (w * per <= u0 ? 1 : 0)) * part_floats(ROWS); };
-  float m[NT], l[NT];
-  float4 o[NT];
+  const int lane = threadIdx.x & 31, i = (threadIdx.x >> 5) & 7, share = threadIdx.x >> 8, g = lane >> 2, t = lane & 3;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int base = blockIdx.x; base < p.warps; base += kLookAhead * gridDim.x) {
+    const int mine = base + lane * (int)gridDim.x;
+    unsigned todo = __ballot_sync(kAll, lane < kLookAhead && mine < p.warps && p.merges[mine].last >= 0);
+    while (todo) {
+      const int w0 = base + (__ffs(todo) - 1) * (int)gridDim.x;
+      todo &= todo - 1;
+      const MergeRecord rec = p.merges[w0];
+      const int w1 = rec.last;
+      // a warp's slot 1 holds the piece that begins a group, slot 0 the one that does not
+      auto part = [&](int w) { return p.partial + (size_t)(2 * w + (w == w0 ? 1 : 0)) * part_floats(ROWS); };
+      float m[NT], l[NT];
+      float4 o[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    m[n] = -INFINITY;
-    for (int w = w0 + t; w <= w1; w += 4) m[n] = fmaxf(m[n], part(w)[ROWS * kHeadDim + 8 * n + g]);
-    m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 1));
-    m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 2));
-    l[n] = 0.f;
-    o[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-#pragma unroll 4
-  for (int w = w0; w <= w1; ++w) {
-    const float* pt = part(w);
+      for (int n = 0; n < NT; ++n) {
+        m[n] = -INFINITY;
+        for (int w = w0 + t; w <= w1; w += 4) m[n] = fmaxf(m[n], part(w)[ROWS * kHeadDim + 8 * n + g]);
+        m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 1));
+        m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 2));
+        l[n] = 0.f;
+        o[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      constexpr int U = 8 / NT;
+      for (int w = w0 + share * U; w <= w1; w += SHARES * U) {
+        float4 x[U][NT];
+        float mw[U][NT], lw[U][NT];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const float mw = pt[ROWS * kHeadDim + 8 * n + g], lw = pt[ROWS * kHeadDim + ROWS + 8 * n + g];
-      const float4 ow = reinterpret_cast<const float4*>(pt)[(n * 8 + i) * 32 + lane];
-      const float f = mw == -INFINITY ? 0.f : exp2f(mw - m[n]);
-      l[n] += f * lw;
-      const float f0 = __shfl_sync(kAll, f, 8 * t), f1 = __shfl_sync(kAll, f, 8 * t + 4);
-      // (a piece that saw nothing of a row has weight 0 and finite sums)
-      o[n].x += f0 * ow.x; o[n].y += f1 * ow.y;
-      o[n].z += f0 * ow.z; o[n].w += f1 * ow.w;
-    }
-  }
-  const int row0 = (int)group * ROWS, rows = (int)min((long long)ROWS, (long long)q.n * p.per_kv - row0);
+        for (int k = 0; k < U; ++k) {
+          const float* pt = part(min(w + k, w1));
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-    const float i0 = __shfl_sync(kAll, inv, 8 * t), i1 = __shfl_sync(kAll, inv, 8 * t + 4);
+          for (int n = 0; n < NT; ++n) {
+            x[k][n] = reinterpret_cast<const float4*>(pt)[(n * 8 + i) * 32 + lane];
+            mw[k][n] = w + k <= w1 ? pt[ROWS * kHeadDim + 8 * n + g] : -INFINITY;
+            lw[k][n] = pt[ROWS * kHeadDim + ROWS + 8 * n + g];
+          }
+        }
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int row = 8 * n + 2 * t + e;
-      if (row >= rows) continue;
-      const int x = row0 + row, tok = x / p.per_kv, head = blockIdx.y * p.per_kv + (x - tok * p.per_kv);
-      T* dst = (T*)a.out + (long long)(q.q0 + tok) * a.out_stride[0] + head * a.out_stride[1] + 16 * i + g;
-      dst[0] = from_float<T>((e ? o[n].y : o[n].x) * (e ? i1 : i0));
-      dst[8] = from_float<T>((e ? o[n].w : o[n].z) * (e ? i1 : i0));
-    }
-    const int row = 8 * n + g;
-    if (a.lse && i == 0 && t == 0 && row < rows) {
-      const int x = row0 + row, tok = x / p.per_kv, head = blockIdx.y * p.per_kv + (x - tok * p.per_kv);
-      a.lse[(long long)(q.q0 + tok) * a.lse_stride[0] + head * a.lse_stride[1]] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+        for (int k = 0; k < U; ++k)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            // (a piece that saw nothing of a row has weight 0; its sums are finite but for a NaN score, which has to stay)
+            const float f = mw[k][n] == -INFINITY ? 0.f : exp2f(mw[k][n] - m[n]);
+            if (w + k <= w1) l[n] += f * lw[k][n];
+            const float f0 = __shfl_sync(kAll, f, 8 * t), f1 = __shfl_sync(kAll, f, 8 * t + 4);
+            if (w + k <= w1) {
+              o[n].x += f0 * x[k][n].x; o[n].y += f1 * x[k][n].y;
+              o[n].z += f0 * x[k][n].z; o[n].w += f1 * x[k][n].w;
+            }
+          }
+      }
+      if constexpr (SHARES > 1) {
+        __shared__ float sums[SHARES][ROWS];
+        if (i == 0 && t == 0)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) sums[share][8 * n + g] = l[n];
+        if (share > 0)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) joined[(((share - 1) * 8 + i) * NT + n) * 32 + lane] = o[n];
+        __syncthreads();
+        if (share == 0) {
+#pragma unroll
+          for (int q = 1; q < SHARES; ++q)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float4 x = joined[(((q - 1) * 8 + i) * NT + n) * 32 + lane];
+              o[n].x += x.x; o[n].y += x.y;
+              o[n].z += x.z; o[n].w += x.w;
+              l[n] += sums[q][8 * n + g];
+            }
+        }
+        __syncthreads();
+        if (share > 0) continue;
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+        const float i0 = __shfl_sync(kAll, inv, 8 * t), i1 = __shfl_sync(kAll, inv, 8 * t + 4);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * n + 2 * t + e;
+          if (row >= rec.rows) continue;
+          const int x = rec.row0 + row, tok = x / p.per_kv, head = rec.kv_head * p.per_kv + (x - tok * p.per_kv);
+          T* dst = (T*)a.out + (long long)(rec.first_token + tok) * a.out_stride[0] + head * a.out_stride[1] + 16 * i + g;
+          dst[0] = from_float<T>((e ? o[n].y : o[n].x) * (e ? i1 : i0));
+          dst[8] = from_float<T>((e ? o[n].w : o[n].z) * (e ? i1 : i0));
+        }
+        const int row = 8 * n + g;
+        if (a.lse && i == 0 && t == 0 && row < rec.rows) {
+          const int x = rec.row0 + row, tok = x / p.per_kv, head = rec.kv_head * p.per_kv + (x - tok * p.per_kv);
+          a.lse[(long long)(rec.first_token + tok) * a.lse_stride[0] + head * a.lse_stride[1]] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+        }
+      }
     }
   }
 }
 
-template <typename T, int NT> int launch_rows(const AttnParams& p, cudaStream_t s) {
-  const int smem = kRowWarps * kWarpRing + (p.a.requests + 1) * 8;
-  cudaError_t e = cudaFuncSetAttribute(chunk_attention_rows<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: %s", cudaGetErrorString(e));
-  chunk_attention_rows<T, NT><<<p.warps / kRowWarps, kRowThreads, smem, s>>>(p);
-  if (int rc = launched("chunk_attention")) return rc;
-  // the merge may be set up while the rows are still being done; it waits for them itself
+cudaError_t launch_after(const void* kernel, dim3 grid, int threads, size_t smem, const AttnParams& p, cudaStream_t s) {
+  // may be set up, and begin, while the kernel before it still runs
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long long)p.a.tokens * p.per_kv / (8 * NT) + p.a.requests), (unsigned)p.a.kv_heads);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, chunk_attention_merge<T, NT>, p);
+  AttnParams copy = p;
+  void* args[1] = {&copy};
+  return cudaLaunchKernelExC(&cfg, kernel, args);
+}
+
+template <typename T, int NT> int launch_rows(const AttnParams& p, bool behind_tiles, cudaStream_t s) {
+  const int smem = kRowWarps * kWarpRing + (p.a.requests + 1) * 8;
+  cudaError_t e = cudaFuncSetAttribute(chunk_attention_rows<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: %s", cudaGetErrorString(e));
+  if (behind_tiles) {  // (the two write different rows; the kernel ahead of the tile kernel is done when that one begins)
+    e = launch_after((const void*)chunk_attention_rows<T, NT>, dim3(p.warps / kRowWarps), kRowThreads, smem, p, s);
+  } else {
+    chunk_attention_rows<T, NT><<<p.warps / kRowWarps, kRowThreads, smem, s>>>(p);
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: launch failed: %s", cudaGetErrorString(e));
+  // few groups: each in many pieces
+  if (p.a.requests * p.a.kv_heads <= 64) e = launch_after((const void*)chunk_attention_merge<T, NT, 4>, dim3(p.warps / kRowWarps), 1024, 0, p, s);
+  else e = launch_after((const void*)chunk_attention_merge<T, NT, 1>, dim3(p.warps), 256, 0, p, s);
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "chunk_attention: launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -513,8 +578,7 @@ Layout layout_of(const mk_chunk_attention_args& a) {
     const long long tokens = 2 * (128 / per_kv), ctas = (a.tokens + tokens - 1) / tokens * a.kv_heads;
     while (l.splits < 16 && 2 * l.splits * ctas <= sm_count()) l.splits *= 2;
   }
-  const size_t plan = ((size_t)(a.requests + 2) * 8 + 255) / 256 * 256;
-  l.partial = l.rows ? plan : 0;
+  l.partial = l.rows ? ((size_t)l.warps * sizeof(MergeRecord) + 255) / 256 * 256 : 0;
   l.tile_partial = l.partial + (l.rows ? (size_t)2 * l.warps * part_floats(8 * l.nt) * sizeof(float) : 0);
   l.bytes = l.tile_partial + (l.splits > 1 ? (size_t)l.splits * a.tokens * a.q_heads * (kHeadDim + 2) * sizeof(float) : 0);
   if (l.bytes == 0) l.bytes = 16;
@@ -567,7 +631,7 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   p.scale_log2 = a.scale * kLog2e;
   p.warps = l.warps;
   p.min_tiles = 4;
-  p.plan = reinterpret_cast<long long*>(a.workspace);
+  p.merges = reinterpret_cast<MergeRecord*>(a.workspace);
   p.partial = reinterpret_cast<float*>((char*)a.workspace + l.partial);
   p.few_rows = l.few_rows;
   p.splits = l.splits;
@@ -576,6 +640,7 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   if (l.tiles)
     if (int rc = launch_tile_attention(p, s)) return rc;
   if (!l.rows) return 0;
-  if (a.dtype == MK_BF16) return l.nt == 1 ? launch_rows<__nv_bfloat16, 1>(p, s) : launch_rows<__nv_bfloat16, 2>(p, s);
-  return l.nt == 1 ? launch_rows<__half, 1>(p, s) : launch_rows<__half, 2>(p, s);
+  const bool behind = l.tiles && l.splits == 1;
+  if (a.dtype == MK_BF16) return l.nt == 1 ? launch_rows<__nv_bfloat16, 1>(p, behind, s) : launch_rows<__nv_bfloat16, 2>(p, behind, s);
+  return l.nt == 1 ? launch_rows<__half, 1>(p, behind, s) : launch_rows<__half, 2>(p, behind, s);
 }

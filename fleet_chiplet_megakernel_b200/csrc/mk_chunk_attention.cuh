@@ -15,6 +15,12 @@ namespace mk_serving {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// What the warp with a group's first piece leaves for the merge; last = -1: no group of several pieces begins with this warp.
+struct MergeRecord {
+  int last;  // warp with the last piece
+  int kv_head, row0, rows, first_token;
+};
+
 struct AttnParams {
   mk_chunk_attention_args a;
   int per_kv;           // q heads of a kv head
@@ -23,7 +29,7 @@ struct AttnParams {
   int few_rows;         // requests with at most so many rows (new tokens x q heads of a kv head) are the row kernel's, others the tile kernel's
   int min_tiles;        // a warp's share of the row kernel is no shorter
   int warps;            // of the row kernel
-  long long* plan;      // row kernel -> merge: [tiles a warp][first tile of request 0 .. R]
+  MergeRecord* merges;  // row kernel -> merge, one a warp
   float* partial;       // of the row kernel's pieces
   int splits;           // of the tile kernel: pieces of every row's positions
   float* tile_partial;  // [splits][tokens][q heads][130]

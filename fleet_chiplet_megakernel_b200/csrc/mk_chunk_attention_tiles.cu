@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
   extern __shared__ unsigned char raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the row kernel takes the SMs as they become free
   // the CTA's rows: heaviest (last) rows of the batch first
   const int pieces = a.kv_heads * p.splits, tokens = 2 * tp.tokens_per_tile;
   const int slot = (int)(gridDim.x / pieces) - 1 - (int)(blockIdx.x / pieces), piece = blockIdx.x % pieces;
