@@ -3,10 +3,13 @@
 // Few rows (one new token per request up to short chunks).  The rows of a kv head (new tokens x its q heads) are cut into groups
 // of 8 or 16; a group has to walk over all K and V rows that it sees, 512 bytes and 4 x 128 x 8 multiplications a position:
 // bound by HBM as long as all SMs stream evenly.  So the unit of work is a tile of 16 positions of a group, and all units of
-// the batch are dealt out as contiguous ranges of equal length to warps, whatever the requests' lengths are: no CTA-wide
-// synchronisation, and one long request among short ones takes no longer than the sum says.  A warp that holds a group's whole
-// range writes its outputs; pieces of a group leave (max, sum, weighted V) in the workspace, and a second kernel merges them
-// in the order of the positions.  K and V tiles come by 16-byte cp.async into a ring of the warp's own, three deep.
+// the batch are dealt out as contiguous ranges of equal length to warps, whatever the requests' lengths are: no synchronisation while
+// the data streams, and one long request among short ones takes no longer than the sum says.  A warp that holds a group's whole
+// range writes its outputs; pieces of a group are joined in shared memory by the CTA when its warps are done, and what is left of groups
+// that several CTAs have worked on by a second kernel, both in the order of the positions.  K and V tiles come by 16-byte
+// cp.async into a ring of the warp's own, two tiles ahead of the sums and across the border between two groups.
+// (CTAs taking a group's tiles with all warps in turn, joined after every group: 46 us like this for long contexts, but twice the
+// time for short ones, 123 and 62 us, where what begins and ends a group is longer than the ring covers.)
 //
 // S = Q K^T with the rows on the M side of mma.m16n8k16, then O^T += V^T P^T with 16 dims on M, for which the scores are the B
 // operand as they are.  P enters as the sum of two 16-bit values (their product with V is cheap here, and the rounding of P would
@@ -20,8 +23,7 @@ namespace {
 constexpr int kRowWarps = 8, kRowThreads = 32 * kRowWarps;
 constexpr int kPos = 16;                          // positions of a tile
 constexpr int kTileBytes = kPos * kHeadDim * 2;   // of K, and of V behind it
-constexpr int kRing = 3;
-constexpr int kWarpRing = kRing * 2 * kTileBytes;
+constexpr int kBegin = 4;                         // units that a group counts more than its tiles: what beginning and ending one takes
 constexpr int kMaxRequests = MK_STEP_MAX_REQUESTS / 2;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
@@ -69,13 +71,110 @@ template <int ROWS> struct Groups {
 // 16 dims of m-tile i, dims g and g + 8 of rows 2 t and 2 t + 1 (and of the rows 8 further on)
 __host__ __device__ constexpr int part_floats(int rows) { return rows * kHeadDim + 2 * rows; }
 
-template <typename T, int NT> struct RowWarp {
+// Pieces of a group being joined by a warp, for the 16 dims of one m-tile: maximum and sum of rows g (and g + 8), weighted sums as the
+// fragments.  U: pieces whose loads are in flight together.
+template <int NT, int U> struct Joined {
   static constexpr int ROWS = 8 * NT;
+  float m[NT], l[NT];
+  float4 o[NT];
+  // part(q): piece q of n
+  template <typename F> __device__ __forceinline__ void add(const F& part, int n_parts, int tile, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      m[n] = -INFINITY;
+      l[n] = 0.f;
+      o[n] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll 1
+    for (int w = 0; w < n_parts; w += U) {
+      float4 x[U][NT];
+      float mw[U][NT], lw[U][NT];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const float* pt = part(min(w + k, n_parts - 1));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          x[k][n] = reinterpret_cast<const float4*>(pt)[(n * 8 + tile) * 32 + lane];
+          mw[k][n] = pt[ROWS * kHeadDim + 8 * n + g];
+          lw[k][n] = pt[ROWS * kHeadDim + ROWS + 8 * n + g];
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float top = m[n];
+#pragma unroll
+        for (int k = 0; k < U; ++k) top = fmaxf(top, mw[k][n]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float f = exp2f(m[n] - base);
+        m[n] = top;
+#pragma unroll
+        for (int k = 0; k < U; ++k) {
+          if (w + k >= n_parts) break;
+          // (a piece that saw nothing of a row has weight 0 and finite sums; a NaN score has left its mark in l)
+          const float fx = exp2f(mw[k][n] - base);
+          l[n] = l[n] * f + lw[k][n] * fx;
+          const float a0 = __shfl_sync(kAll, f, 8 * t), a1 = __shfl_sync(kAll, f, 8 * t + 4), b0 = __shfl_sync(kAll, fx, 8 * t), b1 = __shfl_sync(kAll, fx, 8 * t + 4);
+          const float4& y = x[k][n];
+          o[n].x = o[n].x * a0 + b0 * y.x; o[n].y = o[n].y * a1 + b1 * y.y;
+          o[n].z = o[n].z * a0 + b0 * y.z; o[n].w = o[n].w * a1 + b1 * y.w;
+          f = 1.f;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(float* pt, int tile, int lane) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      reinterpret_cast<float4*>(pt)[(n * 8 + tile) * 32 + lane] = o[n];
+      if (tile == 0 && (lane & 3) == 0) {
+        pt[ROWS * kHeadDim + 8 * n + (lane >> 2)] = m[n];
+        pt[ROWS * kHeadDim + ROWS + 8 * n + (lane >> 2)] = l[n];
+      }
+    }
+  }
+  // The rows of `rec`: outputs and logarithms of the sums.
+  template <typename T> __device__ __forceinline__ void write(const AttnParams& p, const MergeRecord& rec, int tile, int lane) const {
+    const mk_chunk_attention_args& a = p.a;
+    const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
+      const float i0 = __shfl_sync(kAll, inv, 8 * t), i1 = __shfl_sync(kAll, inv, 8 * t + 4);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 8 * n + 2 * t + e;
+        if (row >= rec.rows) continue;
+        const int x = rec.row0 + row, tok = x / p.per_kv, head = rec.kv_head * p.per_kv + (x - tok * p.per_kv);
+        T* dst = (T*)a.out + (long long)(rec.first_token + tok) * a.out_stride[0] + head * a.out_stride[1] + 16 * tile + g;
+        dst[0] = from_float<T>((e ? o[n].y : o[n].x) * (e ? i1 : i0));
+        dst[8] = from_float<T>((e ? o[n].w : o[n].z) * (e ? i1 : i0));
+      }
+      const int row = 8 * n + g;
+      if (a.lse && tile == 0 && t == 0 && row < rec.rows) {
+        const int x = rec.row0 + row, tok = x / p.per_kv, head = rec.kv_head * p.per_kv + (x - tok * p.per_kv);
+        a.lse[(long long)(rec.first_token + tok) * a.lse_stride[0] + head * a.lse_stride[1]] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
+      }
+    }
+  }
+};
+
+// RING: stages of a warp, three where shared memory has the room.
+template <typename T, int NT, int RING> struct RowWarp {
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int kRing = RING;
+  static constexpr int kWarpRing = kRing * 2 * kTileBytes;
+  static constexpr int kPartsBytes = kRowWarps * part_floats(ROWS) * (int)sizeof(float);
+  static int smem_bytes(int requests) { return kRowWarps * kWarpRing + kPartsBytes + (requests + 1) * 8; }
+  // Where a warp leaves its pieces for the CTA: the first, if its group has begun in another's range, in a place of its own, the last, if
+  // its group goes on, in the ring, which is done with by then.
+  static __device__ __forceinline__ float* piece(unsigned char* smem, int warp, bool from_start) {
+    return reinterpret_cast<float*>(from_start ? smem + warp * kWarpRing : smem + kRowWarps * kWarpRing + warp * part_floats(ROWS) * sizeof(float));
+  }
   const AttnParams& p;
   const long long* first;  // first unit of every request (shared memory)
+  unsigned char* smem;
   int lane, warp;
-
-  __device__ __forceinline__ RowWarp(const AttnParams& p_, const long long* f, int w) : p(p_), first(f), lane(threadIdx.x & 31), warp(w) {}
 
   // A piece: tiles k .. k_end of one group of one kv head; u units are behind this warp, it goes on to u_end.
   struct Cursor {
@@ -85,18 +184,20 @@ template <typename T, int NT> struct RowWarp {
     bool from_start, to_end;  // the piece has the group's first tile, its last
     __device__ __forceinline__ int position(int i) const { return i < sink ? i * kPos : start + (i - sink) * kPos; }
   };
-  // the piece that begins at unit c.u
+  // the piece that begins at unit c.u, or behind the units of a group's beginning there: c.u is moved to its first tile
   __device__ __forceinline__ void open(Cursor& c) const {
     c.r = find_owner(p.a.requests, c.u, [&](int i) { return first[i]; });
     c.q = request_of(p.a, c.r);
     const Groups<ROWS> g(p, c.q);
     const long long in = c.u - first[c.r];
-    const int item = (int)(in / g.tiles);
+    const int item = (int)(in / (g.tiles + kBegin)), x = (int)(in - (long long)item * (g.tiles + kBegin));
     c.tiles = g.tiles;
-    c.k = (int)(in - (long long)item * g.tiles);
+    c.k = max(0, x - kBegin);
     c.from_start = c.k == 0;
-    c.k_end = (int)min((long long)g.tiles, c.k + (c.u_end - c.u));
+    c.k_end = (int)min((long long)g.tiles, max(0ll, x - kBegin + (c.u_end - c.u)));
     c.to_end = c.k_end == g.tiles;
+    // (a range that ends within the units of a group's beginning has none of its tiles)
+    c.u = c.k_end > c.k ? c.u + max(0, kBegin - x) : c.u_end;
     c.kv_head = item / g.groups;
     c.group = item - c.kv_head * g.groups;
     c.row0 = c.group * ROWS;
@@ -109,43 +210,60 @@ template <typename T, int NT> struct RowWarp {
     c.count = s.count;
   }
 
-  // K and V rows of tile i of the cursor's piece -> stage; rows that are not there become zeros
-  __device__ __forceinline__ void load(const Cursor& c, int i, uint32_t stage) const {
-    const int pos = c.position(i) + (lane & 15);
-    int page, in_page;
-    locate(p, c.q, i < c.count ? pos : c.q.len, &page, &in_page);
+  // What a lane has to know of the tile that is loaded next: where a page holds whole tiles its page, else the page of position
+  // lane & 15.  Looked up a tile ahead: the address waits for it.
+  __device__ __forceinline__ int page_ahead(const Cursor& c) const {
+    if (c.k >= c.count) return -1;
+    const int pos = c.position(c.k) + (p.tile_in_page ? 0 : lane & 15);
+    if (pos >= c.q.len) return -1;
+    return __ldg(p.a.kv_indices + c.q.kv0 + (p.page_shift >= 0 ? pos >> p.page_shift : pos / p.a.page_size));
+  }
+  // K and V rows of the cursor's tile -> stage; rows that are not there become zeros
+  __device__ __forceinline__ void load(const Cursor& c, int page, uint32_t stage) const {
     const mk_chunk_attention_args& a = p.a;
+    const int start = c.position(c.k), live = c.k < c.count ? c.q.len - start : 0;  // rows of the tile that the request has
+    const bool known = (unsigned)page < (unsigned)a.pages;
     const T* kc = (const T*)a.k_cache + c.kv_head * a.k_cache_stride[2] + (lane & 7) * 8;
     const T* vc = (const T*)a.v_cache + c.kv_head * a.v_cache_stride[2] + (lane & 7) * 8;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    auto in_page = [&](int pos) { return p.page_shift >= 0 ? pos & (a.page_size - 1) : pos % a.page_size; };
+    // a lane copies 16 bytes of the rows lane / 8 + 4 j, of either half of the dims
+    auto copy = [&](int j, const T* kr, const T* vr, bool there) {
       const int row = (lane >> 3) + 4 * j;
-      const int pg = __shfl_sync(kAll, page, row), in = __shfl_sync(kAll, in_page, row);
-      const bool there = pg >= 0;
-      const T* kr = kc + (there ? (long long)pg * a.k_cache_stride[0] + (long long)in * a.k_cache_stride[1] : 0);
-      const T* vr = vc + (there ? (long long)pg * a.v_cache_stride[0] + (long long)in * a.v_cache_stride[1] : 0);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t dst = stage + (uint32_t)(row * 256 + ((((lane & 7) + 8 * half) ^ (row & 7)) << 4));
         cp_async16(dst, kr + 64 * half, there);
         cp_async16(dst + kTileBytes, vr + 64 * half, there);
       }
+    };
+    if (p.tile_in_page) {
+      const long long pg = known ? page : 0, in = in_page(start) + (lane >> 3);
+      const T *kr = kc + pg * a.k_cache_stride[0] + in * a.k_cache_stride[1], *vr = vc + pg * a.v_cache_stride[0] + in * a.v_cache_stride[1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) copy(j, kr + 4 * j * a.k_cache_stride[1], vr + 4 * j * a.v_cache_stride[1], known && (lane >> 3) + 4 * j < live);
+    } else {
+      const bool mine = known && (lane & 15) < live;
+      const long long pg = mine ? page : 0, in = mine ? in_page(start + (lane & 15)) : 0;
+      const long long ko = pg * a.k_cache_stride[0] + in * a.k_cache_stride[1], vo = pg * a.v_cache_stride[0] + in * a.v_cache_stride[1];
+      const unsigned there = __ballot_sync(kAll, mine);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = (lane >> 3) + 4 * j;
+        copy(j, kc + __shfl_sync(kAll, ko, row), vc + __shfl_sync(kAll, vo, row), there >> row & 1);
+      }
     }
   }
 
-  __device__ __forceinline__ float* slot_of(const Cursor& c) const {
-    return p.partial + (size_t)(2 * warp + (c.from_start ? 1 : 0)) * part_floats(ROWS);
-  }
-  // A group that begins here and goes on in other warps' ranges: what the merge needs to know of it.
-  __device__ __forceinline__ void leave_merge(const Cursor& c, long long per) const {
-    const int last = (int)((c.u - 1 + c.tiles - c.k_end) / per);  // (c.u: behind the piece)
-    if (lane == 0) {
-      p.merges[warp].last = last;
-      p.merges[warp].kv_head = c.kv_head;
-      p.merges[warp].row0 = c.row0;
-      p.merges[warp].rows = c.rows;
-      p.merges[warp].first_token = c.q.q0;
-    }
+  __device__ __forceinline__ float* slot_of(const Cursor& c) const { return piece(smem, warp, c.from_start); }
+  // A group that begins here and goes on in other warps' ranges, or that has come into this CTA's from the one before: what joining
+  // its pieces takes.
+  __device__ __forceinline__ void leave(const Cursor& c, long long per, MergeRecord* rec) const {
+    if (lane != 0) return;
+    rec->last = (int)((c.u - 1 + c.tiles - c.k_end) / per);  // warp with the group's last piece (c.u: behind this one)
+    rec->kv_head = c.kv_head;
+    rec->row0 = c.row0;
+    rec->rows = c.rows;
+    rec->first_token = c.q.q0;
   }
   __device__ __forceinline__ long long row_token(const Cursor& c, int row, int* head) const {
     const int x = c.row0 + row, tok = x / p.per_kv;
@@ -182,20 +300,24 @@ template <typename T, int NT> struct RowWarp {
     }
   }
 
-  __device__ void run(long long u0, long long u1, long long per, uint32_t ring) {
+  // came_in: record of the CTA's first piece, where its group has begun before; begun: of the group that this warp begins and does not end
+  __device__ void run(long long u0, long long u1, long long per, MergeRecord* came_in, MergeRecord* begun) {
     const mk_chunk_attention_args& a = p.a;
     const int g = lane >> 2, t = lane & 3;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem + warp * kWarpRing);
     Cursor ld, c;
     ld.u = c.u = u0;
     ld.u_end = c.u_end = u1;
     open(ld);
     c = ld;
     // The loader is kRing - 1 tiles ahead of the sums, across the border between two pieces.
+    int page = page_ahead(ld);
     auto load_next = [&](int stage) {
       if (ld.u < ld.u_end) {
-        load(ld, ld.k, ring + (uint32_t)(stage * 2 * kTileBytes));
+        load(ld, page, ring + (uint32_t)(stage * 2 * kTileBytes));
         ++ld.u;
         if (++ld.k == ld.k_end && ld.u < ld.u_end) open(ld);
+        if (ld.u < ld.u_end) page = page_ahead(ld);
       }
       cp_async_commit();
     };
@@ -365,17 +487,21 @@ template <typename T, int NT> struct RowWarp {
           }
         }
       }
-      if (c.from_start && !c.to_end) leave_merge(c, per);
+      if (c.from_start ? !c.to_end : came_in != nullptr) leave(c, per, c.from_start ? begun : came_in);
+      came_in = nullptr;
       if (c.u < c.u_end) open(c);
     }
     cp_async_wait<0>();
   }
 };
 
-template <typename T, int NT>
+template <typename T, int NT, int RING>
 __global__ void __launch_bounds__(kRowThreads, 1) chunk_attention_rows(const __grid_constant__ AttnParams p) {
+  using Warp = RowWarp<T, NT, RING>;
+  constexpr int ROWS = 8 * NT;
   extern __shared__ __align__(128) unsigned char smem[];
-  long long* first = reinterpret_cast<long long*>(smem + kRowWarps * kWarpRing);
+  __shared__ MergeRecord chains[kRowWarps + 1];
+  long long* first = reinterpret_cast<long long*>(smem + kRowWarps * Warp::kWarpRing + Warp::kPartsBytes);
   __shared__ long long carry[kRowWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, R = p.a.requests;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // (the merge waits for this grid's end before it reads)
@@ -385,7 +511,7 @@ __global__ void __launch_bounds__(kRowThreads, 1) chunk_attention_rows(const __g
     long long v = 0;
     if (r < R) {
       const Groups<8 * NT> g(p, request_of(p.a, r));
-      v = (long long)g.groups * g.tiles * p.a.kv_heads;
+      v = (long long)g.groups * (g.tiles + kBegin) * p.a.kv_heads;
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -405,122 +531,55 @@ __global__ void __launch_bounds__(kRowThreads, 1) chunk_attention_rows(const __g
   }
   if (threadIdx.x == 0) first[0] = 0;
   __syncthreads();
-  long long per = (total + p.warps - 1) / p.warps;
+  // Ranges that follow each other go to the warps of a CTA, whose pieces of a group are joined there.
+  const long long shares = (long long)gridDim.x * kRowWarps;
+  long long per = (total + shares - 1) / shares;
   per = per > p.min_tiles ? per : p.min_tiles;
-  // ranges that follow each other go to different SMs
-  const int w = warp * gridDim.x + blockIdx.x;
+  const int w = blockIdx.x * kRowWarps + warp, w_end = blockIdx.x * kRowWarps + kRowWarps - 1;
   const long long u0 = w * per, u1 = min(total, u0 + per);
-  if (lane == 0) p.merges[w].last = -1;
-  if (u0 < u1) RowWarp<T, NT>(p, first, w).run(u0, u1, per, (uint32_t)__cvta_generic_to_shared(smem + warp * kWarpRing));
+  if (lane == 0) chains[warp].last = -1;
+  if (threadIdx.x == 0) {
+    chains[kRowWarps].last = -1;
+    p.merges[blockIdx.x].last = -1;
+  }
+  __syncthreads();
+  if (u0 < u1) Warp{p, first, smem, lane, warp}.run(u0, u1, per, warp == 0 ? chains + kRowWarps : nullptr, chains + warp);
+  __syncthreads();
+  // The CTA's chains of pieces, the one that has come in first; a warp has 16 of the dims of each.
+#pragma unroll 1
+  for (int k = kRowWarps; k >= 0; --k) {
+    const MergeRecord rec = chains[k];
+    if (rec.last < 0) continue;
+    const bool came_in = k == kRowWarps;
+    const int k0 = came_in ? 0 : k, k1 = min(rec.last, w_end) - blockIdx.x * kRowWarps;
+    Joined<NT, 4> j;
+    j.add([&](int q) { return Warp::piece(smem, k0 + q, q == 0 && !came_in); }, k1 - k0 + 1, warp, lane);
+    if (!came_in && rec.last <= w_end) {
+      j.template write<T>(p, rec, warp, lane);
+    } else {
+      j.store(p.joined + (size_t)(2 * blockIdx.x + (came_in ? 0 : 1)) * part_floats(ROWS), warp, lane);
+      if (!came_in && threadIdx.x == 0) {
+        MergeRecord r = rec;
+        r.last = rec.last / kRowWarps;  // CTA with the last piece
+        p.merges[blockIdx.x] = r;
+      }
+    }
+  }
   // (launched while the tile kernel may still run: the stream goes on when both are done)
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// Joins the pieces of the groups that several warps have worked on, in the order of the positions.  The warp with a group's first piece has
-// left a record of it; a CTA looks at the records blockIdx + k gridDim.  Warp i of a CTA's first, second, ... eight has the 16 dims
-// of m-tile i and every first, second, ... of the pieces: one request with a long context has a hundred of them, and what they cost is
-// the latency of their loads, while with many groups a few pieces each it is the number of CTAs that counts.
-constexpr int kLookAhead = 8;
-template <typename T, int NT, int SHARES>
-__global__ void __launch_bounds__(256 * SHARES) chunk_attention_merge(const __grid_constant__ AttnParams p) {
-  constexpr int ROWS = 8 * NT;
-  __shared__ float4 joined[SHARES > 1 ? (SHARES - 1) * 8 * NT * 32 : 1];
-  const mk_chunk_attention_args& a = p.a;
-  const int lane = threadIdx.x & 31, i = (threadIdx.x >> 5) & 7, share = threadIdx.x >> 8, g = lane >> 2, t = lane & 3;
+// Joins what the CTAs of the row kernel have left of the groups that several of them have worked on, in the order of the positions.
+template <typename T, int NT>
+__global__ void __launch_bounds__(256) chunk_attention_merge(const __grid_constant__ AttnParams p) {
+  const int lane = threadIdx.x & 31, tile = threadIdx.x >> 5;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int base = blockIdx.x; base < p.warps; base += kLookAhead * gridDim.x) {
-    const int mine = base + lane * (int)gridDim.x;
-    unsigned todo = __ballot_sync(kAll, lane < kLookAhead && mine < p.warps && p.merges[mine].last >= 0);
-    while (todo) {
-      const int w0 = base + (__ffs(todo) - 1) * (int)gridDim.x;
-      todo &= todo - 1;
-      const MergeRecord rec = p.merges[w0];
-      const int w1 = rec.last;
-      // a warp's slot 1 holds the piece that begins a group, slot 0 the one that does not
-      auto part = [&](int w) { return p.partial + (size_t)(2 * w + (w == w0 ? 1 : 0)) * part_floats(ROWS); };
-      float m[NT], l[NT];
-      float4 o[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        m[n] = -INFINITY;
-        for (int w = w0 + t; w <= w1; w += 4) m[n] = fmaxf(m[n], part(w)[ROWS * kHeadDim + 8 * n + g]);
-        m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 1));
-        m[n] = fmaxf(m[n], __shfl_xor_sync(kAll, m[n], 2));
-        l[n] = 0.f;
-        o[n] = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      constexpr int U = 8 / NT;
-      for (int w = w0 + share * U; w <= w1; w += SHARES * U) {
-        float4 x[U][NT];
-        float mw[U][NT], lw[U][NT];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const float* pt = part(min(w + k, w1));
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            x[k][n] = reinterpret_cast<const float4*>(pt)[(n * 8 + i) * 32 + lane];
-            mw[k][n] = w + k <= w1 ? pt[ROWS * kHeadDim + 8 * n + g] : -INFINITY;
-            lw[k][n] = pt[ROWS * kHeadDim + ROWS + 8 * n + g];
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < U; ++k)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            // (a piece that saw nothing of a row has weight 0; its sums are finite but for a NaN score, which has to stay)
-            const float f = mw[k][n] == -INFINITY ? 0.f : exp2f(mw[k][n] - m[n]);
-            if (w + k <= w1) l[n] += f * lw[k][n];
-            const float f0 = __shfl_sync(kAll, f, 8 * t), f1 = __shfl_sync(kAll, f, 8 * t + 4);
-            if (w + k <= w1) {
-              o[n].x += f0 * x[k][n].x; o[n].y += f1 * x[k][n].y;
-              o[n].z += f0 * x[k][n].z; o[n].w += f1 * x[k][n].w;
-            }
-          }
-      }
-      if constexpr (SHARES > 1) {
-        __shared__ float sums[SHARES][ROWS];
-        if (i == 0 && t == 0)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) sums[share][8 * n + g] = l[n];
-        if (share > 0)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) joined[(((share - 1) * 8 + i) * NT + n) * 32 + lane] = o[n];
-        __syncthreads();
-        if (share == 0) {
-#pragma unroll
-          for (int q = 1; q < SHARES; ++q)
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float4 x = joined[(((q - 1) * 8 + i) * NT + n) * 32 + lane];
-              o[n].x += x.x; o[n].y += x.y;
-              o[n].z += x.z; o[n].w += x.w;
-              l[n] += sums[q][8 * n + g];
-            }
-        }
-        __syncthreads();
-        if (share > 0) continue;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        const float inv = l[n] == 0.f ? 0.f : 1.f / l[n];
-        const float i0 = __shfl_sync(kAll, inv, 8 * t), i1 = __shfl_sync(kAll, inv, 8 * t + 4);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = 8 * n + 2 * t + e;
-          if (row >= rec.rows) continue;
-          const int x = rec.row0 + row, tok = x / p.per_kv, head = rec.kv_head * p.per_kv + (x - tok * p.per_kv);
-          T* dst = (T*)a.out + (long long)(rec.first_token + tok) * a.out_stride[0] + head * a.out_stride[1] + 16 * i + g;
-          dst[0] = from_float<T>((e ? o[n].y : o[n].x) * (e ? i1 : i0));
-          dst[8] = from_float<T>((e ? o[n].w : o[n].z) * (e ? i1 : i0));
-        }
-        const int row = 8 * n + g;
-        if (a.lse && i == 0 && t == 0 && row < rec.rows) {
-          const int x = rec.row0 + row, tok = x / p.per_kv, head = rec.kv_head * p.per_kv + (x - tok * p.per_kv);
-          a.lse[(long long)(rec.first_token + tok) * a.lse_stride[0] + head * a.lse_stride[1]] = l[n] == 0.f ? -INFINITY : (m[n] + log2f(l[n])) * kLn2;
-        }
-      }
-    }
-  }
+  const MergeRecord rec = p.merges[blockIdx.x];
+  if (rec.last < 0) return;
+  auto part = [&](int q) { return p.joined + (size_t)(2 * (blockIdx.x + q) + (q == 0 ? 1 : 0)) * part_floats(8 * NT); };
+  Joined<NT, 8 / NT> j;
+  j.add(part, rec.last - (int)blockIdx.x + 1, tile, lane);
+  j.template write<T>(p, rec, tile, lane);
 }
 
 cudaError_t launch_after(const void* kernel, dim3 grid, int threads, size_t smem, const AttnParams& p, cudaStream_t s) {
@@ -540,20 +599,22 @@ cudaError_t launch_after(const void* kernel, dim3 grid, int threads, size_t smem
   return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
-template <typename T, int NT> int launch_rows(const AttnParams& p, bool behind_tiles, cudaStream_t s) {
-  const int smem = kRowWarps * kWarpRing + (p.a.requests + 1) * 8;
-  cudaError_t e = cudaFuncSetAttribute(chunk_attention_rows<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+constexpr int kMostSmem = 232448;  // of a CTA
+template <typename T, int NT, int RING> int launch_rows(const AttnParams& p, bool behind_tiles, cudaStream_t s) {
+  const int smem = RowWarp<T, NT, RING>::smem_bytes(p.a.requests);
+  if constexpr (RING > 2) {
+    if (smem > kMostSmem) return launch_rows<T, NT, RING - 1>(p, behind_tiles, s);  // (some hundreds of requests)
+  }
+  cudaError_t e = cudaFuncSetAttribute(chunk_attention_rows<T, NT, RING>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: %s", cudaGetErrorString(e));
   if (behind_tiles) {  // (the two write different rows; the kernel ahead of the tile kernel is done when that one begins)
-    e = launch_after((const void*)chunk_attention_rows<T, NT>, dim3(p.warps / kRowWarps), kRowThreads, smem, p, s);
+    e = launch_after((const void*)chunk_attention_rows<T, NT, RING>, dim3(p.row_ctas), kRowThreads, smem, p, s);
   } else {
-    chunk_attention_rows<T, NT><<<p.warps / kRowWarps, kRowThreads, smem, s>>>(p);
+    chunk_attention_rows<T, NT, RING><<<p.row_ctas, kRowThreads, smem, s>>>(p);
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: launch failed: %s", cudaGetErrorString(e));
-  // few groups: each in many pieces
-  if (p.a.requests * p.a.kv_heads <= 64) e = launch_after((const void*)chunk_attention_merge<T, NT, 4>, dim3(p.warps / kRowWarps), 1024, 0, p, s);
-  else e = launch_after((const void*)chunk_attention_merge<T, NT, 1>, dim3(p.warps), 256, 0, p, s);
+  e = launch_after((const void*)chunk_attention_merge<T, NT>, dim3(p.row_ctas), 256, 0, p, s);
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "chunk_attention: launch failed: %s", cudaGetErrorString(e));
 }
 
@@ -561,8 +622,8 @@ template <typename T, int NT> int launch_rows(const AttnParams& p, bool behind_t
 constexpr int kFewRows = 32;
 struct Layout {
   bool rows, tiles;
-  int nt, few_rows, warps, splits;
-  size_t partial, tile_partial, bytes;
+  int nt, few_rows, row_ctas, splits;
+  size_t joined, tile_partial, bytes;
 };
 Layout layout_of(const mk_chunk_attention_args& a) {
   Layout l = {};
@@ -572,14 +633,14 @@ Layout layout_of(const mk_chunk_attention_args& a) {
   l.rows = !l.tiles || a.requests > 1;
   l.few_rows = !l.tiles ? 0x7fffffff : l.rows ? kFewRows : 0;
   l.nt = most * per_kv <= 8 ? 1 : 2;
-  l.warps = sm_count() * kRowWarps;
+  l.row_ctas = sm_count();
   l.splits = 1;
   if (l.tiles) {
     const long long tokens = 2 * (128 / per_kv), ctas = (a.tokens + tokens - 1) / tokens * a.kv_heads;
     while (l.splits < 16 && 2 * l.splits * ctas <= sm_count()) l.splits *= 2;
   }
-  l.partial = l.rows ? ((size_t)l.warps * sizeof(MergeRecord) + 255) / 256 * 256 : 0;
-  l.tile_partial = l.partial + (l.rows ? (size_t)2 * l.warps * part_floats(8 * l.nt) * sizeof(float) : 0);
+  l.joined = l.rows ? (l.row_ctas * sizeof(MergeRecord) + 255) / 256 * 256 : 0;
+  l.tile_partial = l.joined + (l.rows ? 2 * l.row_ctas * part_floats(8 * l.nt) * sizeof(float) : 0);
   l.bytes = l.tile_partial + (l.splits > 1 ? (size_t)l.splits * a.tokens * a.q_heads * (kHeadDim + 2) * sizeof(float) : 0);
   if (l.bytes == 0) l.bytes = 16;
   return l;
@@ -629,10 +690,11 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   for (int s = 0; s < 31; ++s)
     if (a.page_size == 1 << s) p.page_shift = s;
   p.scale_log2 = a.scale * kLog2e;
-  p.warps = l.warps;
-  p.min_tiles = 4;
+  p.row_ctas = l.row_ctas;
+  p.tile_in_page = a.page_size % kPos == 0;
+  p.min_tiles = 2;
   p.merges = reinterpret_cast<MergeRecord*>(a.workspace);
-  p.partial = reinterpret_cast<float*>((char*)a.workspace + l.partial);
+  p.joined = reinterpret_cast<float*>((char*)a.workspace + l.joined);
   p.few_rows = l.few_rows;
   p.splits = l.splits;
   p.tile_partial = reinterpret_cast<float*>((char*)a.workspace + l.tile_partial);
@@ -641,6 +703,7 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
     if (int rc = launch_tile_attention(p, s)) return rc;
   if (!l.rows) return 0;
   const bool behind = l.tiles && l.splits == 1;
-  if (a.dtype == MK_BF16) return l.nt == 1 ? launch_rows<__nv_bfloat16, 1>(p, behind, s) : launch_rows<__nv_bfloat16, 2>(p, behind, s);
-  return l.nt == 1 ? launch_rows<__half, 1>(p, behind, s) : launch_rows<__half, 2>(p, behind, s);
+  // (two stages beside the parts of 16 rows)
+  if (a.dtype == MK_BF16) return l.nt == 1 ? launch_rows<__nv_bfloat16, 1, 3>(p, behind, s) : launch_rows<__nv_bfloat16, 2, 2>(p, behind, s);
+  return l.nt == 1 ? launch_rows<__half, 1, 3>(p, behind, s) : launch_rows<__half, 2, 2>(p, behind, s);
 }

@@ -15,22 +15,23 @@ namespace mk_serving {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// What the warp with a group's first piece leaves for the merge; last = -1: no group of several pieces begins with this warp.
+// Pieces of a group that are to be joined: the warp, or CTA, with the last one (-1: none), and the group's rows.
 struct MergeRecord {
-  int last;  // warp with the last piece
+  int last;
   int kv_head, row0, rows, first_token;
 };
 
 struct AttnParams {
   mk_chunk_attention_args a;
   int per_kv;           // q heads of a kv head
+  bool tile_in_page;    // a page holds whole tiles of the row kernel
   int page_shift;       // log2 of the page size, -1 if it is no power of two
   float scale_log2;     // scale * log2(e): scores and maxima are kept in base 2
   int few_rows;         // requests with at most so many rows (new tokens x q heads of a kv head) are the row kernel's, others the tile kernel's
   int min_tiles;        // a warp's share of the row kernel is no shorter
-  int warps;            // of the row kernel
-  MergeRecord* merges;  // row kernel -> merge, one a warp
-  float* partial;       // of the row kernel's pieces
+  int row_ctas;         // of the row kernel
+  MergeRecord* merges;  // row kernel -> merge: of the group that a CTA begins and does not end
+  float* joined;        // its pieces, two a CTA (of a group from the CTA before, of one that goes on in the next)
   int splits;           // of the tile kernel: pieces of every row's positions
   float* tile_partial;  // [splits][tokens][q heads][130]
 };
