@@ -8,7 +8,8 @@
 //   warp 8           loads: Q once, then K and V tiles through a ring of five 32 KB stages; a box is as much of a page as a tile holds
 //   warp 9           tcgen05.mma: S = Q K^T (both from shared memory), O += P V (P from tensor memory, V with the dims on the N side as
 //                    it lies in the cache); while one row tile is in its softmax the other one's products run
-// Tensor memory: S and O of both row tiles, 4 x 128 columns; P overwrites the S that it comes from.  O is scaled only when a
+// Tensor memory: S and O of both row tiles, 4 x 128 columns; P overwrites the S that it comes from, and
+// its product with V begins with the first 64 positions.  O is scaled only when a
 // row's maximum has grown by more than 2^8 over the one in use: until then weights above 1 are as good as any, the sum has them too.
 // P is rounded to the type of V, which adds as much error as the rounding of the output; everything else is fp32.
 // V rows behind a request's last position are cleared in shared memory (weight 0 times NaN is NaN); pieces whose sums are not
@@ -132,6 +133,35 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// two fp32 values in a register pair
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Bit e: position first + e is seen by a row at position at, 0 <= e < 32.
+__device__ __forceinline__ uint32_t seen_bits(const mk_chunk_attention_args& a, int first, int at) {
+  auto below = [](long long n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << (int)n) - 1u; };  // bits 0 .. n - 1
+  uint32_t bits = below((long long)at - first + 1);
+  if (a.window) bits &= ~below((long long)at - a.window + 1 - first) | below((long long)a.sinks - first);
+  return bits;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const __grid_constant__ TileParams tp) {
   const AttnParams& p = tp.p;
@@ -157,7 +187,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
 
   const uint32_t smem = (smem_addr(raw) + 1023u) & ~1023u;
   const uint32_t sq = smem, skv = smem + 2 * kStageBytes, bars = skv + kStages * kStageBytes;
-  const uint32_t q_full = bars, tail_full = bars + 8, s_full = bars + 16, p_full = bars + 32, o_full = bars + 48, kv_full = bars + 64, kv_empty = kv_full + 8 * kStages;
+  const uint32_t q_full = bars, tail_full = bars + 8, s_full = bars + 16, p_full = bars + 32, o_full = bars + 64, kv_full = bars + 80, kv_empty = kv_full + 8 * kStages;
   const uint32_t tm_slot = kv_empty + 8 * kStages;
   volatile int* dead = reinterpret_cast<volatile int*>(raw + (tm_slot + 8 - smem_addr(raw)));
   if (tid == 0) {
@@ -165,7 +195,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     bar_init(tail_full, 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(s_full + 8 * i, 1);
-      bar_init(p_full + 8 * i, kTile);
+      bar_init(p_full + 16 * i, kTile);      // the first half of the positions, the second
+      bar_init(p_full + 16 * i + 8, kTile);
       bar_init(o_full + 8 * i, 1);
     }
     for (int i = 0; i < kStages; ++i) {
@@ -262,10 +293,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       }
       __syncwarp();
     };
-    auto sums = [&](int w, uint32_t v, bool add) {  // O_w += P_w V
+    auto sums = [&](int w, uint32_t v, bool add, int half) {  // O_w += P_w V over half of the positions
       if (elect()) {
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) mma_ts(tm_o + 128 * w, tm + 128 * w + 8 * ks, desc_mn(v + ks * 2048), pv, add || ks > 0);
+        for (int ks = 0; ks < 4; ++ks) {
+          const int k = 4 * half + ks;
+          mma_ts(tm_o + 128 * w, tm + 128 * w + 8 * k, desc_mn(v + k * 2048), pv, add || k > 0);
+        }
       }
       __syncwarp();
     };
@@ -290,10 +324,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         if (w && !two) break;
-        ok = ok && bar_wait(p_full + 8 * w, i & 1, dead);
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && bar_wait(p_full + 16 * w + 8 * half, i & 1, dead);
+          if (!ok) break;
+          fence_after();
+          sums(w, v, i > 0, half);
+        }
         if (!ok) break;
-        fence_after();
-        sums(w, v, i > 0);
         if (!more) release(o_full + 8 * w);
         if (more && w == 0) ok = bar_wait(kv_full + 8 * stage, parity, dead);
         if (!ok) break;
@@ -325,24 +362,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
         break;
       }
       fence_after();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tm_load(ts + 32 * c, s[c]);
-      tm_wait_load();
       const int start = span.position(k0 + i);
-      if (!(start + kTile - 1 <= at0 && (a.window == 0 || start > (long long)at1 - a.window || start + kTile <= a.sinks))) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            if (!sees(a, start + 32 * c + e, at)) s[c][e] = 0xff800000u;
-      }
+      const bool masked = !(start + kTile - 1 <= at0 && (a.window == 0 || start > (long long)at1 - a.window || start + kTile <= a.sinks));
+      uint32_t s[4][32];
       float mx[4];
+      // the maximum of a quarter while the next is on its way
+      tm_load(ts, s[0]);
+      tm_wait_load();
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        mx[c] = __uint_as_float(s[c][0]);
+        if (c < 3) tm_load(ts + 32 * (c + 1), s[c + 1]);
+        if (masked) {
+          const uint32_t bits = seen_bits(a, start + 32 * c, at);
 #pragma unroll
-        for (int e = 1; e < 32; ++e) mx[c] = fmaxf(mx[c], __uint_as_float(s[c][e]));
+          for (int e = 0; e < 32; ++e) s[c][e] = bits >> e & 1 ? s[c][e] : 0xff800000u;
+        }
+        float x = __uint_as_float(s[c][0]), y = __uint_as_float(s[c][1]);
+#pragma unroll
+        for (int e = 2; e < 32; e += 4) {
+          x = fmaxf(fmaxf(x, __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
+          if (e + 2 < 32) y = fmaxf(fmaxf(y, __uint_as_float(s[c][e + 2])), __uint_as_float(s[c][e + 3]));
+        }
+        mx[c] = fmaxf(x, y);
+        if (c < 3) tm_wait_load();
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
       const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
@@ -363,23 +405,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         uint32_t w16[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15)]), p.scale_log2, -base));
-          const float y = ex2(fmaf(__uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15) + 1]), p.scale_log2, -base));
-          sum[e & 3] += x + y;
-          w16[e] = pack2<T>(x, y);
+          const float2 y = unpair(fma2(pair(__uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15)]), __uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15) + 1])), scale2, base2));
+          const float2 x = make_float2(ex2(y.x), ex2(y.y));
+          sum[e & 1] = add2(sum[e & 1], pair(x.x, x.y));
+          w16[e] = pack2<T>(x.x, x.y);
         }
         tm_store(ts + 32 * c, w16);
+        tm_wait_store();
+        fence_before();
+        bar_arrive(p_full + 16 * w + 8 * c);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tm_wait_store();
-      fence_before();
-      bar_arrive(p_full + 8 * w);
+      const float2 both = unpair(add2(sum[0], sum[1]));
+      l += both.x + both.y;
     }
     // ---- the rows' outputs
     if (ok && n > 0) ok = bar_wait(o_full + 8 * w, 0, dead);
