@@ -26,8 +26,8 @@ constexpr int kTile = 128;                       // rows, and positions
 constexpr int kHalfBytes = kTile * 128;          // 128 rows of 64 elements, 128-byte swizzle
 constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 5;
-constexpr int kTileThreads = 320;
-constexpr int kSmemBytes = 2 * kStageBytes + kStages * kStageBytes + 1024 + 256;
+constexpr int kTileThreads = 320, kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kSmemBytes = 2 * kStageBytes + kStages * kStageBytes + 256;
 constexpr unsigned long long kWaitNs = 2000000000ull;  // a wait that takes longer has lost its partner
 constexpr float kGrow = 8.f;                     // log2 of the weights that a stale maximum may lead to
 
@@ -119,11 +119,11 @@ __device__ __forceinline__ void tm_load(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tm_store(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::MK_I8(0),
-      MK_I8(8), MK_I8(16), MK_I8(24), "r"(taddr)
-      : "memory");
+__device__ __forceinline__ void tm_load16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];" : MK_R8(0), MK_R8(8) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tm_store16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::MK_I8(0), MK_I8(8), "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void tm_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tm_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -166,7 +166,7 @@ template <typename T>
 __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const __grid_constant__ TileParams tp) {
   const AttnParams& p = tp.p;
   const mk_chunk_attention_args& a = p.a;
-  extern __shared__ unsigned char raw[];
+  extern __shared__ __align__(1024) unsigned char raw[];  // (the swizzle's groups of 8 rows)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the row kernel takes the SMs as they become free
@@ -185,12 +185,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
   const int k0 = (int)((long long)span.count * split / p.splits), k1 = (int)((long long)span.count * (split + 1) / p.splits);
   const int n = k1 - k0;
 
-  const uint32_t smem = (smem_addr(raw) + 1023u) & ~1023u;
+  const uint32_t smem = smem_addr(raw);
   const uint32_t sq = smem, skv = smem + 2 * kStageBytes, bars = skv + kStages * kStageBytes;
   const uint32_t q_full = bars, tail_full = bars + 8, s_full = bars + 16, p_full = bars + 32, o_full = bars + 64, kv_full = bars + 80, kv_empty = kv_full + 8 * kStages;
   const uint32_t tm_slot = kv_empty + 8 * kStages;
-  volatile int* dead = reinterpret_cast<volatile int*>(raw + (tm_slot + 8 - smem_addr(raw)));
-  if (tid == 0) {
+  volatile int* dead = reinterpret_cast<volatile int*>(raw + (tm_slot + 8 - smem));
+  if (tid == 32 * kLoadWarp) {
     bar_init(q_full, 1);
     bar_init(tail_full, 1);
     for (int i = 0; i < 2; ++i) {
@@ -206,9 +206,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     *dead = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(tm_slot) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == kLoadWarp) {  // (Q needs nothing of the others)
+    __syncwarp();
+    if (n > 0 && elect()) {
+      const uint32_t bytes = (uint32_t)(p.per_kv * tp.tokens_per_tile * 256);
+      bar_expect(q_full, two ? 2 * bytes : bytes);
+      for (int i = 0; i < (two ? 2 : 1); ++i)
+        for (int h = 0; h < 2; ++h)
+          load_box3(sq + i * kStageBytes + h * kHalfBytes, &tp.q, q_full, 64 * h, kv_head * p.per_kv, q.q0 + t0 + i * tp.tokens_per_tile);
+    }
   }
   fence_before();
   __syncthreads();
@@ -217,15 +227,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tm) : "r"(tm_slot));
   const uint32_t tm_o = tm + 256;
 
-  if (n > 0 && warp == 8) {
+  if (n > 0 && warp == kLoadWarp) {
     // ---- loads
-    if (elect()) {
-      const uint32_t bytes = (uint32_t)(p.per_kv * tp.tokens_per_tile * 256);
-      bar_expect(q_full, two ? 2 * bytes : bytes);
-      for (int i = 0; i < (two ? 2 : 1); ++i)
-        for (int h = 0; h < 2; ++h)
-          load_box3(sq + i * kStageBytes + h * kHalfBytes, &tp.q, q_full, 64 * h, kv_head * p.per_kv, q.q0 + t0 + i * tp.tokens_per_tile);
-    }
     const int boxes = kTile / tp.box;           // of a half tile: at most 16
     const int rg = lane % boxes, half = lane / boxes;
     int stage = 0, parity = 1, sent = 0;  // (the first round of empty waits passes)
@@ -269,7 +272,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       bar_wait_slow(q_full, 0, &none);
       for (int k = max(0, sent - kStages); k < sent; ++k) bar_wait_slow(kv_full + 8 * (k % kStages), (k / kStages) & 1, &none);
     }
-  } else if (n > 0 && warp == 9) {
+  } else if (n > 0 && warp == kMmaWarp) {
     // ---- products
     constexpr uint32_t type = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
     constexpr uint32_t qk = (1u << 4) | (type << 7) | (type << 10) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);
@@ -353,8 +356,69 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     const int at0 = q.len - q.n + t0 + w * tp.tokens_per_tile, at1 = min(at0 + tp.tokens_per_tile, q.len - q.n + t0 + live) - 1;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t ts = tm + 128 * w + lanes, to = tm_o + 128 * w + lanes;
-    float m = -INFINITY, l = 0.f;
+    // Weights are exp2(score - base).  The base is a maximum of the row's scores that may lag behind: it moves when a score is more
+    // than 2^kGrow above it, and no weight is lost meanwhile as long as the type holds it.  bf16 has the range of fp32, so there the
+    // scores of a tile are weighed with the base that the tiles before have left, as they come out of tensor memory, and
+    // their maximum moves the base for the next tile; fp16 has no such range, and its tiles are looked through first.
+    // (A weight that is too large even so makes the row's sums infinite, and exact_row does it again.)
+    constexpr bool kLag = __is_same(T, __nv_bfloat16);
+    bool unset = mine;
+    float base = 0.f, l = 0.f, top = -INFINITY;
     bool ok = true;
+    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+    uint64_t sum[2] = {0, 0};
+    auto hide = [&](uint32_t (&s)[32], int first) {
+      const uint32_t bits = seen_bits(a, first, at);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) s[e] = bits >> e & 1 ? s[e] : 0xff800000u;
+    };
+    auto largest = [&](const uint32_t (&s)[32]) -> float {
+      float x = __uint_as_float(s[0]), y = __uint_as_float(s[1]);
+#pragma unroll
+      for (int e = 2; e < 32; e += 4) {
+        x = fmaxf(fmaxf(x, __uint_as_float(s[e])), __uint_as_float(s[e + 1]));
+        if (e + 2 < 32) y = fmaxf(fmaxf(y, __uint_as_float(s[e + 2])), __uint_as_float(s[e + 3]));
+      }
+      return fmaxf(x, y);
+    };
+    auto weigh = [&](const uint32_t (&s)[32], int c) {  // the weights of quarter c of a tile
+      const uint64_t base2 = pair(-base, -base);
+      uint32_t w16[16];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float2 y = unpair(fma2(pair(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), scale2, base2));
+        const float2 x = make_float2(ex2(y.x), ex2(y.y));
+        sum[e & 1] = add2(sum[e & 1], pair(x.x, x.y));
+        w16[e] = pack2<T>(x.x, x.y);
+      }
+      tm_store16(ts + 16 * c, w16);
+      if (c & 1) {  // half of the positions: their product with V can begin
+        tm_wait_store();
+        fence_before();
+        bar_arrive(p_full + 16 * w + 4 * (c - 1));
+      }
+    };
+    // the base of a row that has moved; what there is of the row's sums follows
+    auto move_base = [&](bool sums) {
+      const bool grow = top > base + kGrow || (unset && top > -INFINITY);
+      if (!__any_sync(kAll, grow)) return;
+      const float alpha = !grow ? 1.f : unset ? 0.f : ex2(base - top);  // (no weight yet: whatever there is, is zero)
+      if (grow) {
+        base = top;
+        unset = false;
+      }
+      l *= alpha;
+      if (!sums) return;
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        uint32_t o[16];
+        tm_load16(to + 16 * c, o);
+        tm_wait_load();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+        tm_store16(to + 16 * c, o);
+      }
+    };
     for (int i = 0; i < n; ++i) {
       ok = bar_wait(s_full + 8 * w, i & 1, dead);
       if (!__all_sync(kAll, ok)) {
@@ -364,67 +428,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       fence_after();
       const int start = span.position(k0 + i);
       const bool masked = !(start + kTile - 1 <= at0 && (a.window == 0 || start > (long long)at1 - a.window || start + kTile <= a.sinks));
-      uint32_t s[4][32];
-      float mx[4];
-      // the maximum of a quarter while the next is on its way
-      tm_load(ts, s[0]);
+      uint32_t s[2][32];
+      if constexpr (kLag) move_base(i > 0);
+      if (!kLag || __any_sync(kAll, unset)) {  // (kLag: the first tile; rows whose first tiles are all hidden)
+        tm_load(ts, s[0]);
+        tm_wait_load();
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (c < 3) tm_load(ts + 32 * (c + 1), s[(c + 1) & 1]);
+          if (masked) hide(s[c & 1], start + 32 * c);
+          mx = fmaxf(mx, largest(s[c & 1]));
+          if (c < 3) tm_wait_load();
+        }
+        top = mx * p.scale_log2;
+        tm_load(ts, s[0]);  // (for the weights)
+        move_base(i > 0);
+      } else {
+        tm_load(ts, s[0]);
+      }
+      float mx = -INFINITY;
       tm_wait_load();
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (c < 3) tm_load(ts + 32 * (c + 1), s[c + 1]);
-        if (masked) {
-          const uint32_t bits = seen_bits(a, start + 32 * c, at);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) s[c][e] = bits >> e & 1 ? s[c][e] : 0xff800000u;
-        }
-        float x = __uint_as_float(s[c][0]), y = __uint_as_float(s[c][1]);
-#pragma unroll
-        for (int e = 2; e < 32; e += 4) {
-          x = fmaxf(fmaxf(x, __uint_as_float(s[c][e])), __uint_as_float(s[c][e + 1]));
-          if (e + 2 < 32) y = fmaxf(fmaxf(y, __uint_as_float(s[c][e + 2])), __uint_as_float(s[c][e + 3]));
-        }
-        mx[c] = fmaxf(x, y);
+        if (c < 3) tm_load(ts + 32 * (c + 1), s[(c + 1) & 1]);
+        if (masked) hide(s[c & 1], start + 32 * c);
+        if constexpr (kLag) mx = fmaxf(mx, largest(s[c & 1]));
+        weigh(s[c & 1], c);
         if (c < 3) tm_wait_load();
       }
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-      const bool grow = top > m + kGrow || (m == -INFINITY && top > m);
-      if (__any_sync(kAll, grow)) {
-        const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
-        if (grow) m = top;
-        l *= alpha;
-        if (i > 0) {
-#pragma unroll 1
-          for (int c = 0; c < 4; ++c) {
-            uint32_t o[32];
-            tm_load(to + 32 * c, o);
-            tm_wait_load();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tm_store(to + 32 * c, o);
-          }
-        }
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
-      uint64_t sum[2] = {0, 0};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w16[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float2 y = unpair(fma2(pair(__uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15)]), __uint_as_float(s[2 * c + (e >> 4)][2 * (e & 15) + 1])), scale2, base2));
-          const float2 x = make_float2(ex2(y.x), ex2(y.y));
-          sum[e & 1] = add2(sum[e & 1], pair(x.x, x.y));
-          w16[e] = pack2<T>(x.x, x.y);
-        }
-        tm_store(ts + 32 * c, w16);
-        tm_wait_store();
-        fence_before();
-        bar_arrive(p_full + 16 * w + 8 * c);
-      }
+      if constexpr (kLag) top = mx * p.scale_log2;
       const float2 both = unpair(add2(sum[0], sum[1]));
       l += both.x + both.y;
+      sum[0] = sum[1] = 0;
     }
+    const float m = l == 0.f ? -INFINITY : base;
     // ---- the rows' outputs
     if (ok && n > 0) ok = bar_wait(o_full + 8 * w, 0, dead);
     ok = __all_sync(kAll, ok);
@@ -499,7 +537,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
   }
   fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
   }
