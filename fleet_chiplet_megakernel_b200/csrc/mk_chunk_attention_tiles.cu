@@ -133,27 +133,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// two fp32 values in a register pair
-__device__ __forceinline__ uint64_t pair(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ float2 unpair(uint64_t v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 // Bit e: position first + e is seen by a row at position at, 0 <= e < 32.
 __device__ __forceinline__ uint32_t seen_bits(const mk_chunk_attention_args& a, int first, int at) {
   auto below = [](long long n) -> uint32_t { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << (int)n) - 1u; };  // bits 0 .. n - 1

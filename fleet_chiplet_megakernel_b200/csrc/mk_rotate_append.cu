@@ -12,106 +12,172 @@ namespace mk_serving {
 namespace {
 
 constexpr int kRowLanes = 8;
-constexpr int kRotThreads = 256;
+constexpr int kRotThreads = 128;
+constexpr int kRows = 4;  // of a lane on their way together
 
-template <typename T, bool WIDE> __device__ __forceinline__ void load8(const T* p, float* f) {
-  if constexpr (WIDE && sizeof(T) == 2) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+// Eight elements as they lie in memory, so that several rows can be on their way in few registers.
+template <typename T> struct Raw {
+  uint4 w[sizeof(T) / 2];
+  template <bool WIDE> __device__ __forceinline__ void load(const T* p) {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 d = unpack2<T>(w[i]);
-      f[2 * i] = d.x;
-      f[2 * i + 1] = d.y;
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k) w[k] = reinterpret_cast<const uint4*>(p)[k];
+    } else {
+      T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
     }
-  } else if constexpr (WIDE) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_float(p[i]);
   }
-}
-template <typename T, bool WIDE> __device__ __forceinline__ void store8(T* p, const float* f) {
-  if constexpr (WIDE) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(f[0], f[1]), pack2<T>(f[2], f[3]), pack2<T>(f[4], f[5]), pack2<T>(f[6], f[7]));
-  } else {
+  __device__ __forceinline__ void zero() {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) p[i] = from_float<T>(f[i]);
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) w[k] = make_uint4(0, 0, 0, 0);
   }
-}
-
-// T: rows and caches, A: rotary tables; WIDE: every row starts at a multiple of 16 bytes
-template <typename T, typename A, bool WIDE>
-__global__ void __launch_bounds__(kRotThreads) rotate_append_kernel(const __grid_constant__ mk_rotate_append_args a) {
-  const int heads = a.q_heads + 2 * a.kv_heads;
-  const long long row = ((long long)blockIdx.x * kRotThreads + threadIdx.x) / kRowLanes;
-  const int l = threadIdx.x % kRowLanes;
-  const bool in = row < (long long)a.tokens * heads;  // the norm's shuffles take whole warps
-  const int t = in ? (int)(row / heads) : 0, h = in ? (int)(row - (long long)t * heads) : 0;
-  const long long slot = in ? a.slots[t] : -1;
-  const int pos = in ? a.positions[t] : 0;
-  const bool live = slot >= 0 && slot < (long long)a.pages * a.page_size && pos >= 0 && pos < a.table_rows;
-  const int kind = h < a.q_heads ? 0 : h < a.q_heads + a.kv_heads ? 1 : 2;  // q, k, v
-  const int head = kind == 0 ? h : kind == 1 ? h - a.q_heads : h - a.q_heads - a.kv_heads;
-  const T* src = kind == 0 ? (const T*)a.q + t * a.q_stride[0] + head * a.q_stride[1]
-               : kind == 1 ? (const T*)a.k + t * a.k_stride[0] + head * a.k_stride[1]
-                           : (const T*)a.v + t * a.v_stride[0] + head * a.v_stride[1];
-  float lo[8], hi[8];
+  __device__ __forceinline__ void get(uint64_t (&f)[4]) const {  // as pairs of fp32
 #pragma unroll
-  for (int i = 0; i < 8; ++i) lo[i] = hi[i] = 0.f;
-  if (live) {
-    load8<T, WIDE>(src + 8 * l, lo);
-    load8<T, WIDE>(src + 64 + 8 * l, hi);
-  }
-  float sq = 0.f;
+    for (int k = 0; k < (int)sizeof(T) / 2; ++k) {
+      const uint32_t v[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sq += lo[i] * lo[i] + hi[i] * hi[i];
-#pragma unroll
-  for (int o = 1; o < kRowLanes; o <<= 1) sq += __shfl_xor_sync(kAll, sq, o);  // (by whole warps: rows of v and rows without a slot too)
-  if (!live) return;
-  if (kind < 2) {
-    const T* norm = (const T*)(kind == 0 ? a.q_norm : a.k_norm);
-    float c[8], s[8];
-    if (norm) {
-      const float scale = rsqrtf(sq * (1.f / kHeadDim) + a.eps);
-      load8<T, WIDE>(norm + 8 * l, c);
-      load8<T, WIDE>(norm + 64 + 8 * l, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        lo[i] *= scale * c[i];
-        hi[i] *= scale * s[i];
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 2) {
+          const float2 d = unpack2<T>(v[i]);
+          f[i] = pair(d.x, d.y);
+        } else if (i < 2) {
+          f[2 * k + i] = pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        }
       }
     }
-    const A* cs = (const A*)a.cos + pos * a.table_stride[0];
-    const A* sn = (const A*)a.sin + pos * a.table_stride[1];
-    float x[8];
-    load8<A, WIDE>(cs + 8 * l, c);
-    load8<A, WIDE>(sn + 8 * l, s);
+  }
+  template <bool WIDE> __device__ __forceinline__ void store(T* p) const {
+    if constexpr (WIDE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = lo[i] * c[i] - hi[i] * s[i];
-    load8<A, WIDE>(cs + 64 + 8 * l, c);
-    load8<A, WIDE>(sn + 64 + 8 * l, s);
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k) reinterpret_cast<uint4*>(p)[k] = w[k];
+    } else {
+      const T* e = reinterpret_cast<const T*>(w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      hi[i] = hi[i] * c[i] + lo[i] * s[i];
-      lo[i] = x[i];
+      for (int i = 0; i < 8; ++i) p[i] = e[i];
     }
   }
-  const long long pg = slot / a.page_size, in_page = slot - pg * a.page_size;
-  T* dst = kind == 0 ? (T*)a.out + t * a.out_stride[0] + head * a.out_stride[1]
-         : kind == 1 ? (T*)a.k_cache + pg * a.k_cache_stride[0] + in_page * a.k_cache_stride[1] + head * a.k_cache_stride[2]
-                     : (T*)a.v_cache + pg * a.v_cache_stride[0] + in_page * a.v_cache_stride[1] + head * a.v_cache_stride[2];
-  store8<T, WIDE>(dst + 8 * l, lo);
-  store8<T, WIDE>(dst + 64 + 8 * l, hi);
+  __device__ __forceinline__ void put(const uint64_t (&f)[4]) {  // (16-bit types)
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 d = unpair(f[i]);
+      v[i] = pack2<T>(d.x, d.y);
+    }
+    w[0] = make_uint4(v[0], v[1], v[2], v[3]);
+  }
+};
+
+// T: rows and caches, A: rotary tables; WIDE: every row starts at a multiple of 16 bytes; ROWS heads of a token, next to each other, to eight
+// lanes: the token's slot, position and rotary row are looked up once for them, and their loads are on their way together.
+template <typename T, typename A, bool WIDE, int ROWS>
+__global__ void __launch_bounds__(kRotThreads, 4) rotate_append_kernel(const __grid_constant__ mk_rotate_append_args a) {
+  const int heads = a.q_heads + 2 * a.kv_heads, l = threadIdx.x % kRowLanes, groups = (heads + ROWS - 1) / ROWS;
+  const unsigned group = (blockIdx.x * kRotThreads + threadIdx.x) / kRowLanes;  // (fewer than 2^31: the launch sees to it)
+  const int t = (int)(group / (unsigned)groups), h0 = (int)(group - (unsigned)t * (unsigned)groups) * ROWS;
+  if (t >= a.tokens) return;  // (eight lanes together, and so below: the norm's shuffles are theirs alone)
+  const unsigned lanes = 0xffu << (threadIdx.x & 24);
+  const long long slot = __ldg(a.slots + t);
+  const int pos = __ldg(a.positions + t);
+  if (slot < 0 || slot >= (long long)a.pages * a.page_size || pos < 0 || pos >= a.table_rows) return;
+  auto kind_of = [&](int h) { return h < a.q_heads ? 0 : h < a.q_heads + a.kv_heads ? 1 : 2; };  // q, k, v
+  auto head_of = [&](int h, int kind) { return kind == 0 ? h : kind == 1 ? h - a.q_heads : h - a.q_heads - a.kv_heads; };
+  Raw<T> lo[ROWS], hi[ROWS];
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const int h = h0 + j, kind = kind_of(h), head = head_of(h, kind);
+    if (h >= heads) break;
+    const T* src = 8 * l + (kind == 0 ? (const T*)a.q + t * a.q_stride[0] + head * a.q_stride[1]
+                          : kind == 1 ? (const T*)a.k + t * a.k_stride[0] + head * a.k_stride[1]
+                                      : (const T*)a.v + t * a.v_stride[0] + head * a.v_stride[1]);
+    lo[j].template load<WIDE>(src);
+    hi[j].template load<WIDE>(src + 64);
+  }
+  long long pg, in_page;
+  if ((unsigned long long)slot >> 31) {
+    pg = slot / a.page_size;
+    in_page = slot - pg * a.page_size;
+  } else {
+    pg = (unsigned)slot / (unsigned)a.page_size;
+    in_page = (unsigned)slot - (unsigned)pg * (unsigned)a.page_size;
+  }
+  // the lane's 8 + 8 elements of the rotary row (rows of v need none)
+  uint64_t c0[4], c1[4], s0[4], s1[4];
+  if (kind_of(h0) < 2) {
+    const A* cs = (const A*)a.cos + pos * a.table_stride[0] + 8 * l;
+    const A* sn = (const A*)a.sin + pos * a.table_stride[1] + 8 * l;
+    Raw<A> x0, x1, x2, x3;
+    x0.template load<WIDE>(cs);
+    x1.template load<WIDE>(cs + 64);
+    x2.template load<WIDE>(sn);
+    x3.template load<WIDE>(sn + 64);
+    x0.get(c0);
+    x1.get(c1);
+    x2.get(s0);
+    x3.get(s1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s0[i] ^= 0x8000000080000000ull;  // (its products are taken away)
+  }
+  uint64_t w0[4], w1[4];
+  int normed = -1;  // kind whose weights are in w0, w1
+#pragma unroll
+  for (int j = 0; j < ROWS; ++j) {
+    const int h = h0 + j, kind = kind_of(h), head = head_of(h, kind);
+    if (h >= heads) break;
+    if (kind < 2) {
+      uint64_t x[4], y[4];
+      lo[j].get(x);
+      hi[j].get(y);
+      if (const T* norm = (const T*)(kind == 0 ? a.q_norm : a.k_norm)) {
+        if (normed != kind) {
+          Raw<T> r0, r1;
+          r0.template load<WIDE>(norm + 8 * l);
+          r1.template load<WIDE>(norm + 64 + 8 * l);
+          r0.get(w0);
+          r1.get(w1);
+          normed = kind;
+        }
+        uint64_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum = fma2(y[i], y[i], fma2(x[i], x[i], sum));
+        const float2 both = unpair(sum);
+        float sq = both.x + both.y;
+#pragma unroll
+        for (int o = 1; o < kRowLanes; o <<= 1) sq += __shfl_xor_sync(lanes, sq, o);
+        const float f = rsqrtf(sq * (1.f / kHeadDim) + a.eps);
+        const uint64_t scale = pair(f, f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = mul2(mul2(x[i], scale), w0[i]);
+          y[i] = mul2(mul2(y[i], scale), w1[i]);
+        }
+      }
+      uint64_t z[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        z[i] = fma2(y[i], s0[i], mul2(x[i], c0[i]));
+        y[i] = fma2(x[i], s1[i], mul2(y[i], c1[i]));
+      }
+      lo[j].put(z);
+      hi[j].put(y);
+    }
+    T* dst = 8 * l + (kind == 0 ? (T*)a.out + t * a.out_stride[0] + head * a.out_stride[1]
+                    : kind == 1 ? (T*)a.k_cache + pg * a.k_cache_stride[0] + in_page * a.k_cache_stride[1] + head * a.k_cache_stride[2]
+                                : (T*)a.v_cache + pg * a.v_cache_stride[0] + in_page * a.v_cache_stride[1] + head * a.v_cache_stride[2]);
+    lo[j].template store<WIDE>(dst);
+    hi[j].template store<WIDE>(dst + 64);
+  }
 }
 
 template <typename T, typename A> int launch(const mk_rotate_append_args& a, bool wide, cudaStream_t s) {
-  const long long rows = (long long)a.tokens * (a.q_heads + 2 * a.kv_heads), per = kRotThreads / kRowLanes;
-  const unsigned grid = (unsigned)((rows + per - 1) / per);
-  if (wide) rotate_append_kernel<T, A, true><<<grid, kRotThreads, 0, s>>>(a);
-  else rotate_append_kernel<T, A, false><<<grid, kRotThreads, 0, s>>>(a);
+  const int heads = a.q_heads + 2 * a.kv_heads;
+  const long long per = kRotThreads / kRowLanes;
+  // one row to eight lanes as long as that leaves SMs with little work
+  const bool many = (long long)a.tokens * heads > 4 * per * sm_count();
+  const long long grid = ((long long)a.tokens * (many ? (heads + kRows - 1) / kRows : heads) + per - 1) / per;
+  if (!wide) rotate_append_kernel<T, A, false, 1><<<(unsigned)(((long long)a.tokens * heads + per - 1) / per), kRotThreads, 0, s>>>(a);
+  else if (many) rotate_append_kernel<T, A, true, kRows><<<(unsigned)grid, kRotThreads, 0, s>>>(a);
+  else rotate_append_kernel<T, A, true, 1><<<(unsigned)grid, kRotThreads, 0, s>>>(a);
   return launched("rotate_append");
 }
 
@@ -128,7 +194,7 @@ extern "C" int mk_rotate_append(const mk_rotate_append_args* args, void* stream)
   if (a.table_dtype != a.dtype && a.table_dtype != MK_F32) return fail(MK_E_INVALID, "rotate_append: cos and sin have the rows' type or fp32");
   if (a.tokens < 0 || a.q_heads < 1 || a.kv_heads < 1 || a.page_size < 1 || a.pages < 1 || a.table_rows < 1)
     return fail(MK_E_INVALID, "rotate_append: sizes must be positive");
-  if ((long long)a.tokens * (a.q_heads + 2 * a.kv_heads) > (1ll << 36)) return fail(MK_E_TOO_LARGE, "rotate_append: too many rows");
+  if ((long long)a.tokens * ((long long)a.q_heads + 2ll * a.kv_heads) > 0x7fffffff / kRowLanes) return fail(MK_E_TOO_LARGE, "rotate_append: too many rows");
   if (a.tokens == 0) return 0;
   bool wide = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.cos) && aligned16(a.sin) && aligned16(a.k_cache) &&
               aligned16(a.v_cache) && aligned16(a.out) && aligned16(a.q_norm) && aligned16(a.k_norm);

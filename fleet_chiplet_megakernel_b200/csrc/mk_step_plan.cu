@@ -15,92 +15,106 @@ constexpr int kPlanWarps = kPlanThreads / 32;
 
 struct PlanParams {
   mk_step_plan_args a;
+  int shift;  // log2 of the page size, -1 if it is no power of two
 };
 
-// Inclusive sum over the block, and the block's total; `carry` holds kPlanWarps + 1 values and is free again on return.
-__device__ __forceinline__ long long block_scan(long long v, long long* carry, long long* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Inclusive sums of N values over the block, and the block's totals.  One barrier: `turn` alternates between two places for the warps'
+// totals, and whoever writes a place again has passed the barrier of the other one since it was read.
+template <int N> struct Scan {
+  long long (*carry)[N][kPlanWarps];  // [2]
+  int turn = 0;
+  __device__ __forceinline__ void operator()(long long (&v)[N], long long (&total)[N], int used) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long u = __shfl_up_sync(kAll, v, o);
-    if (lane >= o) v += u;
-  }
-  if (lane == 31) carry[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    long long c = lane < kPlanWarps ? carry[lane] : 0;
+    for (int k = 0; k < used; ++k)
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long u = __shfl_up_sync(kAll, c, o);
-      if (lane >= o) c += u;
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(kAll, v[k], o);
+        if (lane >= o) v[k] += u;
+      }
+    if (lane == 31)
+#pragma unroll
+      for (int k = 0; k < used; ++k) carry[turn][k][warp] = v[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < used; ++k) {
+      long long c = lane < kPlanWarps ? carry[turn][k][lane] : 0;
+#pragma unroll
+      for (int o = 1; o < kPlanWarps; o <<= 1) {
+        const long long u = __shfl_up_sync(kAll, c, o);
+        if (lane >= o) c += u;
+      }
+      total[k] = __shfl_sync(kAll, c, kPlanWarps - 1);
+      const long long before = __shfl_sync(kAll, c, warp > 0 ? warp - 1 : 0);
+      if (warp > 0) v[k] += before;
     }
-    if (lane < kPlanWarps) carry[lane] = c;
+    turn ^= 1;
   }
-  __syncthreads();
-  const long long before = warp ? carry[warp - 1] : 0;
-  *total = carry[kPlanWarps - 1];
-  __syncthreads();
-  return before + v;
-}
+};
 
 __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_constant__ PlanParams p) {
   const mk_step_plan_args& a = p.a;
   extern __shared__ int table[];  // three tables of R + 1 first entries: token rows, pages of the index, pages given back
-  __shared__ long long carry[kPlanWarps];
+  __shared__ long long carry[2][3][kPlanWarps];
+  Scan<3> scan{carry};
   const int R = a.requests, page = a.page_size;
   int* tok0 = table;
   int* kv0 = tok0 + R + 1;
   int* need0 = kv0 + R + 1;
   int* back0 = need0 + R + 1;
   const long long head = a.free_range_in[0], tail = a.free_range_in[1];
-  const long long longest = min((long long)a.table_width * page, 0x7fffffffll);  // what a row of the block table can hold
-  auto length_of = [&](int r) { return (int)min((long long)max(0, a.lengths[r]), longest); };
-  auto pages_of = [&](long long n) { return (n + page - 1) / page; };
+  const unsigned longest = (unsigned)min((long long)a.table_width * page, 0x7fffffffll);  // what a row of the block table can hold
+  auto length_of = [&](int r) { return (int)min((unsigned)max(0, __ldg(a.lengths + r)), longest); };
+  auto divided = [&](unsigned n) { return p.shift >= 0 ? n >> p.shift : n / (unsigned)page; };
+  auto pages_of = [&](unsigned n) { return n ? (int)(divided(n - 1) + 1) : 0; };
 
   // pages that ended requests give back: they count as free in this step already
-  long long back = 0, total;
+  long long back = 0, total[3];
   for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
     const int r = r0 + threadIdx.x;
-    const long long mine = r < R && a.new_tokens[r] < 0 ? pages_of(length_of(r)) : 0;
-    const long long upto = back + block_scan(mine, carry, &total);
-    if (r < R) back0[r + 1] = (int)upto;
-    back += total;
+    long long v[3] = {r < R && __ldg(a.new_tokens + r) < 0 ? pages_of(length_of(r)) : 0, 0, 0};
+    scan(v, total, 1);
+    if (r < R) back0[r + 1] = (int)(back + v[0]);
+    back += total[0];
   }
   const long long free_pages = tail - head + back;
 
   long long wanted = 0, rows = 0, kv = 0, taken = 0, tokens = 0;
   for (int r0 = 0; r0 < R; r0 += kPlanThreads) {
     const int r = r0 + threadIdx.x;
-    const int len = r < R ? length_of(r) : 0, want = r < R ? a.new_tokens[r] : 0;
-    const long long held = pages_of(len), after = pages_of((long long)len + max(0, want));
+    const int len = r < R ? length_of(r) : 0, want = r < R ? __ldg(a.new_tokens + r) : 0;
+    const int held = pages_of(len), after = pages_of((unsigned)len + (unsigned)max(0, want));
     const bool valid = want > 0 && after <= a.table_width;
-    const long long need = valid ? after - held : 0;
-    const long long upto = wanted + block_scan(need, carry, &total);
-    wanted += total;
-    const bool fits = valid && (need == 0 || upto <= free_pages);
-    const long long row_end = rows + block_scan(fits ? want : 0, carry, &total);
-    rows += total;
-    const int granted = fits && row_end <= a.max_tokens ? want : 0;
-    const long long take = granted > 0 ? need : 0;
+    const int need = valid ? after - held : 0;
+    long long v[3] = {need, 0, 0};
+    scan(v, total, 1);
+    const bool fits = valid && (need == 0 || wanted + v[0] <= free_pages);
+    wanted += total[0];
+    v[0] = fits ? want : 0;
+    scan(v, total, 1);
+    const int granted = fits && rows + v[0] <= a.max_tokens ? want : 0;
+    rows += total[0];
+    const int take = granted > 0 ? need : 0;
     // (want < 0: ended.  A request that gets nothing keeps the pages that it has.)
-    const long long pages = want < 0 ? 0 : held + take;
-    const long long tok_end = tokens + block_scan(granted, carry, &total);
-    tokens += total;
-    const long long need_end = taken + block_scan(take, carry, &total);
-    taken += total;
-    const long long kv_end = kv + block_scan(pages, carry, &total);
-    kv += total;
+    const int pages = want < 0 ? 0 : held + take;
+    v[0] = granted;
+    v[1] = take;
+    v[2] = pages;
+    scan(v, total, 3);
     if (r < R) {
-      tok0[r + 1] = (int)tok_end;
-      need0[r + 1] = (int)need_end;
-      kv0[r + 1] = (int)kv_end;
+      tok0[r + 1] = (int)(tokens + v[0]);
+      need0[r + 1] = (int)(taken + v[1]);
+      kv0[r + 1] = (int)(kv + v[2]);
       if (blockIdx.x == 0) {
         a.granted[r] = granted;
-        a.qo_indptr[r + 1] = (int)tok_end;
-        a.kv_indptr[r + 1] = (int)kv_end;
-        a.last_page_len[r] = pages > 0 ? (int)(len + granted - (pages - 1) * page) : 0;
+        a.qo_indptr[r + 1] = (int)(tokens + v[0]);
+        a.kv_indptr[r + 1] = (int)(kv + v[2]);
+        a.last_page_len[r] = pages > 0 ? (int)((long long)len + granted - (long long)(pages - 1) * page) : 0;
       }
     }
+    tokens += total[0];
+    taken += total[1];
+    kv += total[2];
   }
   if (threadIdx.x == 0) {
     tok0[0] = kv0[0] = need0[0] = back0[0] = 0;
@@ -126,7 +140,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     return a.block_table[(long long)r * a.table_stride + (b - back0[r])];
   };
   auto page_at = [&](int r, int k) -> int {  // page k of request r, held or taken
-    const int held = (int)pages_of(length_of(r));
+    const int held = pages_of(length_of(r));
     return k < held ? a.block_table[(long long)r * a.table_stride + k] : taken_page((long long)need0[r] + k - held);
   };
 
@@ -136,7 +150,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
   for (long long e = (long long)blockIdx.x * kPlanThreads + threadIdx.x; e < all; e += (long long)gridDim.x * kPlanThreads) {
     if (e < n_kv) {  // an entry of the page index; a new page enters its request's table as well
       const int r = find_owner(R, e, [&](int k) { return (long long)kv0[k]; });
-      const int k = (int)e - kv0[r], held = (int)pages_of(length_of(r));
+      const int k = (int)e - kv0[r], held = pages_of(length_of(r));
       const int pg = page_at(r, k);
       a.kv_indices[e] = pg;
       if (k >= held) a.block_table[(long long)r * a.table_stride + k] = pg;
@@ -147,7 +161,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       if (t < tokens) {
         const int r = find_owner(R, t, [&](int k) { return (long long)tok0[k]; });
         pos = length_of(r) + t - tok0[r];
-        const int k = pos / page;
+        const int k = (int)divided((unsigned)pos);
         slot = (long long)page_at(r, k) * page + (pos - k * page);
       }
       a.slots[t] = slot;
@@ -201,7 +215,9 @@ extern "C" int mk_plan_step(const mk_step_plan_args* args, void* stream) {
   }
   const long long entries = (long long)a.max_indices + a.max_tokens;
   const int ctas = (int)((entries + kPlanThreads - 1) / kPlanThreads);
-  PlanParams p{a};
+  PlanParams p{a, -1};
+  for (int k = 0; k < 31; ++k)
+    if (a.page_size == 1 << k) p.shift = k;
   step_plan_kernel<<<ctas < sm_count() ? ctas : sm_count(), kPlanThreads, smem, (cudaStream_t)stream>>>(p);
   return launched("plan_step");
 }
