@@ -15,6 +15,7 @@ import torch
 
 from .persistent_kernel import PersistentKernel, get_configurations_from_gpu
 from .qwen3_graph import Qwen3Geometry, build_qwen3_graph
+from .serving import StepPlan, plan_step, sample_tokens
 
 
 @dataclass
@@ -76,6 +77,7 @@ class MPKMetadata:
     spec_decode_config: Optional[object] = None
     use_cutlass_kernel: bool = True
     eos_token_id: int = -1
+    logits: Optional[torch.Tensor] = None  # [max_num_batched_tokens, vocab] bf16: filled by every pass (extension; sample_tokens reads it)
     extra: dict = field(default_factory=dict)  # further PersistentKernel arguments (numerics, max_iterations, ...)
 
     def check_valid(self):
@@ -153,6 +155,7 @@ class MPK:
             use_cutlass_kernel=meta.use_cutlass_kernel, eos_token_id=meta.eos_token_id, **meta.extra)
         self.is_built = self.is_compiled = False
         self.returned_hidden_state = None
+        self.step_plan = None
 
     def compensate_meta_tensors(self):
         """mpk.py:237-268: allocate the meta tensors the caller left out."""
@@ -182,7 +185,7 @@ class MPK:
         w = weights_from_state_dict(mc.state_dict, mc.num_layers)
         cos, sin = mc.position_embeddings
         out = build_qwen3_graph(self.persistent_kernel, geom, w, mc.k_cache, mc.v_cache, cos, sin, self.input_tokens,
-                                self.output_tokens, lm_head=self.with_lm_head)
+                                self.output_tokens, logits=self.metadata.logits, lm_head=self.with_lm_head)
         if not self.with_lm_head:
             self.returned_hidden_state = out  # online_notoken without a head: the last hidden state (a DTensor)
         self.is_built = True
@@ -229,6 +232,29 @@ class MPK:
         self.persistent_kernel(**kwargs)
         if not self.with_lm_head and self.persistent_kernel.mode == "online_notoken":
             return self.persistent_kernel.read_tensor(self.returned_hidden_state)
+
+    # -- a serving engine's step (extension; modes that take the caller's metadata) --------
+    def plan_step(self, lengths, new_tokens, block_table, free_pages, free_range) -> StepPlan:
+        """Plan the next pass on the GPU (``serving.plan_step``): pages for the new tokens, and this wrapper's ``qo_indptr_buffer`` and
+        ``paged_kv_*`` buffers as the pass reads them.  The caller puts the granted tokens into ``input_tokens`` (row order of
+        ``qo_indptr_buffer``) and calls the wrapper."""
+        if self.metadata.mode == "offline":
+            raise ValueError("mode 'offline' plans its iterations itself; use 'online_notoken'")
+        if self.step_plan is None:
+            plan = StepPlan.empty(self.max_num_batched_requests, self.max_num_batched_tokens, 1, self.device)
+            plan.qo_indptr, plan.kv_indptr = self.qo_indptr_buffer, self.paged_kv_indptr_buffer
+            plan.kv_indices, plan.last_page_len = self.paged_kv_indices_buffer, self.paged_kv_last_page_len_buffer
+            self.step_plan = plan
+        return plan_step(lengths, new_tokens, block_table, free_pages, free_range, self.metadata.page_size, self.step_plan)
+
+    def sample_tokens(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logprobs: bool = False):
+        """A token per request from the logits of its last row in the pass before (``serving.sample_tokens``); -1 for requests that
+        were fed nothing.  Needs ``MPKMetadata.logits``."""
+        if self.metadata.logits is None:
+            raise ValueError("sample_tokens needs MPKMetadata.logits")
+        if self.metadata.mode == "offline":
+            raise ValueError("mode 'offline' takes the largest logit itself; use 'online_notoken'")
+        return sample_tokens(self.metadata.logits, u, temperature, top_k, top_p, min_p, qo_indptr=self.qo_indptr_buffer, return_logprobs=return_logprobs)
 
     def finalize(self):
         if not getattr(self.persistent_kernel, "__finalized__", True):

@@ -124,7 +124,7 @@ def sample_tokens(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, qo_
     Row r belongs to request r; with ``qo_indptr`` [requests + 1] int32 (``StepPlan``) its last one does, and a request without rows gets -1.
     ``temperature``, ``top_p``, ``min_p`` (fp32) and ``top_k`` (int32) are numbers or a tensor [requests] each.  temperature 0: the largest logit,
     the lowest index on ties.  Otherwise weights exp((l - max) / temperature); top_k (0: off) keeps the k largest, top_p (1: off) of
-    these the ones before which less than top_p of their weight lies, min_p (0: off) those of at least min_p times the largest;
+    these the ones before which less than top_p of their weight lies, min_p (0: off; above 1 it counts as 1) those of at least min_p times the largest;
     equal logits count in the order of the index.  The token is the first by index at which the running sum of the kept weights exceeds
     u times their sum.  NaN logits count as minus infinity; a row of nothing else gives -1.  Returns tokens int64 [requests] (``out``), and
     with ``return_logprobs`` the logarithms of the probabilities with which they were drawn as well."""

@@ -276,7 +276,7 @@ int mk_chunk_attention(const mk_chunk_attention_args* args, void* stream);
 
 /* A token per request from logits [rows, vocab] (row r, or with qo_indptr the request's last row; -1 where it has none or where no
  * token can be chosen) and u[r] in [0, 1).  temperature 0: the largest logit, the lowest index on ties.  Otherwise top_k (0: off),
- * then top_p (1: off) of what top_k leaves, and min_p (0: off) relative to the largest weight; the token is the first by
+ * then top_p (1: off) of what top_k leaves, and min_p (0: off, at most 1) relative to the largest weight; the token is the first by
  * index at which the running sum of kept weights exceeds u times their sum.  Settings are per request, or the values where the
  * pointer is NULL.  logprobs (may be NULL): logarithm of the probability with which the token was drawn. */
 typedef struct mk_sample_args {

@@ -435,7 +435,7 @@ def sample_reference(logits, u, t, k, p, m):
     if p < 1:
         before = torch.cat((w.new_zeros(1), torch.cumsum(w, 0)[:-1]))
         n = max(1, int((before < float(torch.tensor(p)) * w.sum()).sum()))
-    n = min(n, int((w >= float(torch.tensor(m))).sum()))
+    n = min(n, int((w >= min(float(torch.tensor(m)), 1.0)).sum()))
     by, turn = by[:n].sort()
     w = w[:n][turn]
     c = torch.cumsum(w, 0)
