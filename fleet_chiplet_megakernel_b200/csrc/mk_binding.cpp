@@ -30,17 +30,42 @@ struct {
   decltype(&mk_op_error) error;
 } g_lib;
 
-void need(bool ok, const char* what, const char* msg) {
-  if (!ok) TORCH_CHECK_VALUE(false, what, msg);
+// Texts are put together by std::to_string alone: formatting numbers through a C++ stream of this module ended the process on a
+// machine with a GPU, where more libraries are loaded than here.
+void put(std::string& s, const char* t) { s += t; }
+void put(std::string& s, const std::string& t) { s += t; }
+void put(std::string& s, int64_t v) { s += std::to_string(v); }
+void put(std::string& s, at::IntArrayRef v) {
+  s += '[';
+  for (size_t i = 0; i < v.size(); ++i) s += (i ? ", " : "") + std::to_string(v[i]);
+  s += ']';
 }
+void put(std::string& s, at::ScalarType t) { s += c10::toString(t); }
+void put(std::string& s, const c10::Device& d) { s += d.str(); }
+template <typename... P> std::string text(const P&... parts) {
+  std::string s;
+  (put(s, parts), ...);
+  return s;
+}
+template <typename... P> [[noreturn, gnu::noinline]] void refuse(const P&... parts) { C10_THROW_ERROR(ValueError, text(parts...)); }
+template <typename... P> [[noreturn, gnu::noinline]] void too_large(const P&... parts) { C10_THROW_ERROR(NotImplementedError, text(parts...)); }
+#define REFUSE_IF(bad, ...) \
+  do {                      \
+    if (bad) refuse(__VA_ARGS__); \
+  } while (0)
+#define TOO_LARGE_IF(bad, ...) \
+  do {                         \
+    if (bad) too_large(__VA_ARGS__); \
+  } while (0)
+void need(bool ok, const char* what, const char* msg) { REFUSE_IF(!ok, what, msg); }
 // A status of the library as the exceptions of PersistentKernel.
 void status(int64_t rc) {
   if (rc >= 0) return;
-  char text[512] = "";
-  g_lib.error(text, sizeof text);
-  if (rc == MK_E_UNSUPPORTED || rc == MK_E_TOO_LARGE) TORCH_CHECK_NOT_IMPLEMENTED(false, text);
-  if (rc == MK_E_INVALID) TORCH_CHECK_VALUE(false, text);
-  TORCH_CHECK(false, text);
+  char said[512] = "";
+  g_lib.error(said, sizeof said);
+  TOO_LARGE_IF(rc == MK_E_UNSUPPORTED || rc == MK_E_TOO_LARGE, said);
+  REFUSE_IF(rc == MK_E_INVALID, said);
+  C10_THROW_ERROR(Error, std::string(said));
 }
 
 const at::Tensor& tensor(PyObject* o, const char* what) {
@@ -51,7 +76,7 @@ const at::Tensor* maybe(PyObject* o, const char* what) { return o == Py_None ? n
 int64_t number(PyObject* o, const char* what, int64_t lo, int64_t hi) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw python_error();
-  if (v < lo || v > hi) TORCH_CHECK_VALUE(false, what, ": ", v, ", ", lo, " to ", hi, " is allowed");
+  REFUSE_IF(v < lo || v > hi, what, ": ", v, ", ", lo, " to ", hi, " is allowed");
   return v;
 }
 double real(PyObject* o) {
@@ -70,39 +95,38 @@ struct Checks {
     need(!t.requires_grad() || !c10::GradMode::is_enabled(), what, " requires a gradient and the serving operators have none: call them under torch.no_grad()");
   }
   void here(const at::Tensor& t, const char* what) const {
-    if (t.device() != device) TORCH_CHECK_VALUE(false, what, " is on ", t.device(), ", the first tensor on ", device);
+    REFUSE_IF(t.device() != device, what, " is on ", t.device(), ", the first tensor on ", device);
     need(t.layout() == at::kStrided, what, ": a strided tensor is needed");
     no_gradient(t, what);
   }
   void type(const at::Tensor& t, const char* what, at::ScalarType dt) const {
     here(t, what);
-    if (t.scalar_type() != dt) TORCH_CHECK_VALUE(false, what, ".dtype: ", t.scalar_type(), ", ", dt, " is needed");
+    REFUSE_IF(t.scalar_type() != dt, what, ".dtype: ", t.scalar_type(), ", ", dt, " is needed");
   }
   // one dimension of n entries (n < 0: of any number), contiguous
   template <typename P = void> P* list(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t n) const {
     type(t, what, dt);
-    if (t.dim() != 1 || (n >= 0 && t.size(0) != n)) TORCH_CHECK_VALUE(false, what, ".shape: ", t.sizes(), ", one dimension", n >= 0 ? " of " + std::to_string(n) : std::string(), " is needed");
+    REFUSE_IF(t.dim() != 1 || (n >= 0 && t.size(0) != n), what, ".shape: ", t.sizes(), ", one dimension", n >= 0 ? " of " + std::to_string(n) : std::string(), " is needed");
     need(t.is_contiguous(), what, " must be contiguous");
-    if (t.size(0) > kMaxInt) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": over 2^31 entries");
+    TOO_LARGE_IF(t.size(0) > kMaxInt, what, ": over 2^31 entries");
     return static_cast<P*>(t.data_ptr());
   }
   // [tokens, heads, 128], any token and head stride
   void* rows(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t tokens, int64_t heads, int64_t* stride) const {
     type(t, what, dt);
-    if (t.dim() != 3 || t.size(2) != kHeadDim || (tokens >= 0 && t.size(0) != tokens) || (heads >= 0 && t.size(1) != heads))
-      TORCH_CHECK_VALUE(false, what, ".shape: ", t.sizes(), ", [", tokens >= 0 ? std::to_string(tokens) : "tokens", ", ", heads >= 0 ? std::to_string(heads) : "heads", ", 128] is needed");
+    REFUSE_IF(t.dim() != 3 || t.size(2) != kHeadDim || (tokens >= 0 && t.size(0) != tokens) || (heads >= 0 && t.size(1) != heads), what, ".shape: ", t.sizes(), ", [", tokens >= 0 ? std::to_string(tokens) : "tokens", ", ", heads >= 0 ? std::to_string(heads) : "heads", ", 128] is needed");
     need(t.stride(2) == 1, what, ": the elements of a row must be contiguous");
-    if (t.size(0) > kMaxInt || t.size(1) > kMaxInt) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": over 2^31 rows");
+    TOO_LARGE_IF(t.size(0) > kMaxInt || t.size(1) > kMaxInt, what, ": over 2^31 rows");
     stride[0] = t.stride(0);
     stride[1] = t.stride(1);
     return t.data_ptr();
   }
   void* cache(const at::Tensor& t, const char* what, at::ScalarType dt, int64_t* stride) const {
     type(t, what, dt);
-    if (t.dim() != 4 || t.size(3) != kHeadDim || t.numel() == 0) TORCH_CHECK_VALUE(false, what, ".shape: ", t.sizes(), ", [pages, page_size, kv_heads, 128] is needed");
+    REFUSE_IF(t.dim() != 4 || t.size(3) != kHeadDim || t.numel() == 0, what, ".shape: ", t.sizes(), ", [pages, page_size, kv_heads, 128] is needed");
     need(t.stride(3) == 1, what, ": the elements of a row must be contiguous");
     for (int i = 0; i < 3; ++i) {
-      if (t.size(i) > kMaxInt) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": over 2^31 pages or rows");
+      TOO_LARGE_IF(t.size(i) > kMaxInt, what, ": over 2^31 pages or rows");
       stride[i] = t.stride(i);
     }
     return t.data_ptr();
@@ -124,7 +148,7 @@ struct Checks {
   }
 };
 at::ScalarType row_type(const at::Tensor& t, const char* what) {
-  if (t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf) TORCH_CHECK_VALUE(false, what, ".dtype: ", t.scalar_type(), ", bf16 or fp16 is needed");
+  REFUSE_IF(t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kHalf, what, ".dtype: ", t.scalar_type(), ", bf16 or fp16 is needed");
   return t.scalar_type();
 }
 int code(at::ScalarType t) { return t == at::kBFloat16 ? MK_BF16 : t == at::kHalf ? MK_F16 : MK_F32; }
@@ -157,7 +181,7 @@ PyObject* plan_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
   a.new_tokens = c.list<int32_t>(tensor(v[1], "new_tokens"), "new_tokens", at::kInt, R);
   const at::Tensor& table = tensor(v[2], "block_table");
   c.type(table, "block_table", at::kInt);
-  if (table.dim() != 2 || table.size(0) != R || table.size(1) < 1 || table.size(1) > kMaxInt) TORCH_CHECK_VALUE(false, "block_table.shape: ", table.sizes(), ", [", R, ", pages of the longest request] is needed");
+  REFUSE_IF(table.dim() != 2 || table.size(0) != R || table.size(1) < 1 || table.size(1) > kMaxInt, "block_table.shape: ", table.sizes(), ", [", R, ", pages of the longest request] is needed");
   need(table.stride(1) == 1 && (R == 1 || table.stride(0) >= table.size(1)), "block_table", ": rows must be contiguous and apart");
   a.block_table = static_cast<int32_t*>(table.data_ptr());
   a.table_width = (int32_t)table.size(1);
@@ -204,10 +228,8 @@ PyObject* rotate_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
   for (const at::Tensor* t : {&cos, &sin}) {
     const char* what = t == &cos ? "cos" : "sin";
     c.here(*t, what);
-    if (t->dim() != 2 || t->size(1) != kHeadDim || t->size(0) < 1 || t->size(0) > kMaxInt || t->stride(1) != 1 || t->sizes() != cos.sizes())
-      TORCH_CHECK_VALUE(false, what, ".shape: ", t->sizes(), ", [positions, 128] with contiguous rows, cos and sin alike, is needed");
-    if ((t->scalar_type() != dt && t->scalar_type() != at::kFloat) || t->scalar_type() != cos.scalar_type())
-      TORCH_CHECK_VALUE(false, what, ".dtype: ", t->scalar_type(), ", ", dt, " or fp32, cos and sin alike, is needed");
+    REFUSE_IF(t->dim() != 2 || t->size(1) != kHeadDim || t->size(0) < 1 || t->size(0) > kMaxInt || t->stride(1) != 1 || t->sizes() != cos.sizes(), what, ".shape: ", t->sizes(), ", [positions, 128] with contiguous rows, cos and sin alike, is needed");
+    REFUSE_IF((t->scalar_type() != dt && t->scalar_type() != at::kFloat) || t->scalar_type() != cos.scalar_type(), what, ".dtype: ", t->scalar_type(), ", ", dt, " or fp32, cos and sin alike, is needed");
   }
   a.cos = cos.data_ptr();
   a.sin = sin.data_ptr();
@@ -218,7 +240,7 @@ PyObject* rotate_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
   const at::Tensor &kc = tensor(v[7], "k_cache"), &vc = tensor(v[8], "v_cache");
   a.k_cache = c.cache(kc, "k_cache", dt, a.k_cache_stride);
   a.v_cache = c.cache(vc, "v_cache", dt, a.v_cache_stride);
-  if (kc.size(2) != n_kv || vc.sizes() != kc.sizes()) TORCH_CHECK_VALUE(false, "caches of shape ", kc.sizes(), " and ", vc.sizes(), " for ", n_kv, " kv heads");
+  REFUSE_IF(kc.size(2) != n_kv || vc.sizes() != kc.sizes(), "caches of shape ", kc.sizes(), " and ", vc.sizes(), " for ", n_kv, " kv heads");
   Checks::apart(kc, "k_cache");
   Checks::apart(vc, "v_cache");
   if (const at::Tensor* t = maybe(v[9], "q_norm")) a.q_norm = c.list(*t, "q_norm", dt, kHeadDim);
@@ -253,9 +275,9 @@ PyObject* chunk_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
   const at::Tensor &kc = tensor(v[1], "k_cache"), &vc = tensor(v[2], "v_cache");
   a.k_cache = c.cache(kc, "k_cache", dt, a.k_cache_stride);
   a.v_cache = c.cache(vc, "v_cache", dt, a.v_cache_stride);
-  if (vc.sizes() != kc.sizes()) TORCH_CHECK_VALUE(false, "k_cache is ", kc.sizes(), ", v_cache ", vc.sizes());
+  REFUSE_IF(vc.sizes() != kc.sizes(), "k_cache is ", kc.sizes(), ", v_cache ", vc.sizes());
   const int64_t n_kv = kc.size(2);
-  if (n_q % n_kv) TORCH_CHECK_VALUE(false, n_q, " q heads on ", n_kv, " kv heads");
+  REFUSE_IF(n_q % n_kv, n_q, " q heads on ", n_kv, " kv heads");
   const at::Tensor& last = tensor(v[6], "last_page_len");
   a.last_page_len = c.list<int32_t>(last, "last_page_len", at::kInt, -1);
   const int64_t R = last.size(0);
@@ -273,7 +295,7 @@ PyObject* chunk_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
   need(a.out != a.q || T * n_q == 0, "out", " may not be q");
   if (const at::Tensor* t = maybe(v[11], "lse")) {
     c.type(*t, "lse", at::kFloat);
-    if (t->dim() != 2 || t->size(0) != T || t->size(1) != n_q) TORCH_CHECK_VALUE(false, "lse.shape: ", t->sizes(), ", [", T, ", ", n_q, "] is needed");
+    REFUSE_IF(t->dim() != 2 || t->size(0) != T || t->size(1) != n_q, "lse.shape: ", t->sizes(), ", [", T, ", ", n_q, "] is needed");
     a.lse = static_cast<float*>(t->data_ptr());
     a.lse_stride[0] = t->stride(0);
     a.lse_stride[1] = t->stride(1);
@@ -306,8 +328,8 @@ PyObject* sample_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
   const at::Tensor& logits = tensor(v[0], "logits");
   const Checks c(logits, "logits");
   const at::ScalarType dt = logits.scalar_type();
-  if (dt != at::kBFloat16 && dt != at::kHalf && dt != at::kFloat) TORCH_CHECK_VALUE(false, "logits.dtype: ", dt, ", bf16, fp16 or fp32 is needed");
-  if (logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > kMaxInt || logits.size(0) > kMaxInt) TORCH_CHECK_VALUE(false, "logits.shape: ", logits.sizes(), ", [rows, vocab] is needed");
+  REFUSE_IF(dt != at::kBFloat16 && dt != at::kHalf && dt != at::kFloat, "logits.dtype: ", dt, ", bf16, fp16 or fp32 is needed");
+  REFUSE_IF(logits.dim() != 2 || logits.size(1) < 1 || logits.size(1) > kMaxInt || logits.size(0) > kMaxInt, "logits.shape: ", logits.sizes(), ", [rows, vocab] is needed");
   need(logits.stride(1) == 1 || logits.size(1) == 1, "logits", ": the elements of a row must be contiguous");
   const at::Tensor& u = tensor(v[1], "u");
   a.u = c.list<float>(u, "u", at::kFloat, -1);
@@ -321,7 +343,7 @@ PyObject* sample_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (THPVariable_Check(v[5])) a.min_p = c.list<float>(tensor(v[5], "min_p"), "min_p", at::kFloat, R);
   else a.min_p_value = (float)real(v[5]);
   if (const at::Tensor* t = maybe(v[6], "qo_indptr")) a.qo_indptr = c.list<int32_t>(*t, "qo_indptr", at::kInt, R + 1);
-  else if (logits.size(0) < R) TORCH_CHECK_VALUE(false, logits.size(0), " rows of logits for ", R, " requests");
+  else REFUSE_IF(logits.size(0) < R, logits.size(0), " rows of logits for ", R, " requests");
   const c10::cuda::CUDAGuard guard(c.device);
   at::Tensor out = v[7] == Py_None ? at::empty({R}, logits.options().dtype(at::kLong).requires_grad(false)) : tensor(v[7], "out");
   a.tokens = c.list<int64_t>(out, "out", at::kLong, R);
