@@ -236,6 +236,19 @@ template <typename T> struct Sampler {
   uint32_t count;         // of this thread's bin, over the cluster
   double low_w, high_w;   // bounds of the mean weight in it
 
+  // exp is convex: the mean weight in a bin is at least the weight at the mean depth and at most the chord's value there.  The depth is
+  // known to 1 / kInner of a bin and to some units of 2^-24 relative.
+  __device__ __forceinline__ void mean_bounds(uint32_t inner, double per_unit) {
+    low_w = high_w = 0.0;
+    const double edge = exp(-(double)threadIdx.x / per_unit);
+    if (threadIdx.x == kBins - 1) {
+      high_w = edge * (1.0 + 1e-4);
+    } else if (count > 0) {
+      const double f = (double)inner / ((double)count * kInner);
+      low_w = edge * exp(-(f + 1.0 / kInner) / per_unit) * (1.0 - 1e-5);
+      high_w = edge * (1.0 - (1.0 - exp(-1.0 / per_unit)) * f) * (1.0 + 1e-5);
+    }
+  }
   // Histogram of the linear bins; with `sum`, *mass: the sum of all weights.
   __device__ void linear_bins(bool sum, double* mass) {
     double w = 0.0;
@@ -255,30 +268,11 @@ template <typename T> struct Sampler {
       count += *peer(&s.hist[threadIdx.x], q);
       inner += *peer(&s.inner[threadIdx.x], q);
     }
-    // exp is convex: the mean weight is at least the weight at the mean depth and at most the chord's value there.  The depth is
-    // known to 1 / kInner of a bin and to some units of 2^-24 relative.
-    low_w = high_w = 0.0;
-    const double edge = exp(-(double)threadIdx.x / kBinsPerUnit);
-    if (threadIdx.x == kBins - 1) {
-      high_w = edge * (1.0 + 1e-4);
-    } else if (count > 0) {
-      const double f = (double)inner / ((double)count * kInner);
-      low_w = edge * exp(-(f + 1.0 / kInner) / kBinsPerUnit) * (1.0 - 1e-5);
-      high_w = edge * (1.0 - (1.0 - exp(-1.0 / kBinsPerUnit)) * f) * (1.0 + 1e-5);
-    }
+    mean_bounds(inner, kBinsPerUnit);
   }
 
-  // List all elements with depth_of(l) < bins (bins <= kBins) at rank 0; returns how many there are, in the whole cluster (kCandidates + 1: more).
-  template <typename F> __device__ int list_above(const F& depth_of, float unit, int bins) {
-    // most are far below: one comparison with a bound that is safely too low
-    float bound = bins < kBins ? r.top - (float)bins / unit * 1.0001f - fabsf(r.top) * 1e-6f : -INFINITY;
-    if (isnan(bound)) bound = -INFINITY;  // (the largest is infinite)
-    r.template each<true>([&](float l, int i) {
-      if (l >= bound && (bins >= kBins || (int)depth_of(l) < bins)) {
-        const uint32_t at = atomicAdd(&s.listed[2], 1u);
-        if (at < kCandidates) s.list[at] = place_of(l, i);
-      }
-    });
+  // The CTAs' lists (s.list, s.listed[2]) end to end at rank 0; returns how long it is (kCandidates + 1: longer than that).
+  __device__ int collected() {
     __syncthreads();
     const uint32_t mine = s.listed[2];
     if ((int)threadIdx.x < ranks) *peer(&s.counts[rank], threadIdx.x) = mine;
@@ -296,6 +290,19 @@ template <typename T> struct Sampler {
     cluster.sync();
     return (int)all;
   }
+  // List all elements with depth_of(l) < bins (bins <= kBins) at rank 0; returns how many there are, in the whole cluster (kCandidates + 1: more).
+  template <typename F> __device__ int list_above(const F& depth_of, float unit, int bins) {
+    // most are far below: one comparison with a bound that is safely too low
+    float bound = bins < kBins ? r.top - (float)bins / unit * 1.0001f - fabsf(r.top) * 1e-6f : -INFINITY;
+    if (isnan(bound)) bound = -INFINITY;  // (the largest is infinite)
+    r.template each<true>([&](float l, int i) {
+      if (l >= bound && (bins >= kBins || (int)depth_of(l) < bins)) {
+        const uint32_t at = atomicAdd(&s.listed[2], 1u);
+        if (at < kCandidates) s.list[at] = place_of(l, i);
+      }
+    });
+    return collected();
+  }
   // Bins 0 .. of which hold at least k of the threads' maxima: what top_k keeps is in them.
   __device__ int bins_of_top(float mine, bool any, int k) {
     auto depth_of = [&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * kTopBins, (float)(kBins - 1)); };
@@ -311,8 +318,8 @@ template <typename T> struct Sampler {
     const int bins = s.last_bin;
     return bins;
   }
-  // Bins 0 .. that hold what top_p keeps, by sums to kSumError; *mass: the sum of all weights, as exactly.
-  __device__ int bins_of_mass(double top_p, float unit, double* mass) {
+  // Bins 0 .. that hold what top_p keeps, by sums to kSumError; *mass: the sum of all weights, as exactly; *elements: in these bins.
+  __device__ int bins_of_mass(double top_p, float unit, double* mass, long long* elements) {
     const float log2_scale = (float)(r.scale / 64.0);
     auto depth_of = [&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * unit, (float)(kBins - 1)); };
     const float top = r.top == INFINITY ? 3.4028235e38f : r.top;  // (differences without NaN)
@@ -329,7 +336,11 @@ template <typename T> struct Sampler {
         w += x;
         if (l[e] >= near) {
           const float d = depth_of(l[e]);
-          if (d < (float)(kBins - 1)) atomicAdd(&s.hist[(int)d], 1u);
+          if (d < (float)(kBins - 1)) {
+            const int b = (int)d;
+            atomicAdd(&s.hist[b], 1u);
+            atomicAdd(&s.inner[b], (uint32_t)((d - (float)b) * (float)kInner));
+          }
         }
       }
       if (++n_w == 8) {  // (no more than 64 terms in fp32)
@@ -341,8 +352,11 @@ template <typename T> struct Sampler {
     give(sum + (double)w);
     cluster.sync();
     *mass = taken();
-    uint32_t n = 0;
-    for (int q = 0; q < ranks; ++q) n += *peer(&s.hist[threadIdx.x], q);
+    uint32_t n = 0, inner = 0;
+    for (int q = 0; q < ranks; ++q) {
+      n += *peer(&s.hist[threadIdx.x], q);
+      inner += *peer(&s.inner[threadIdx.x], q);
+    }
     // at least so much weight is in the bins up to this one
     double total;
     const double low = (double)n * (double)exp2f(-(float)(threadIdx.x + 1) * (1.4427f / kNearBins)) * (1.0 - 1e-4);
@@ -352,7 +366,47 @@ template <typename T> struct Sampler {
     const double limit = top_p * *mass * (1.0 + 4.0 * (double)kSumError);
     if (threadIdx.x < kBins - 1 && before + low >= limit) atomicMin(&s.last_bin, (int)threadIdx.x + 1);
     __syncthreads();
-    return s.last_bin;
+    const int bins = s.last_bin;
+    uint64_t in;
+    block_before((uint64_t)((int)threadIdx.x < bins ? n : 0), s.words, &in);
+    *elements = (long long)in;
+    count = (int)threadIdx.x < bins ? n : 0;
+    mean_bounds(inner, (double)kNearBins);
+    return bins;
+  }
+  // The border of top_p where the kept are too many for a list: from the bins of bins_of_mass those that it can be in, whose elements are
+  // listed, in the pass that sums all weights and those above in 64 bits.  False: too many even so.
+  __device__ bool near_border(double top_p, float unit, double mass, uint64_t* place) {
+    find_bins(true, top_p * mass, 0, 0, 0.0, 4.0 * (double)kSumError);
+    const int first_bin = min(s.first_bin, s.last_bin), last_bin = s.last_bin;
+    const uint64_t in = (int)threadIdx.x < first_bin ? (uint64_t)count : (int)threadIdx.x <= last_bin ? (uint64_t)count << 32 : 0;
+    uint64_t both;
+    block_before(in, s.words, &both);
+    if ((both >> 32) > kCandidates) return false;
+    double sum = 0.0, ahead = 0.0;
+    r.each([&](float l, int i) {
+      const double w = r.weight(l);
+      sum += w;
+      const int b = l == r.top ? 0 : (int)fminf((r.top - l) * unit, (float)(kBins - 1));
+      if (b < first_bin) {
+        ahead += w;
+      } else if (b <= last_bin) {
+        const uint32_t at = atomicAdd(&s.listed[2], 1u);
+        if (at < kCandidates) s.list[at] = place_of(l, i);
+      }
+    });
+    give(sum);
+    const int from_sum = turn++;
+    give(ahead);
+    const int n_list = collected();  // (its barriers stand between giving and taking)
+    ahead = taken();
+    sum = 0.0;
+    for (int k = 0; k < ranks; ++k) sum += s.slot[from_sum & (kSlots - 1)][k];
+    if (n_list > kCandidates) return false;
+    if (rank == 0) cut(n_list, false, 0, true, top_p * sum, (long long)(both & 0xffffffffu), ahead);
+    cluster.sync();
+    *place = s.border;
+    return true;
   }
   // Histograms anew, for the way in steps.
   __device__ void clear_bins() {
@@ -362,7 +416,7 @@ template <typename T> struct Sampler {
   }
 
   // Which bins can the border be in?  -> s.first_bin, s.last_bin (of the places behind `above` elements with the weights above_mass)
-  __device__ void find_bins(bool by_mass, double limit, long long k, long long above, double above_mass) {
+  __device__ void find_bins(bool by_mass, double limit, long long k, long long above, double above_mass, double slack = 1e-9) {
     if (threadIdx.x == 0) {
       s.first_bin = kBins - 1;
       s.last_bin = 0;
@@ -376,8 +430,8 @@ template <typename T> struct Sampler {
       const double low_before = above_mass + block_before(count * low_w, s.sums, &total);
       const double high_before = above_mass + block_before(count * high_w, s.sums, &total);
       // kept for certain: all of a bin whose weights with those before it stay below the limit; left out for certain: low_before >= limit
-      if (count > 0 && low_before * (1.0 - 1e-9) < limit) {
-        if ((high_before + count * high_w) * (1.0 + 1e-9) >= limit) atomicMin(&s.first_bin, (int)threadIdx.x);
+      if (count > 0 && low_before * (1.0 - slack) < limit) {
+        if ((high_before + count * high_w) * (1.0 + slack) >= limit) atomicMin(&s.first_bin, (int)threadIdx.x);
         atomicMax(&s.last_bin, (int)threadIdx.x);
       }
     }
@@ -757,13 +811,17 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
     double mass = 0.0;
     // the short way: a list of all that can be kept
     int listed;
+    bool near = false, done = false;
+    const float near_unit = (float)((double)kNearBins * inv_t);
     if (cut_k) {
       const int bins = d.bins_of_top(top, top_at != 0x7fffffff, top_k);
       listed = d.list_above([&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * kTopBins, (float)(kBins - 1)); }, kTopBins, bins);
     } else {
-      const float unit = (float)((double)kNearBins * inv_t);
-      const int bins = d.bins_of_mass((double)top_p, unit, &mass);
-      listed = bins < kBins ? d.list_above([&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * unit, (float)(kBins - 1)); }, unit, bins) : kCandidates + 1;
+      const float unit = near_unit;
+      long long elements;
+      const int bins = d.bins_of_mass((double)top_p, unit, &mass, &elements);
+      near = bins < kBins;
+      listed = near && elements <= kCandidates ? d.list_above([&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * unit, (float)(kBins - 1)); }, unit, bins) : kCandidates + 1;
     }
     if (listed <= kCandidates) {
       bool open = false;
@@ -773,6 +831,9 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
       cluster.sync();
       if (!s.close) return;
     }
+    // the border by itself
+    if (near && listed > kCandidates) done = d.near_border((double)top_p, near_unit, mass, &least);
+    if (!done) {
     // the way in steps
     d.clear_bins();
     d.linear_bins(!cut_k, &mass);
@@ -788,6 +849,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
     if (cut_p && !both) {
       double unused;
       least = max(least, d.border(false, 0, true, (double)top_p * mass, &unused, &both));
+    }
     }
   }
 

@@ -518,6 +518,16 @@ def test_sample_wide_spread_of_weights():
         check_sample(l, u, 3.0, 0, p, 0.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("vocab", [5000, 40001, 151936])
+@pytest.mark.parametrize("temperature,top_p,top_k", [(1.3, 0.95, 0), (1.0, 0.5, 0), (2.0, 0.9, 0), (1.0, 0.99, 20000), (0.5, 0.9, 3000), (1.0, 1 - 2.0 ** -20, 0)])
+def test_sample_rows_that_keep_thousands(temperature, top_p, top_k, vocab, dtype):
+    """Broad rows: top_p and top_k leave more tokens than one list holds."""
+    g = gen(vocab + 1)
+    logits = rnd(g, 4, vocab, dtype=dtype, scale=1.5)
+    check_sample(logits, torch.rand(4, generator=g, device="cuda"), temperature, top_k, top_p, 0.0)
+
+
 def test_sample_of_the_last_rows_of_requests():
     g = gen(1)
     logits, u = rnd(g, 9, 5000, dtype=torch.float32, scale=2.0)[:, 7:4007], torch.rand(5, generator=g, device="cuda")
