@@ -599,7 +599,7 @@ cudaError_t launch_after(const void* kernel, dim3 grid, int threads, size_t smem
   return cudaLaunchKernelExC(&cfg, kernel, args);
 }
 
-constexpr int kMostSmem = 232448;  // of a CTA
+constexpr int kMostSmem = 232448 - 1024;  // of a CTA, without what the kernel declares
 template <typename T, int NT, int RING> int launch_rows(const AttnParams& p, bool behind_tiles, cudaStream_t s) {
   const int smem = RowWarp<T, NT, RING>::smem_bytes(p.a.requests);
   if constexpr (RING > 2) {
