@@ -131,10 +131,9 @@ struct Checks {
     }
     return t.data_ptr();
   }
-  // Rows that are written may not share memory, as those of an expanded tensor do.
-  static void apart(const at::Tensor& t, const char* what) {
-    const int n = (int)t.dim() - 1;
-    int64_t reach = kHeadDim;
+  // What is written may not share memory, as the rows of an expanded tensor do: n dimensions of entries of `reach` elements.
+  static void apart(const at::Tensor& t, const char* what) { apart(t, what, (int)t.dim() - 1, kHeadDim); }
+  static void apart(const at::Tensor& t, const char* what, int n, int64_t reach) {
     bool done[4] = {};
     for (int k = 0; k < n; ++k) {
       int best = -1;
@@ -250,6 +249,7 @@ PyObject* rotate_append(PyObject*, PyObject* const* v, Py_ssize_t n) {
   at::Tensor out = v[12] == Py_None ? new_rows(T, n_q, q) : tensor(v[12], "out");
   a.out = c.rows(out, "out", dt, T, n_q, a.out_stride);
   Checks::apart(out, "out");
+  need(a.out != a.q || (a.out_stride[0] == a.q_stride[0] && a.out_stride[1] == a.q_stride[1]), "out", " shares memory with q and has other strides");
   a.dtype = code(dt);
   a.table_dtype = code(cos.scalar_type());
   a.tokens = (int32_t)T;
@@ -296,6 +296,7 @@ PyObject* chunk_attention(PyObject*, PyObject* const* v, Py_ssize_t n) {
   if (const at::Tensor* t = maybe(v[11], "lse")) {
     c.type(*t, "lse", at::kFloat);
     REFUSE_IF(t->dim() != 2 || t->size(0) != T || t->size(1) != n_q, "lse.shape: ", t->sizes(), ", [", T, ", ", n_q, "] is needed");
+    Checks::apart(*t, "lse", 2, 1);
     a.lse = static_cast<float*>(t->data_ptr());
     a.lse_stride[0] = t->stride(0);
     a.lse_stride[1] = t->stride(1);

@@ -196,6 +196,7 @@ extern "C" int mk_rotate_append(const mk_rotate_append_args* args, void* stream)
     return fail(MK_E_INVALID, "rotate_append: sizes must be positive");
   if ((long long)a.tokens * ((long long)a.q_heads + 2ll * a.kv_heads) > 0x7fffffff / kRowLanes) return fail(MK_E_TOO_LARGE, "rotate_append: too many rows");
   if (a.tokens == 0) return 0;
+  if (a.k_cache == a.v_cache) return fail(MK_E_INVALID, "rotate_append: k_cache and v_cache share memory");
   bool wide = aligned16(a.q) && aligned16(a.k) && aligned16(a.v) && aligned16(a.cos) && aligned16(a.sin) && aligned16(a.k_cache) &&
               aligned16(a.v_cache) && aligned16(a.out) && aligned16(a.q_norm) && aligned16(a.k_norm);
   for (int i = 0; i < 2; ++i) wide = wide && !((a.q_stride[i] | a.k_stride[i] | a.v_stride[i] | a.out_stride[i] | a.table_stride[i]) & 7);

@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
   const unsigned longest = (unsigned)min((long long)a.table_width * page, 0x7fffffffll);  // what a row of the block table can hold
   auto length_of = [&](int r) { return (int)min((unsigned)max(0, __ldg(a.lengths + r)), longest); };
   auto divided = [&](unsigned n) { return p.shift >= 0 ? n >> p.shift : n / (unsigned)page; };
-  auto pages_of = [&](unsigned n) { return n ? (int)(divided(n - 1) + 1) : 0; };
+  auto pages_of = [&](unsigned n) { return n ? (int)min(divided(n - 1) + 1, 0x7fffffffu) : 0; };  // (a length with more is refused)
 
   // pages that ended requests give back: they count as free in this step already
   long long back = 0, total[3];
@@ -144,18 +144,17 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     return k < held ? a.block_table[(long long)r * a.table_stride + k] : taken_page((long long)need0[r] + k - held);
   };
 
-  const long long n_kv = min(kv, (long long)a.max_indices);
   const long long n_back = ring > 0 ? back : 0;
-  const long long all = n_kv + a.max_tokens + n_back;
+  const long long all = kv + a.max_tokens + n_back;
   for (long long e = (long long)blockIdx.x * kPlanThreads + threadIdx.x; e < all; e += (long long)gridDim.x * kPlanThreads) {
-    if (e < n_kv) {  // an entry of the page index; a new page enters its request's table as well
+    if (e < kv) {  // an entry of the page index; a new page enters its request's table as well
       const int r = find_owner(R, e, [&](int k) { return (long long)kv0[k]; });
       const int k = (int)e - kv0[r], held = pages_of(length_of(r));
       const int pg = page_at(r, k);
-      a.kv_indices[e] = pg;
+      if (e < a.max_indices) a.kv_indices[e] = pg;
       if (k >= held) a.block_table[(long long)r * a.table_stride + k] = pg;
-    } else if (e < n_kv + a.max_tokens) {  // a token row: its position and cache slot
-      const int t = (int)(e - n_kv);
+    } else if (e < kv + a.max_tokens) {  // a token row: its position and cache slot
+      const int t = (int)(e - kv);
       long long slot = -1;
       int pos = 0;
       if (t < tokens) {
@@ -167,7 +166,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
       a.slots[t] = slot;
       a.positions[t] = pos;
     } else {  // a page given back
-      const int b = (int)(e - n_kv - a.max_tokens);
+      const int b = (int)(e - kv - a.max_tokens);
       const int r = find_owner(R, b, [&](int k) { return (long long)back0[k]; });
       a.free_pages[(tail_at + b) % ring] = a.block_table[(long long)r * a.table_stride + (b - back0[r])];
     }
@@ -207,8 +206,33 @@ extern "C" int mk_plan_step(const mk_step_plan_args* args, void* stream) {
     return fail(a.requests < 1 ? MK_E_INVALID : MK_E_TOO_LARGE, "plan_step: %d requests (1 to %d)", a.requests, MK_STEP_MAX_REQUESTS);
   if (a.page_size < 1 || a.table_width < 1 || a.table_stride < a.table_width || a.max_tokens < 1 || a.max_indices < 1 || a.ring_size < 1)
     return fail(MK_E_INVALID, "plan_step: sizes must be positive and table rows may not overlap");
-  if ((long long)a.requests * a.table_width > 0x7fffffffll) return fail(MK_E_TOO_LARGE, "plan_step: block table of over 2^31 entries");
-  const size_t smem = 4 * (size_t)(a.requests + 1) * sizeof(int);
+  if ((long long)a.requests * a.table_width >= 0x7fffffffll) return fail(MK_E_TOO_LARGE, "plan_step: block table of over 2^31 entries");
+  // Every CTA works the sums out for itself, so what one writes no other may read or write.
+  const size_t n = (size_t)a.requests;
+  const struct {
+    const void* at;
+    size_t bytes;
+    const char* name;
+  } arrays[] = {{a.block_table, ((n - 1) * (size_t)a.table_stride + (size_t)a.table_width) * 4, "block_table"},
+                {a.free_pages, (size_t)a.ring_size * 4, "free_pages"},
+                {a.qo_indptr, (n + 1) * 4, "qo_indptr"},
+                {a.kv_indptr, (n + 1) * 4, "kv_indptr"},
+                {a.kv_indices, (size_t)a.max_indices * 4, "kv_indices"},
+                {a.last_page_len, n * 4, "last_page_len"},
+                {a.slots, (size_t)a.max_tokens * 8, "slots"},
+                {a.positions, (size_t)a.max_tokens * 4, "positions"},
+                {a.granted, n * 4, "granted"},
+                {a.free_range_out, 16, "free_range"},
+                {a.lengths, n * 4, "lengths"},
+                {a.new_tokens, n * 4, "new_tokens"},
+                {a.free_range_in, 16, "free_range"}};
+  constexpr int kWritten = 10;
+  for (int i = 0; i < kWritten; ++i)
+    for (int j = i + 1; j < (int)(sizeof arrays / sizeof *arrays); ++j) {
+      const uintptr_t x = (uintptr_t)arrays[i].at, y = (uintptr_t)arrays[j].at;
+      if (x < y + arrays[j].bytes && y < x + arrays[i].bytes) return fail(MK_E_INVALID, "plan_step: %s and %s share memory", arrays[i].name, arrays[j].name);
+    }
+  const size_t smem = 4 * (n + 1) * sizeof(int);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return fail(MK_E_CUDA, "plan_step: %s", cudaGetErrorString(e));

@@ -50,11 +50,11 @@ def _load():
 # ------------------------------------------------------------------------------------
 @dataclass
 class StepPlan:
-    """What ``plan_step`` writes, for up to ``len(granted)`` requests and ``len(slots)`` token rows.  The first four may be the meta
-    tensors of a ``PersistentKernel``."""
+    """What ``plan_step`` writes, for ``len(granted)`` requests and up to ``len(slots)`` token rows.  The first four may be the meta
+    tensors of a ``PersistentKernel``.  No two tensors of a call may share memory."""
     qo_indptr: torch.Tensor      # [requests + 1] int32: first token row of every request
     kv_indptr: torch.Tensor      # [requests + 1] int32: its first entry of kv_indices
-    kv_indices: torch.Tensor     # [pages] int32: the pages of every request in order
+    kv_indices: torch.Tensor     # [pages] int32: the pages of every request in order (those behind its end are left out)
     last_page_len: torch.Tensor  # [requests] int32: tokens in its last page, the new ones included (0: no page)
     slots: torch.Tensor          # [tokens] int64: cache row (page * page_size + row in the page) of every new token, -1 behind the last
     positions: torch.Tensor      # [tokens] int32: its position in its request
@@ -94,7 +94,7 @@ def rotate_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_norm=
     q [tokens, q_heads, 128], k and v [tokens, kv_heads, 128]: bf16 or fp16, any token and head stride (slices of one projection).  cos and
     sin [positions, 128], of the rows' type or fp32; row ``positions[t]`` is used.  norm(x) = w x / sqrt(mean(x^2) + eps) where ``q_norm`` /
     ``k_norm`` [128] are given.  fp32 throughout, rounded once.  Tokens with a slot or position outside (-1: padding) are left out,
-    their rows of ``out`` as they were.  A slot may not occur twice."""
+    their rows of ``out`` as they were.  A slot may not occur twice; ``out`` may be q."""
     return (_native or _load()).rotate_append(q, k, v, cos, sin, positions, slots, k_cache, v_cache, q_norm, k_norm, eps, out)
 
 
@@ -111,7 +111,7 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, last_
     p - window and the first ``sinks``.  ``scale``: 1/sqrt(128) if None.  Rows behind the last request are left as they were; a row that
     sees nothing is zero.  ``lse`` [tokens, q_heads] fp32, if given, takes the natural logarithm of each row's sum of weights.
     ``max_new``: the largest number of new tokens of a request, if the caller knows it; it chooses kernels, nothing else depends on it.
-    Returns ``out`` [tokens, q_heads, 128], which may not be q."""
+    Returns ``out`` [tokens, q_heads, 128], which may not share memory with q."""
     return (_native or _load()).chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, last_page_len, scale, window, sinks, out, lse, max_new)
 
 

@@ -147,6 +147,36 @@ def test_plan_where_a_table_row_is_too_short():
     run_plan([16, 3, 30], [1, 30, 1], 16, 9, 50, width_more=-1)
 
 
+def test_plan_of_more_tokens_than_there_are_positions():
+    """A request for as many tokens as an int holds, on pages of one token, is granted nothing and takes nothing from those behind it."""
+    for page in (1, 2):
+        lengths, new = i32([9, 4, 3]), i32([2 ** 31 - 1, 2, 5])
+        table = torch.full((3, 12), -7, dtype=torch.int32, device="cuda")
+        held = [-(-n // page) for n in (9, 4, 3)]
+        for r, h in enumerate(held):
+            table[r, :h] = torch.arange(h, dtype=torch.int32, device="cuda") + 20 * r
+        plan = mk.StepPlan.empty(3, 16, 40)
+        after = [-(-n // page) for n in (9, 6, 8)]
+        free = sum(after) - sum(held) - 1  # one page too few for the last
+        mk.plan_step(lengths, new, table, i32(list(range(100, 110))), torch.tensor([0, free], device="cuda"), page, plan)
+        assert plan.granted.tolist() == [0, 2, 0] and plan.qo_indptr.tolist() == [0, 0, 2, 2]
+        assert plan.free_range.tolist() == [after[1] - held[1], free]
+        assert plan.positions.tolist() == [4, 5] + [0] * 14
+
+
+def test_plan_with_a_page_index_that_is_too_short():
+    """The index ends where its tensor ends; tables, slots and positions are those of the whole step."""
+    plan, short = mk.StepPlan.empty(2, 8, 12), mk.StepPlan.empty(2, 8, 3)
+    tables = []
+    for p in (plan, short):
+        table = torch.tensor([[0, 1, -7, -7], [2, 3, -7, -7]], dtype=torch.int32, device="cuda")
+        mk.plan_step(i32([8, 7]), i32([2, 6]), table, i32([9, 8, 7]), torch.tensor([0, 3], device="cuda"), 4, p)
+        tables.append(table)
+    assert tables[0].tolist() == [[0, 1, 9, -7], [2, 3, 8, 7]] and torch.equal(tables[0], tables[1])
+    assert plan.kv_indices.tolist() == [0, 1, 9, 2, 3, 8, 7] + [0] * 5 and short.kv_indices.tolist() == [0, 1, 9]
+    assert torch.equal(plan.slots, short.slots) and torch.equal(plan.positions, short.positions) and torch.equal(plan.free_range, short.free_range)
+
+
 def test_plan_many_requests():
     new = [(-1 if i % 31 == 7 else i % 3) for i in range(2500)]
     run_plan([(i * 37) % 300 for i in range(2500)], new, 16, 2000, 2600)
@@ -226,6 +256,21 @@ def test_rotate_append_position_and_slot_bounds():
     kc, vc, out = torch.zeros(1, 2, 2, D, device="cuda", dtype=BF), torch.zeros(1, 2, 2, D, device="cuda", dtype=BF), torch.zeros(3, 2, D, device="cuda", dtype=BF)
     mk.rotate_append(q, k, v, cos, sin, i32([4, -1, 0]), torch.tensor([0, 1, 2], device="cuda"), kc, vc, out=out)
     assert not kc.any() and not vc.any() and not out.any()
+
+
+def test_rotate_append_in_place():
+    g = gen(3)
+    x = rnd(g, 70, 10 * D).view(70, 10, D)
+    q, k, v = x.split([6, 2, 2], 1)
+    ang = torch.rand(80, D, generator=g, device="cuda")
+    args = (ang.cos(), ang.sin(), torch.arange(70, device="cuda", dtype=torch.int32), torch.arange(70, device="cuda"))
+    caches = [torch.zeros(5, 16, 2, D, device="cuda", dtype=BF) for _ in range(4)]
+    want = mk.rotate_append(q, k, v, *args, *caches[:2], rnd(g, D), rnd(g, D), 1e-6)
+    g2 = gen(3)
+    rnd(g2, 70, 10 * D), torch.rand(80, D, generator=g2, device="cuda")
+    kept = x[:, 6:].clone()
+    assert mk.rotate_append(q, k, v, *args, *caches[2:], rnd(g2, D), rnd(g2, D), 1e-6, out=q) is q
+    assert torch.equal(q, want) and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3]) and torch.equal(x[:, 6:], kept)
 
 
 # ------------------------------------------------------------------------------------
@@ -313,6 +358,12 @@ def test_attention_of_single_tokens(n_q, n_kv, page, dtype):
 @pytest.mark.parametrize("max_new", [0, 1])
 def test_attention_of_one_request(cached, max_new):
     Batch([(cached, 1)], 8, 2, 64).check(max_new=max_new)
+
+
+@pytest.mark.parametrize("requests", [250, 288, 300, 319, 320, 1000])
+def test_attention_of_many_single_tokens(requests):
+    """The table of the requests and the stages share the row kernel's shared memory."""
+    Batch([((7 * i) % 50, 1) for i in range(requests)], 8, 2, 16).check()
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])

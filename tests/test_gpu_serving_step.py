@@ -295,6 +295,7 @@ def test_attention_refusals():
                          (dict(k_cache=b.k[:, :, :1]), "v_cache"), (dict(kv_indices=b.kv_indices.long()), "dtype"), (dict(qo_indptr=b.qo_indptr[:2]), "qo_indptr"),
                          (dict(last_page_len=b.last[None]), "one dimension"), (dict(window=-1), "window"), (dict(sinks=-2), "sinks"), (dict(out=b.q), "may not be q"),
                          (dict(out=b.out[:1].expand(3, 8, D)), "share memory"), (dict(out=b.out.cpu()), "is on cpu"), (dict(lse=torch.zeros(3, 7, device="cuda")), "lse"),
+                         (dict(lse=torch.zeros(3, 1, device="cuda").expand(3, 8)), "share memory"),
                          (dict(q=wide[..., :D]), "multiples of 16 bytes"), (dict(kv_indices=torch.zeros(40, dtype=torch.int32, device="cuda")[::2]), "contiguous"),
                          (dict(q=[1]), "tensor is needed"), (dict(q=b.q.clone().requires_grad_()), "gradient")]:
         with pytest.raises(ValueError, match=text):
@@ -314,14 +315,17 @@ def test_other_refusals():
     ok = dict(lengths=i32([1, 2]), new_tokens=i32([1, 1]), block_table=z(2, 3, dt=torch.int32), free_pages=i32([5, 6]), free_range=z(2, dt=torch.int64), page_size=4, plan=plan)
     for change, text in [(dict(new_tokens=i32([1])), "new_tokens"), (dict(block_table=z(3, 3, dt=torch.int32)), "block_table"), (dict(page_size=0), "page_size"),
                          (dict(free_range=plan.free_range), "may not be"), (dict(plan=None), "StepPlan"), (dict(block_table=z(1, 3, dt=torch.int32).expand(2, 3)), "apart"),
-                         (dict(lengths=torch.ones(2, device="cuda")), "dtype")]:
+                         (dict(lengths=torch.ones(2, device="cuda")), "dtype"), (dict(new_tokens=plan.granted), "granted and new_tokens share"),
+                         (dict(lengths=plan.positions[1:3]), "positions and lengths share"), (dict(free_pages=plan.kv_indices), "free_pages and kv_indices share")]:
         with pytest.raises(ValueError, match=text):
             mk.plan_step(**{**ok, **change})
+    qq = z(3, 4, D, dt=BF)
     q, kv, cache, t = z(3, 4, D, dt=BF), z(3, 2, D, dt=BF), z(2, 4, 2, D, dt=BF), z(9, D, dt=BF)
     ok = dict(q=q, k=kv, v=kv, cos=t, sin=t, positions=i32([0, 1, 2]), slots=z(3, dt=torch.int64), k_cache=cache, v_cache=cache.clone())
     for change, text in [(dict(k=kv[:2]), "k.shape"), (dict(v=z(3, 1, D, dt=BF)), "v.shape"), (dict(cos=t.half()), "dtype"), (dict(sin=t[:4]), "sin"),
                          (dict(positions=z(3, dt=torch.int64)), "dtype"), (dict(k_cache=z(2, 4, 1, D, dt=BF)), "kv heads"), (dict(q_norm=z(64, dt=BF)), "q_norm"),
-                         (dict(k_cache=cache[:1].expand(2, 4, 2, D)), "share memory"), (dict(out=z(3, 4, D)), "dtype")]:
+                         (dict(k_cache=cache[:1].expand(2, 4, 2, D)), "share memory"), (dict(out=z(3, 4, D)), "dtype"),
+                         (dict(v_cache=cache), "k_cache and v_cache share"), (dict(q=qq, out=qq.as_strided((3, 4, D), (D, 3 * D, 1))), "other strides")]:
         with pytest.raises(ValueError, match=text):
             mk.rotate_append(**{**ok, **change})
     for args, text in [((z(2, 9).double(), z(2)), "fp32"), ((z(2, 9), z(3)), "rows of logits"), ((z(2, 9), z(2).double()), "dtype"), ((z(9), z(1)), "vocab"),

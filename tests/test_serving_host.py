@@ -81,6 +81,19 @@ def test_sample_refusals(native_lib, change, code, text):
     refused(native_lib, "mk_sample_tokens", filled(_cabi.MkSampleArgs, **{"dtype": _cabi.MK_F32, **change}), code, text)
 
 
+def test_arrays_that_share_memory_are_refused(native_lib):
+    names = [n for n, kind in _cabi.MkStepPlanArgs._fields_ if kind is C.c_void_p]
+    apart = {n: FAKE + (k << 12) for k, n in enumerate(names)}
+    written = [n for n in names if n not in ("lengths", "new_tokens", "free_range_in")]
+    for name in written:
+        for other in names:
+            if other != name:
+                refused(native_lib, "mk_plan_step", filled(_cabi.MkStepPlanArgs, **{**apart, "table_stride": 1, "requests": 4, "max_indices": 4, "max_tokens": 4, "ring_size": 4, other: apart[name] + 4}),
+                        _cabi.MK_E_INVALID, "share memory")
+    a = filled(_cabi.MkRotateAppendArgs, dtype=_cabi.MK_BF16, table_dtype=_cabi.MK_F32)
+    refused(native_lib, "mk_rotate_append", a, _cabi.MK_E_INVALID, "k_cache and v_cache share")
+
+
 def test_null_arguments_and_empty_calls(native_lib):
     for fn in ("mk_plan_step", "mk_rotate_append", "mk_chunk_attention", "mk_sample_tokens"):
         refused(native_lib, fn, None, _cabi.MK_E_INVALID, "null")
