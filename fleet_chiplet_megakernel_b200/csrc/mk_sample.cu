@@ -9,7 +9,7 @@
 // A token is a whole number: with sums in fp32 one draw in some thousands would fall on the neighbour's side of a border.  Weights
 // and their sums are therefore 64-bit, and every sum has one fixed order (no atomics on anything but counts).
 //
-// A row is taken by a cluster of up to 8 CTAs, as many as leave no SM with two; each has a contiguous part of the vocabulary and
+// A row is taken by a cluster of up to 8 CTAs, as many as run at once for all rows; each has a contiguous part of the vocabulary and
 // reads it two to four times in 16-byte words, from L2 after the first.  What is kept is mostly a few tokens, so the usual way is to find a
 // bound that few logits exceed, to list these, and to do the rest of the work on the sorted list in one CTA:
 //   top_k: at least k threads of the first pass hold a logit of at least the k-th largest of the threads' maxima, so a histogram
@@ -19,8 +19,9 @@
 // Where the list would be too long, or the border too close, the border is found step by step with sums in 64 bits: bins that the
 // border can be in, the weights above them, and again over the candidates' range of (logit, index), which a step divides by 1024;
 // the draw then reads the row once more.  CTAs hand each other sums by storing them into their neighbours' shared memory ahead of a
-// cluster barrier.  A weight in 64 bits is 10 operations, 64 a cycle and SM: the rows that keep all tokens are bound by these, the
-// others by the latency of the steps, and from some tens of rows on by the reads.
+// cluster barrier.  Rows that keep all tokens or thousands are bound by the instructions of the weights in 64 bits (some 40 a logit), the
+// others by the latency of the steps.  151936 fp32 logits, 1 and 64 rows: largest logit 5 and 9 us, all tokens 18 and 35, top_k = 50 15
+// and 22, top_p that keeps some thousands 44 and 87; the 64 rows take 6 us of the memory's time once.
 #include <cooperative_groups.h>
 
 #include "mk_serving.cuh"
@@ -68,6 +69,7 @@ struct SampleShared {
   uint64_t border;                  // written by rank 0 into every CTA
   double border_mass;
   int first_bin, last_bin, last_kept;
+  uint32_t range[2];                // of the list that is being sorted: largest, smallest upper half
 };
 
 // A row, as the groups of 16 bytes (aligned) that it lies in: the first and the last may have elements outside.
@@ -110,23 +112,23 @@ template <typename T> struct Row {
     }
     return outside;
   }
+  float plain;        // from this logit on a weight needs no care: it is a normal number, and neither infinity nor NaN is in its way
   // exp((l - top) / temperature): the argument y in units of ln 2 / 64, its whole part by table (P. T. P. Tang's method, 1989), the rest
   // r (|r| <= 1/2) by the series up to the fourth power; the next term is 4e-14.
-  __device__ __forceinline__ double weight(float l) const {
-    if (l == top) return 1.0;  // (both may be infinite)
+  __device__ __forceinline__ double plain_weight(float l) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: a sum with it is rounded to a whole number
     constexpr double c1 = 0.6931471805599453094 / 64.0, c2 = c1 * c1 / 2.0, c3 = c2 * c1 / 3.0, c4 = c3 * c1 / 4.0;
-    const double x = (double)l, y = fma(x, scale, -top_scaled);
-    if (!(y >= -64.0 * 1021.0)) return far_weight(l);
-    const double big = y + kRound;
+    const double y = fma((double)l, scale, -top_scaled), big = y + kRound;
     const int n = __double2loint(big);
     const double r = y - (big - kRound);
     const double t = power[n & 63];
     const double e = fma(t * r, fma(r, fma(r, fma(r, c4, c3), c2), c1), t);
     return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
   }
+  // (exactly 1 for the largest: it may not fall below min_p = 1)
+  __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : l >= plain ? plain_weight(l) : far_weight(l, top, scale); }
   // next to the smallest numbers, and where infinities meet
-  __device__ __noinline__ double far_weight(float l) const {
+  static __device__ __noinline__ double far_weight(float l, float top, double scale) {
     const double y = ((double)l - (double)top) * scale;
     return l == -INFINITY || isnan(y) ? 0.0 : exp(y * (0.6931471805599453094 / 64.0));
   }
@@ -438,8 +440,8 @@ template <typename T> struct Sampler {
     __syncthreads();
   }
 
-  // Sorts s.list[0 .. n), the largest first, zeros last; all of it is there on return, up to the power of two.
-  __device__ __noinline__ void sort_list(int n_list) {
+  // Sorts s.list[0 .. n), the largest first, zeros behind them.  The upper half of an entry: LOGITS: the key of a logit, else ~index.
+  template <bool LOGITS> static __device__ __noinline__ void sort_list(SampleShared& s, int n_list) {
     const int t = threadIdx.x;
     __syncthreads();
     if (n_list <= kThreads / 8) {
@@ -456,20 +458,74 @@ template <typename T> struct Sampler {
       __syncthreads();
       return;
     }
+    // More: into bins that are even between the smallest and the largest, and counted within them as long as they hold few.
+    // (top_k = 1000 of 151936 fp32 logits, both sorts in it: 24 us like this, 46 by sort_by_steps.)
+    const uint64_t x[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
+    const uint32_t a = x[0] >> 32, b = x[1] >> 32;
+    const uint32_t most = __reduce_max_sync(kAll, max(a, b)), least = __reduce_min_sync(kAll, min(x[0] ? a : ~0u, x[1] ? b : ~0u));
+    if (t == 0) s.range[0] = 0, s.range[1] = ~0u;
+    s.hist[t] = 0;
+    __syncthreads();
+    if ((t & 31) == 0) {
+      atomicMax(&s.range[0], most);
+      atomicMin(&s.range[1], least);
+    }
+    __syncthreads();
+    const uint32_t hi = s.range[0], lo = s.range[1];
+    auto below = [&](uint32_t v) -> float { return LOGITS ? logit_of(hi) - logit_of(v) : (float)(hi - v); };
+    const float per = (float)(kBins - 1) / below(lo);
+    int bin[2], at[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      bin[h] = min(kBins - 1, (int)(below(x[h] >> 32) * per));  // (does not fall; 0 where the range is not finite)
+      if (x[h]) at[h] = (int)atomicAdd(&s.hist[bin[h]], 1u);
+    }
+    __syncthreads();
+    const uint32_t mine = s.hist[t];
+    uint64_t total;
+    const uint64_t before = block_before((uint64_t)mine, s.words, &total);
+    if (__syncthreads_or(mine > 64)) {
+      sort_by_steps(s, n_list);
+      return;
+    }
+    s.inner[t] = (uint32_t)before;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (x[h]) s.list[s.inner[bin[h]] + at[h]] = x[h];
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      at[h] = 0;
+      if (!x[h]) continue;
+      const int i0 = (int)s.inner[bin[h]], n = (int)s.hist[bin[h]];
+      at[h] = i0;
+      for (int j = i0; j < i0 + n; ++j) at[h] += s.list[j] > x[h];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (x[h]) s.list[at[h]] = x[h];
+      if (t + h * kThreads >= n_list) s.list[t + h * kThreads] = 0;
+    }
+    __syncthreads();
+  }
+  static __device__ __noinline__ void sort_by_steps(SampleShared& s, int n_list) {
+    const int t = threadIdx.x;
     int n = kThreads / 4;
     while (n < n_list) n <<= 1;
     uint64_t x0 = t < n_list ? s.list[t] : 0, x1 = t + kThreads < n_list ? s.list[t + kThreads] : 0;
     if (n <= kThreads) {
-      sort_steps<false>(x0, x1, n);
+      sort_steps<false>(s, x0, x1, n);
     } else {
-      sort_steps<true>(x0, x1, n);
+      sort_steps<true>(s, x0, x1, n);
     }
     __syncthreads();
     s.list[t] = x0;
-    if (n > kThreads) s.list[t + kThreads] = x1;
+    s.list[t + kThreads] = x1;
     __syncthreads();
   }
-  template <bool BOTH> __device__ __forceinline__ void sort_steps(uint64_t& x0, uint64_t& x1, int n) {
+  template <bool BOTH> static __device__ __forceinline__ void sort_steps(SampleShared& s, uint64_t& x0, uint64_t& x1, int n) {
     const int t = threadIdx.x;
     // the earlier of two places takes the larger where the run falls, else the smaller
     auto pick = [](uint64_t x, uint64_t y, bool larger) { return larger == (x > y) ? x : y; };
@@ -518,7 +574,7 @@ template <typename T> struct Sampler {
   // kSumError; false where that leaves the border open.
   __device__ bool draw(int n_list, bool by_k, int k, bool by_mass, double top_p, double mass, float min_p, double u, int64_t* token, float* logprob) {
     const int t = threadIdx.x;
-    sort_list(n_list);
+    sort_list<true>(s, n_list);
     const uint64_t place[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
     bool keep[2], open = false;
     double w[2], before[2], total;
@@ -548,7 +604,7 @@ template <typename T> struct Sampler {
     for (int h = 0; h < 2; ++h) s.list[t + h * kThreads] = keep[h] ? (place[h] & 0xffffffffu) << 32 | (uint32_t)(t + h * kThreads + 1) : 0;
     // (what is kept is the beginning of the sorted list)
     const int kept = __syncthreads_count(keep[0]) + (n_list > kThreads ? __syncthreads_count(keep[1]) : 0);
-    sort_list(kept);
+    sort_list<false>(s, kept);
     const uint64_t by_index[2] = {t < kept ? s.list[t] : 0, t + kThreads < kept ? s.list[t + kThreads] : 0};
 #pragma unroll
     for (int h = 0; h < 2; ++h) w[h] = t + h * kThreads < kept ? s.weights[(uint32_t)by_index[h] - 1] : 0.0;
@@ -571,7 +627,7 @@ template <typename T> struct Sampler {
   // of the order are kept; by_mass: those before which less than `limit` lies, with by_k less than limit times the first k's weights.
   __device__ void cut(int n_list, bool by_k, long long k, bool by_mass, double limit, long long above, double mass) {
     const int t = threadIdx.x;
-    sort_list(n_list);
+    sort_list<true>(s, n_list);
     const uint64_t place[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
     if (t == 0) s.last_kept = 0;
     bool keep[2];
@@ -803,6 +859,8 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
   const double inv_t = 1.0 / (double)temperature;
   r.scale = inv_t * (64.0 / 0.6931471805599453094);
   r.top_scaled = (double)r.top * r.scale;
+  // (rounded up; exp(-700) is 1e-304.  With an infinite largest logit or temperature no logit, or every finite one, is plain.)
+  r.plain = r.top == INFINITY ? __uint_as_float(0x7fc00000u) : fmaxf(__double2float_ru((double)r.top - 700.0 * (double)temperature), -3.4028235e38f);
   d.per_bin = (float)(kBinsPerUnit * inv_t);
 
   uint64_t least = 0;  // the border: places from here on are kept
@@ -857,25 +915,39 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int part = ((r.g1 - r.g0 + kWarps - 1) / kWarps + 31) / 32 * 32;
   const int b0 = min(r.g1, r.g0 + warp * part), b1 = min(r.g1, b0 + part);
-  // (min_p: a bound that is safely too low; the weight itself decides)
-  const float least_logit = fmaxf(least ? logit_of((uint32_t)(least >> 32)) : -INFINITY,
-                                  min_p > 0.f ? r.top + temperature * (logf(min_p) - 1e-3f) * 1.0001f - fabsf(r.top) * 1e-6f : -INFINITY);
-  auto kept = [&](float l, int i) -> double {
+  // (min_p: bounds that are safely too low and too high; between them the weight itself decides)
+  const float min_at = r.top + temperature * logf(fmaxf(min_p, 1e-45f)), min_off = (fabsf(r.top) + fabsf(min_at)) * 1e-6f + temperature * 1e-3f;
+  const float border_logit = least ? logit_of((uint32_t)(least >> 32)) : -INFINITY;
+  const float least_logit = fmaxf(border_logit, min_p > 0.f ? min_at - min_off : -INFINITY);
+  const bool never = isnan(r.plain) || (min_p > 0.f && !(min_at + min_off < INFINITY));
+  const float sure = never ? __uint_as_float(0x7fc00000u) : fmaxf(r.plain, min_p > 0.f ? min_at + min_off : -INFINITY);
+  auto perhaps = [&](float l, int i) -> double {
     if (l < least_logit || (least != 0 && place_of(l, i) < least)) return 0.0;
     const double w = r.weight(l);
     return min_p > 0.f && w < (double)min_p ? 0.0 : w;
   };
   auto kept_group = [&](int g, double (&w)[N]) -> double {  // and their sum, in order
     float l[N];
-    uint32_t outside = 0;
+    uint32_t outside = 0, unsure = 0;
     if (r.inside(g)) r.load(g, l);
     else outside = r.load_edge(g, l);
-    double sum = 0.0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      w[e] = outside >> e & 1 ? 0.0 : kept(l[e], r.index(g) + e);
-      sum += w[e];
+      const bool keep = l[e] >= sure && l[e] > border_logit;
+      w[e] = keep ? r.plain_weight(l[e]) : 0.0;
+      unsure |= keep || l[e] < least_logit ? 0u : 1u << e;
     }
+    unsure &= ~outside;
+    while (unsure) {  // (at a border, or next to the smallest numbers)
+      const int k = __ffs(unsure) - 1, i = r.index(g) + k;
+      unsure &= unsure - 1;
+      const double x = perhaps(clean(to_float(r.logits[i])), i);
+#pragma unroll
+      for (int e = 0; e < N; ++e) w[e] = e == k ? x : w[e];
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) sum += w[e];
     return sum;
   };
   double mine = 0.0;
@@ -922,12 +994,34 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
     }
     end += m;
   }
+  // That warp's part again, dealt out to all warps: its sums say which of them has the token.
+  const int o0 = min(r.g1, r.g0 + owner * part), o1 = min(r.g1, o0 + part), share = ((o1 - o0 + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int p0 = min(o1, o0 + warp * share), p1 = min(o1, p0 + share);
+  mine = 0.0;
+  for (int g = p0 + lane; g < p1; g += 32) {
+    double w[N];
+    mine += kept_group(g, w);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kAll, mine, o);
+  if (lane == 0) s.weights[warp] = mine;
+  __syncthreads();
+  end = from;
+  owner = -1;
+  for (int w = 0; w < kWarps; ++w) {
+    const double m = s.weights[w];
+    if (m > 0.0 && (owner < 0 || goal >= end)) {
+      owner = w;
+      from = end;
+    }
+    end += m;
+  }
   if (warp != owner) return;
   int token = -1;
   double w_token = 0.0, run = from;
-  for (int i0 = b0; i0 < b1; i0 += 32) {
+  for (int i0 = p0; i0 < p1; i0 += 32) {
     double w[N] = {};
-    const double sum = i0 + lane < b1 ? kept_group(i0 + lane, w) : 0.0;
+    const double sum = i0 + lane < p1 ? kept_group(i0 + lane, w) : 0.0;
     double up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -964,17 +1058,33 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
   }
 }
 
-template <typename T> cudaError_t launch(const mk_sample_args& a, int ranks, cudaStream_t s) {
+template <typename T> cudaError_t launch(const mk_sample_args& a, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ranks * a.requests));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  // The widest cluster of which the device runs as many at once as there are rows.  (A cluster lies within a group of SMs: 16 rows on
+  // clusters of 8, which take 128 of 148 SMs, need two turns: top_k = 50 of 151936 fp32 logits 30 us, 20 on clusters of 4.)
+  static int at_once[64][4] = {};
+  int dev = 0, ranks = kMaxCluster;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) ranks = 1;
+  for (int k = 3; ranks > 1; ranks >>= 1, --k) {
+    if (a.vocab / ranks < 1024 || (long long)ranks * a.requests > sm_count()) continue;
+    cfg.gridDim = dim3((unsigned)ranks);
+    attr[0].val.clusterDim.x = (unsigned)ranks;
+    if (at_once[dev][k] == 0) {
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<T>, &cfg) != cudaSuccess) n = 0;
+      at_once[dev][k] = n > 0 ? n : -1;
+    }
+    if (a.requests <= at_once[dev][k]) break;
+  }
+  cfg.gridDim = dim3((unsigned)(ranks * a.requests));
+  attr[0].val.clusterDim.x = (unsigned)ranks;
   return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a);
 }
 
@@ -991,9 +1101,7 @@ extern "C" int mk_sample_tokens(const mk_sample_args* args, void* stream) {
   if (a.requests > 0x7fffffff / kMaxCluster) return fail(MK_E_TOO_LARGE, "sample_tokens: %d requests", a.requests);
   if (!a.qo_indptr && a.rows < a.requests) return fail(MK_E_INVALID, "sample_tokens: %d rows of logits for %d requests", a.rows, a.requests);
   if (a.requests == 0) return 0;
-  int ranks = kMaxCluster;
-  while (ranks > 1 && ((long long)ranks * a.requests > sm_count() || a.vocab / ranks < 1024)) ranks >>= 1;
   const cudaStream_t st = (cudaStream_t)stream;
-  const cudaError_t e = a.dtype == MK_F32 ? launch<float>(a, ranks, st) : a.dtype == MK_BF16 ? launch<__nv_bfloat16>(a, ranks, st) : launch<__half>(a, ranks, st);
+  const cudaError_t e = a.dtype == MK_F32 ? launch<float>(a, st) : a.dtype == MK_BF16 ? launch<__nv_bfloat16>(a, st) : launch<__half>(a, st);
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "sample_tokens: launch failed: %s", cudaGetErrorString(e));
 }
