@@ -632,12 +632,18 @@ Layout layout_of(const mk_chunk_attention_args& a) {
   l.tiles = most * per_kv > kFewRows && tiles_take(a);
   l.rows = !l.tiles || a.requests > 1;
   l.few_rows = !l.tiles ? 0x7fffffff : l.rows ? kFewRows : 0;
-  l.nt = most * per_kv <= 8 ? 1 : 2;
+  // Groups of 8 rows, or of 16.  Beside chunks the row kernel mostly has single tokens, and 16 rows take twice the work of 8 whether
+  // they are there or not (a chunk of 500 and 64 single tokens of 4 q heads a kv head: 64 us with 8, 70 with 16; a chunk of 200 and 24
+  // requests of 6 tokens, whose K and V 8 rows read three times: 80 and 73).
+  l.nt = (l.tiles ? per_kv : most * per_kv) <= 8 ? 1 : 2;
   l.row_ctas = sm_count();
   l.splits = 1;
   if (l.tiles) {
     const long long tokens = 2 * (128 / per_kv), ctas = (a.tokens + tokens - 1) / tokens * a.kv_heads;
-    while (l.splits < 16 && 2 * l.splits * ctas <= sm_count()) l.splits *= 2;
+    // As many CTAs as SMs; but every request may have a slot that turns out empty, and a thousand CTAs with nothing to do take longer
+    // than a long chunk in few pieces (18 single tokens that the caller has not said to be such: 43 us for 2300, 28 for 580).
+    const long long grid = (a.tokens / tokens + a.requests) * a.kv_heads;
+    while (l.splits < 16 && 2 * l.splits * ctas <= sm_count() && 2 * l.splits * grid <= 4 * sm_count()) l.splits *= 2;
   }
   l.joined = l.rows ? (l.row_ctas * sizeof(MergeRecord) + 255) / 256 * 256 : 0;
   l.tile_partial = l.joined + (l.rows ? 2 * l.row_ctas * part_floats(8 * l.nt) * sizeof(float) : 0);
