@@ -15,6 +15,9 @@
 // V rows behind a request's last position are cleared in shared memory (weight 0 times NaN is NaN); pieces whose sums are not
 // finite all the same are done again by exact_row.
 // Few CTAs (short chunks of long requests): every row tile's positions are cut into pieces, and a second kernel merges them.
+// 2048 tokens behind 6111, 32 q and 8 kv heads: 230 us in bf16 (1040 TFLOP/s), 256 in fp16, the products alone 172 (256 items take two turns of
+// 148 CTAs).  A pair of tiles takes 2.0 us, the products 1.1 of it, the exponentials as much; a CTA 10 us to begin and to end, which bounds
+// short walks (windows of 1024 over 7100 rows: 174 us).
 #include <cuda.h>
 
 #include "mk_chunk_attention.cuh"

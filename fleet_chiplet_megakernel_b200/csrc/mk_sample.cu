@@ -445,7 +445,8 @@ template <typename T> struct Sampler {
     const int t = threadIdx.x;
     __syncthreads();
     if (n_list <= kThreads / 8) {
-      // few: eight threads count how many of the others are larger than one of them (no two are equal but zeros)
+      // Few: eight threads count how many of the others are larger than one of them (no two are equal but zeros).  (top_k = 50: 14.7 us,
+      // 16.7 through the bins below.)
       const uint64_t mine = (t >> 3) < n_list ? s.list[t >> 3] : 0;
       int larger = 0;
       for (int j = t & 7; j < n_list; j += 8) larger += s.list[j] > mine;
