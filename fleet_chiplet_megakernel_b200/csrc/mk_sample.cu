@@ -16,12 +16,13 @@
 //          of these maxima gives the bound;
 //   top_p: a histogram of all logits near the largest, in bins of a factor exp(1/64) of the weight, and the sum of all weights in fp32 say
 //          to 1e-5 where the border is; the list tells whether a place in it lies that close to the border.
-// Where the list would be too long, or the border too close, the border is found step by step with sums in 64 bits: bins that the
-// border can be in, the weights above them, and again over the candidates' range of (logit, index), which a step divides by 1024;
-// the draw then reads the row once more.  CTAs hand each other sums by storing them into their neighbours' shared memory ahead of a
-// cluster barrier.  Rows that keep all tokens or thousands are bound by the instructions of the weights in 64 bits (some 40 a logit), the
-// others by the latency of the steps.  151936 fp32 logits, 1 and 64 rows: largest logit 5 and 9 us, all tokens 18 and 35, top_k = 50 15
-// and 22, top_p that keeps some thousands 44 and 87; the 64 rows take 6 us of the memory's time once.
+// Where the border is too close to call, all weights are summed in 64 bits and the list is looked at again.  Where the list would be too long, the
+// bins that the border can be in are listed in the pass that sums all weights and those above in 64 bits; where these are too many as well, the
+// border is found step by step: bins that it can be in, the weights above them, and again over the candidates' range of (logit, index),
+// which a step divides by 1024.  The draw then reads the row once more.  CTAs hand each other sums by storing them into their
+// neighbours' shared memory ahead of a cluster barrier.  Rows that keep all tokens or thousands are bound by the instructions of the weights in
+// 64 bits (some 25 a logit) and of the histograms, the others by the latency of the steps.  151936 fp32 logits, 1 and 64 rows: largest logit 5
+// and 9 us, all tokens 13 and 29, top_k = 50 14 and 21, top_p that keeps some thousands 37 and 79; the 64 rows take 6 us of the memory's time.
 #include <cooperative_groups.h>
 
 #include "mk_serving.cuh"
@@ -236,19 +237,20 @@ template <typename T> struct Sampler {
   }
   float per_bin;
   uint32_t count;         // of this thread's bin, over the cluster
+  uint32_t inner_count;   // how far into it they lie, summed
   double low_w, high_w;   // bounds of the mean weight in it
 
   // exp is convex: the mean weight in a bin is at least the weight at the mean depth and at most the chord's value there.  The depth is
   // known to 1 / kInner of a bin and to some units of 2^-24 relative.
-  __device__ __forceinline__ void mean_bounds(uint32_t inner, double per_unit) {
+  __device__ __forceinline__ void mean_bounds(uint32_t inner, float per_unit) {
     low_w = high_w = 0.0;
-    const double edge = exp(-(double)threadIdx.x / per_unit);
+    const float edge = expf(-(float)threadIdx.x / per_unit);  // (fp32 is off by some 1e-6 here)
     if (threadIdx.x == kBins - 1) {
-      high_w = edge * (1.0 + 1e-4);
+      high_w = (double)edge * (1.0 + 1e-4);
     } else if (count > 0) {
-      const double f = (double)inner / ((double)count * kInner);
-      low_w = edge * exp(-(f + 1.0 / kInner) / per_unit) * (1.0 - 1e-5);
-      high_w = edge * (1.0 - (1.0 - exp(-1.0 / per_unit)) * f) * (1.0 + 1e-5);
+      const float f = (float)inner / ((float)count * (float)kInner);
+      low_w = (double)(edge * expf(-(f + 1.f / kInner) / per_unit)) * (1.0 - 1e-5);
+      high_w = (double)(edge * (1.f - (1.f - expf(-1.f / per_unit)) * f)) * (1.0 + 1e-5);
     }
   }
   // Histogram of the linear bins; with `sum`, *mass: the sum of all weights.
@@ -270,7 +272,7 @@ template <typename T> struct Sampler {
       count += *peer(&s.hist[threadIdx.x], q);
       inner += *peer(&s.inner[threadIdx.x], q);
     }
-    mean_bounds(inner, kBinsPerUnit);
+    mean_bounds(inner, (float)kBinsPerUnit);
   }
 
   // The CTAs' lists (s.list, s.listed[2]) end to end at rank 0; returns how long it is (kCandidates + 1: longer than that).
@@ -373,26 +375,28 @@ template <typename T> struct Sampler {
     block_before((uint64_t)((int)threadIdx.x < bins ? n : 0), s.words, &in);
     *elements = (long long)in;
     count = (int)threadIdx.x < bins ? n : 0;
-    mean_bounds(inner, (double)kNearBins);
+    inner_count = inner;
     return bins;
   }
   // The border of top_p where the kept are too many for a list: from the bins of bins_of_mass those that it can be in, whose elements are
   // listed, in the pass that sums all weights and those above in 64 bits.  False: too many even so.
   __device__ bool near_border(double top_p, float unit, double mass, uint64_t* place) {
+    mean_bounds(inner_count, kNearBins);
     find_bins(true, top_p * mass, 0, 0, 0.0, 4.0 * (double)kSumError);
     const int first_bin = min(s.first_bin, s.last_bin), last_bin = s.last_bin;
     const uint64_t in = (int)threadIdx.x < first_bin ? (uint64_t)count : (int)threadIdx.x <= last_bin ? (uint64_t)count << 32 : 0;
     uint64_t both;
     block_before(in, s.words, &both);
     if ((both >> 32) > kCandidates) return false;
+    const float above = (float)first_bin, below = (float)(last_bin + 1);
     double sum = 0.0, ahead = 0.0;
     r.each([&](float l, int i) {
       const double w = r.weight(l);
       sum += w;
-      const int b = l == r.top ? 0 : (int)fminf((r.top - l) * unit, (float)(kBins - 1));
-      if (b < first_bin) {
+      const float d = fminf((r.top - l) * unit, (float)(kBins - 1));  // (NaN: both are infinite)
+      if (!(d >= above)) {
         ahead += w;
-      } else if (b <= last_bin) {
+      } else if (d < below) {
         const uint32_t at = atomicAdd(&s.listed[2], 1u);
         if (at < kCandidates) s.list[at] = place_of(l, i);
       }
@@ -441,7 +445,7 @@ template <typename T> struct Sampler {
   }
 
   // Sorts s.list[0 .. n), the largest first, zeros behind them.  The upper half of an entry: LOGITS: the key of a logit, else ~index.
-  template <bool LOGITS> static __device__ __noinline__ void sort_list(SampleShared& s, int n_list) {
+  template <bool LOGITS> static __device__ __noinline__ void sort_list(SampleShared& s, int n_list, int vocab) {
     const int t = threadIdx.x;
     __syncthreads();
     if (n_list <= kThreads / 8) {
@@ -475,10 +479,17 @@ template <typename T> struct Sampler {
     const uint32_t hi = s.range[0], lo = s.range[1];
     auto below = [&](uint32_t v) -> float { return LOGITS ? logit_of(hi) - logit_of(v) : (float)(hi - v); };
     const float per = (float)(kBins - 1) / below(lo);
+    // 16-bit logits that are next to each other: a bin is one value, or part of the indices of one.
+    constexpr int kZeros = sizeof(T) == 4 ? 0 : __is_same(T, __half) ? 13 : 16;  // low bits that all keys have in common
+    const uint32_t values = ((hi - lo) >> kZeros) + 1, parts = kBins / values;
+    const bool by_value = LOGITS && kZeros && values <= kBins / 2;
+    const float per_index = (float)parts / (float)vocab;
     int bin[2], at[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      bin[h] = min(kBins - 1, (int)(below(x[h] >> 32) * per));  // (does not fall; 0 where the range is not finite)
+      // (does not fall from one place to the next; 0 where the range is not finite)
+      bin[h] = by_value ? (int)(((hi - (uint32_t)(x[h] >> 32)) >> kZeros) * parts + min(parts - 1, (uint32_t)((float)(uint32_t)~(uint32_t)x[h] * per_index)))
+                        : min(kBins - 1, (int)(below(x[h] >> 32) * per));
       if (x[h]) at[h] = (int)atomicAdd(&s.hist[bin[h]], 1u);
     }
     __syncthreads();
@@ -572,10 +583,10 @@ template <typename T> struct Sampler {
   }
 
   // The draw from the sorted list alone (rank 0): it holds all that can be kept.  Without top_k, `mass` is the sum of all weights to
-  // kSumError; false where that leaves the border open.
-  __device__ bool draw(int n_list, bool by_k, int k, bool by_mass, double top_p, double mass, float min_p, double u, int64_t* token, float* logprob) {
+  // `error`, relative; false where that leaves the border open.
+  __device__ bool draw(int n_list, bool by_k, int k, bool by_mass, double top_p, double mass, double error, float min_p, double u, int64_t* token, float* logprob) {
     const int t = threadIdx.x;
-    sort_list<true>(s, n_list);
+    sort_list<true>(s, n_list, r.vocab);
     const uint64_t place[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
     bool keep[2], open = false;
     double w[2], before[2], total;
@@ -590,7 +601,7 @@ template <typename T> struct Sampler {
     for (int h = 0; h < 2; ++h) {
       const int at = t + h * kThreads;
       if (by_mass) {
-        const double limit = top_p * (by_k ? total : mass), slack = by_k ? 0.0 : (double)kSumError * limit;
+        const double limit = top_p * (by_k ? total : mass), slack = error * limit;
         open = open || (keep[h] && at > 0 && before[h] > limit - slack && before[h] < limit + slack);
         // (a list that ends below the limit does not hold the border)
         open = open || (!by_k && at == 0 && total < limit + slack && n_list < r.vocab);
@@ -605,7 +616,7 @@ template <typename T> struct Sampler {
     for (int h = 0; h < 2; ++h) s.list[t + h * kThreads] = keep[h] ? (place[h] & 0xffffffffu) << 32 | (uint32_t)(t + h * kThreads + 1) : 0;
     // (what is kept is the beginning of the sorted list)
     const int kept = __syncthreads_count(keep[0]) + (n_list > kThreads ? __syncthreads_count(keep[1]) : 0);
-    sort_list<false>(s, kept);
+    sort_list<false>(s, kept, r.vocab);
     const uint64_t by_index[2] = {t < kept ? s.list[t] : 0, t + kThreads < kept ? s.list[t + kThreads] : 0};
 #pragma unroll
     for (int h = 0; h < 2; ++h) w[h] = t + h * kThreads < kept ? s.weights[(uint32_t)by_index[h] - 1] : 0.0;
@@ -628,7 +639,7 @@ template <typename T> struct Sampler {
   // of the order are kept; by_mass: those before which less than `limit` lies, with by_k less than limit times the first k's weights.
   __device__ void cut(int n_list, bool by_k, long long k, bool by_mass, double limit, long long above, double mass) {
     const int t = threadIdx.x;
-    sort_list<true>(s, n_list);
+    sort_list<true>(s, n_list, r.vocab);
     const uint64_t place[2] = {t < n_list ? s.list[t] : 0, t + kThreads < n_list ? s.list[t + kThreads] : 0};
     if (t == 0) s.last_kept = 0;
     bool keep[2];
@@ -883,12 +894,22 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
       listed = near && elements <= kCandidates ? d.list_above([&](float l) { return l == r.top ? 0.f : fminf((r.top - l) * unit, (float)(kBins - 1)); }, unit, bins) : kCandidates + 1;
     }
     if (listed <= kCandidates) {
-      bool open = false;
-      if (rank == 0) open = !d.draw(listed, cut_k, top_k, cut_p, (double)top_p, mass, min_p, u, a.tokens + req, a.logprobs ? a.logprobs + req : nullptr);
-      if (cut_k) return;  // (no sum in fp32 is in it: the border is never open, and nobody looks into another CTA any more)
-      if (rank == 0 && (int)threadIdx.x < ranks) *d.peer(&s.close, threadIdx.x) = open;
-      cluster.sync();
-      if (!s.close) return;
+#pragma unroll 1
+      for (bool exact = cut_k;; exact = true) {
+        bool open = false;
+        if (rank == 0) open = !d.draw(listed, cut_k, top_k, cut_p, (double)top_p, mass, exact ? 0.0 : (double)kSumError, min_p, u, a.tokens + req, a.logprobs ? a.logprobs + req : nullptr);
+        if (cut_k) return;  // (no sum in fp32 is in it: the border is never open, and nobody looks into another CTA any more)
+        if (rank == 0 && (int)threadIdx.x < ranks) *d.peer(&s.close, threadIdx.x) = open;
+        cluster.sync();
+        if (!s.close) return;
+        if (exact) break;
+        // too close to call (a row in a few hundred): the sum of all weights in 64 bits
+        mass = 0.0;
+        r.each([&](float l, int) { mass += r.weight(l); });
+        d.give(mass);
+        cluster.sync();
+        mass = d.taken();
+      }
     }
     // the border by itself
     if (near && listed > kCandidates) done = d.near_border((double)top_p, near_unit, mass, &least);
@@ -912,151 +933,106 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
     }
   }
 
-  // the kept weights in the order of the index: a warp has a contiguous part of the CTA's
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int part = ((r.g1 - r.g0 + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int b0 = min(r.g1, r.g0 + warp * part), b1 = min(r.g1, b0 + part);
   // (min_p: bounds that are safely too low and too high; between them the weight itself decides)
   const float min_at = r.top + temperature * logf(fmaxf(min_p, 1e-45f)), min_off = (fabsf(r.top) + fabsf(min_at)) * 1e-6f + temperature * 1e-3f;
-  const float border_logit = least ? logit_of((uint32_t)(least >> 32)) : -INFINITY;
-  const float least_logit = fmaxf(border_logit, min_p > 0.f ? min_at - min_off : -INFINITY);
+  const uint32_t border_key = (uint32_t)(least >> 32);
+  const float border_logit = least ? logit_of(border_key) : -INFINITY;
+  const float nothing_below = __double2float_rd((double)r.top - 760.0 * (double)temperature);  // (exp(-746) is 0 in 64 bits)
+  const float least_logit = fmaxf(fmaxf(border_logit, nothing_below), min_p > 0.f ? min_at - min_off : -INFINITY);
   const bool never = isnan(r.plain) || (min_p > 0.f && !(min_at + min_off < INFINITY));
-  const float sure = never ? __uint_as_float(0x7fc00000u) : fmaxf(r.plain, min_p > 0.f ? min_at + min_off : -INFINITY);
+  // kept for certain from here on: above the border's logit
+  const float sure = never || border_logit == INFINITY ? __uint_as_float(0x7fc00000u)
+                                                       : fmaxf(least ? logit_of(border_key + 1) : -INFINITY, fmaxf(r.plain, min_p > 0.f ? min_at + min_off : -INFINITY));
   auto perhaps = [&](float l, int i) -> double {
     if (l < least_logit || (least != 0 && place_of(l, i) < least)) return 0.0;
     const double w = r.weight(l);
     return min_p > 0.f && w < (double)min_p ? 0.0 : w;
   };
-  auto kept_group = [&](int g, double (&w)[N]) -> double {  // and their sum, in order
+  auto kept_sum = [&](int g) -> double {  // of a group
     float l[N];
     uint32_t outside = 0, unsure = 0;
     if (r.inside(g)) r.load(g, l);
     else outside = r.load_edge(g, l);
+    double sum = 0.0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
-      const bool keep = l[e] >= sure && l[e] > border_logit;
-      w[e] = keep ? r.plain_weight(l[e]) : 0.0;
-      unsure |= keep || l[e] < least_logit ? 0u : 1u << e;
+      const double w = r.plain_weight(l[e]);
+      if (l[e] >= sure) sum += w;
+      else if (l[e] >= least_logit) unsure |= 1u << e;
     }
     unsure &= ~outside;
     while (unsure) {  // (at a border, or next to the smallest numbers)
-      const int k = __ffs(unsure) - 1, i = r.index(g) + k;
+      const int i = r.index(g) + __ffs(unsure) - 1;
       unsure &= unsure - 1;
-      const double x = perhaps(clean(to_float(r.logits[i])), i);
-#pragma unroll
-      for (int e = 0; e < N; ++e) w[e] = e == k ? x : w[e];
+      sum += perhaps(clean(to_float(r.logits[i])), i);
     }
-    double sum = 0.0;
-#pragma unroll
-    for (int e = 0; e < N; ++e) sum += w[e];
     return sum;
   };
-  double mine = 0.0;
-#pragma unroll 2
-  for (int g = b0 + lane; g < b1; g += 32) {
-    double w[N];
-    mine += kept_group(g, w);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kAll, mine, o);
-  __syncthreads();
-  if (lane == 0) s.sums[warp] = mine;
-  __syncthreads();
-  if ((int)threadIdx.x < ranks) {
-    double in_cta = 0.0;
-    for (int w = 0; w < kWarps; ++w) in_cta += s.sums[w];
-    *d.peer(&s.slot[d.turn & (kSlots - 1)][rank], threadIdx.x) = in_cta;
-  }
-  cluster.sync();  // the last time that a CTA touches another
-  // the first CTA whose sum exceeds the goal has the token, and of its warps the first; where rounding leaves none, the last that keeps any
-  const double* in_rank = s.slot[d.turn & (kSlots - 1)];
-  double total = 0.0;
-  for (int q = 0; q < ranks; ++q) total += in_rank[q];
-  const double goal = u * total;
-  double end = 0.0, before = 0.0;
-  int owner = -1;
-  for (int q = 0; q < ranks; ++q) {
-    const double m = in_rank[q];
-    if (m > 0.0 && (owner < 0 || goal >= end)) {
-      owner = q;
-      before = end;
-    }
-    end += m;
-  }
-  if (rank != owner) return;
-  double from = before;
-  end = before;
-  owner = -1;
-  for (int w = 0; w < kWarps; ++w) {
-    const double m = s.sums[w];
-    if (m > 0.0 && (owner < 0 || goal >= end)) {
-      owner = w;
-      from = end;
-    }
-    end += m;
-  }
-  // That warp's part again, dealt out to all warps: its sums say which of them has the token.
-  const int o0 = min(r.g1, r.g0 + owner * part), o1 = min(r.g1, o0 + part), share = ((o1 - o0 + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int p0 = min(o1, o0 + warp * share), p1 = min(o1, p0 + share);
-  mine = 0.0;
-  for (int g = p0 + lane; g < p1; g += 32) {
-    double w[N];
-    mine += kept_group(g, w);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kAll, mine, o);
-  if (lane == 0) s.weights[warp] = mine;
-  __syncthreads();
-  end = from;
-  owner = -1;
-  for (int w = 0; w < kWarps; ++w) {
-    const double m = s.weights[w];
-    if (m > 0.0 && (owner < 0 || goal >= end)) {
-      owner = w;
-      from = end;
-    }
-    end += m;
-  }
-  if (warp != owner) return;
-  int token = -1;
-  double w_token = 0.0, run = from;
-  for (int i0 = p0; i0 < p1; i0 += 32) {
-    double w[N] = {};
-    const double sum = i0 + lane < p1 ? kept_group(i0 + lane, w) : 0.0;
-    double up = sum;
+  // The kept weights in the order of the index: a warp has a contiguous part of the CTA's.  The CTA in which the running sum exceeds the
+  // goal deals that part out to its warps again, until a lane has one group.  (One loop, so that its instructions are fetched once.)
+  double goal = 0.0, total = 0.0, from = 0.0, mine, up;
+  int lo = r.g0, hi = r.g1, owner;
+  // the first of 32 values whose running sum exceeds the goal; where rounding leaves none, the last that is not 0; -1: all are
+  auto find = [&](double v) -> int {
+    up = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const double x = __shfl_up_sync(kAll, up, o);
       if (lane >= o) up += x;
     }
-    const unsigned over = __ballot_sync(kAll, sum > 0.0 && run + up > goal), any = __ballot_sync(kAll, sum > 0.0);
-    if (any) {
-      const int k = over ? __ffs(over) - 1 : 31 - __clz(any);
-      double at = __shfl_up_sync(kAll, up, 1);
-      at = run + (lane == 0 ? 0.0 : at);
-      // of that lane's elements the first that exceeds, else its last that is kept
-      int pick = -1;
-      double w_pick = 0.0;
-      bool done = false;
+    const unsigned over = __ballot_sync(kAll, v > 0.0 && from + up > goal), any = __ballot_sync(kAll, v > 0.0);
+    const int k = over ? __ffs(over) - 1 : 31 - __clz(any);
+    const double ahead = __shfl_sync(kAll, up, max(k - 1, 0));
+    if (k > 0) from += ahead;
+    return k;
+  };
+#pragma unroll 1
+  for (bool first = true;; first = false) {
+    const int part = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
+    const int b0 = min(hi, lo + warp * part), b1 = min(hi, b0 + part);
+    mine = 0.0;
+#pragma unroll 2
+    for (int g = b0 + lane; g < b1; g += 32) mine += kept_sum(g);
+    double sum = mine;
 #pragma unroll
-      for (int e = 0; e < N; ++e) {
-        if (w[e] > 0.0 && !done) {
-          pick = e;
-          w_pick = w[e];
-        }
-        at += w[e];
-        done = done || (w[e] > 0.0 && at > goal);
-      }
-      token = r.index(i0 + k) + __shfl_sync(kAll, pick, k);
-      w_token = __shfl_sync(kAll, w_pick, k);
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
+    __syncthreads();
+    if (lane == 0) s.sums[warp] = sum;
+    __syncthreads();
+    if (first) {
+      const double* in_rank = s.slot[d.turn & (kSlots - 1)];
+      double in_cta = s.sums[lane];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) in_cta += __shfl_xor_sync(kAll, in_cta, o);
+      if ((int)threadIdx.x < ranks) *d.peer(&s.slot[d.turn & (kSlots - 1)][rank], threadIdx.x) = in_cta;
+      cluster.sync();  // the last time that a CTA touches another
+      for (int q = 0; q < ranks; ++q) total += in_rank[q];
+      goal = u * total;
+      if (rank != find(lane < ranks ? in_rank[lane] : 0.0)) return;
     }
-    if (over) break;
-    run += __shfl_sync(kAll, up, 31);
+    owner = find(s.sums[lane]);
+    if (part <= 32) break;
+    lo = min(hi, lo + owner * part);
+    hi = min(hi, lo + part);
   }
-  if (lane == 0) {
-    a.tokens[req] = token;
-    if (a.logprobs) a.logprobs[req] = (float)log(w_token / total);
+  if (warp != owner) return;
+  const int part = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32, k = find(mine);
+  if (lane != k) return;
+  const int i0 = r.index(min(hi, lo + warp * part) + lane);
+  int token = -1;
+  double w_token = 0.0;
+#pragma unroll 1
+  for (int i = max(i0, 0); i < min(i0 + N, r.vocab); ++i) {
+    const double w = perhaps(clean(to_float(r.logits[i])), i);
+    if (!(w > 0.0)) continue;
+    token = i;
+    w_token = w;
+    from += w;
+    if (from > goal) break;
   }
+  a.tokens[req] = token;
+  if (a.logprobs) a.logprobs[req] = (float)log(w_token / total);
 }
 
 template <typename T> cudaError_t launch(const mk_sample_args& a, cudaStream_t s) {

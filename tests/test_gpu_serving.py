@@ -579,6 +579,20 @@ def test_sample_rows_that_keep_thousands(temperature, top_p, top_k, vocab, dtype
     check_sample(logits, torch.rand(4, generator=g, device="cuda"), temperature, top_k, top_p, 0.0)
 
 
+@pytest.mark.parametrize("dtype", [BF, FP, torch.float32])
+@pytest.mark.parametrize("vocab", [900, 20000, 151936])
+@pytest.mark.parametrize("rest", [-30.0, -20.0, -math.inf])
+def test_sample_borders_that_are_too_close_for_32_bits(rest, vocab, dtype):
+    """Eight equal weights and a rest that is 1e-13 to 3e-4 of them: the weights before the third, or the fifth, are the limit but for that."""
+    g = gen(vocab)
+    for top_p in (0.25, 0.5):
+        logits = torch.full((16, vocab), rest, device="cuda")
+        for r in range(16):
+            logits[r, torch.randperm(vocab, generator=g, device="cuda")[:8]] = 3.0
+        u = torch.arange(16, device="cuda") / 16 + 1 / 32
+        check_sample(logits.to(dtype), u, 1.0, 0, top_p, 0.0)
+
+
 def test_sample_of_the_last_rows_of_requests():
     g = gen(1)
     logits, u = rnd(g, 9, 5000, dtype=torch.float32, scale=2.0)[:, 7:4007], torch.rand(5, generator=g, device="cuda")
