@@ -22,7 +22,7 @@
 // which a step divides by 1024.  The draw then reads the row once more.  CTAs hand each other sums by storing them into their
 // neighbours' shared memory ahead of a cluster barrier.  Rows that keep all tokens or thousands are bound by the instructions of the weights in
 // 64 bits (some 25 a logit) and of the histograms, the others by the latency of the steps.  151936 fp32 logits, 1 and 64 rows: largest logit 5
-// and 9 us, all tokens 13 and 29, top_k = 50 14 and 21, top_p that keeps some thousands 37 and 79; the 64 rows take 6 us of the memory's time.
+// and 8 us, all tokens 13 and 28, top_k = 50 14 and 21, top_p that keeps some thousands 37 and 75; the 64 rows take 6 us of the memory's time.
 #include <cooperative_groups.h>
 
 #include "mk_serving.cuh"
@@ -81,7 +81,7 @@ template <typename T> struct Row {
   int g0, g1;         // this CTA's groups
   float top;
   double scale;       // 64 log2(e) / temperature
-  double top_scaled;  // top * scale
+  double largest;     // top
   const double* power;
 
   __device__ __forceinline__ int index(int g) const { return g * N - shift; }
@@ -113,23 +113,24 @@ template <typename T> struct Row {
     }
     return outside;
   }
+  float lowest;       // below this logit a weight is 0
   float plain;        // from this logit on a weight needs no care: it is a normal number, and neither infinity nor NaN is in its way
-  // exp((l - top) / temperature): the argument y in units of ln 2 / 64, its whole part by table (P. T. P. Tang's method, 1989), the rest
+  // exp((l - top) / temperature), exactly 1 for the largest: the argument y in units of ln 2 / 64, its whole part by table (P. T. P. Tang's method, 1989), the rest
   // r (|r| <= 1/2) by the series up to the fourth power; the next term is 4e-14.
   __device__ __forceinline__ double plain_weight(float l) const {
     constexpr double kRound = 6755399441055744.0;  // 1.5 2^52: a sum with it is rounded to a whole number
     constexpr double c1 = 0.6931471805599453094 / 64.0, c2 = c1 * c1 / 2.0, c3 = c2 * c1 / 3.0, c4 = c3 * c1 / 4.0;
-    const double y = fma((double)l, scale, -top_scaled), big = y + kRound;
+    const double y = ((double)l - largest) * scale, big = y + kRound;
     const int n = __double2loint(big);
     const double r = y - (big - kRound);
     const double t = power[n & 63];
     const double e = fma(t * r, fma(r, fma(r, fma(r, c4, c3), c2), c1), t);
     return __hiloint2double(__double2hiint(e) + ((n >> 6) << 20), __double2loint(e));
   }
-  // (exactly 1 for the largest: it may not fall below min_p = 1)
-  __device__ __forceinline__ double weight(float l) const { return l == top ? 1.0 : l >= plain ? plain_weight(l) : far_weight(l, top, scale); }
+  __device__ __forceinline__ double weight(float l) const { return l >= plain ? plain_weight(l) : far_weight(l, top, scale); }
   // next to the smallest numbers, and where infinities meet
   static __device__ __noinline__ double far_weight(float l, float top, double scale) {
+    if (l == top) return 1.0;  // (both may be infinite)
     const double y = ((double)l - (double)top) * scale;
     return l == -INFINITY || isnan(y) ? 0.0 : exp(y * (0.6931471805599453094 / 64.0));
   }
@@ -174,6 +175,27 @@ template <typename T> struct Row {
     });
   }
 };
+
+// f(weight, logit, index) for all elements whose weight is not 0: those that are plain without a branch, so that the weights of a group are
+// worked out side by side.
+template <typename T, typename F> __device__ __forceinline__ void each_weight(const Row<T>& r, const F& f) {
+  constexpr int N = Row<T>::N;
+  r.each_group([&](const float (&l)[N], int n, int i) {
+    uint32_t unsure = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const double w = r.plain_weight(l[e]);
+      if (e < n && l[e] >= r.plain) f(w, l[e], i + e);
+      else if (e < n && l[e] >= r.lowest) unsure |= 1u << e;
+    }
+    while (unsure) {
+      const int k = __ffs(unsure) - 1;
+      unsure &= unsure - 1;
+      const float x = clean(to_float(r.logits[i + k]));
+      f(r.weight(x), x, i + k);
+    }
+  });
+}
 
 // Sum over the block in a fixed order; thread 0 to kMaxCluster - 1 get it (and all others).
 __device__ __forceinline__ double block_sum(double v, SampleShared& s) {
@@ -391,8 +413,7 @@ template <typename T> struct Sampler {
     if ((both >> 32) > kCandidates) return false;
     const float above = (float)first_bin, below = (float)(last_bin + 1);
     double sum = 0.0, ahead = 0.0;
-    r.each([&](float l, int i) {
-      const double w = r.weight(l);
+    each_weight(r, [&](double w, float l, int i) {
       sum += w;
       const float d = fminf((r.top - l) * unit, (float)(kBins - 1));  // (NaN: both are infinite)
       if (!(d >= above)) {
@@ -880,9 +901,10 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
   }
   const double inv_t = 1.0 / (double)temperature;
   r.scale = inv_t * (64.0 / 0.6931471805599453094);
-  r.top_scaled = (double)r.top * r.scale;
+  r.largest = (double)r.top;
   // (rounded up; exp(-700) is 1e-304.  With an infinite largest logit or temperature no logit, or every finite one, is plain.)
   r.plain = r.top == INFINITY ? __uint_as_float(0x7fc00000u) : fmaxf(__double2float_ru((double)r.top - 700.0 * (double)temperature), -3.4028235e38f);
+  r.lowest = fmaxf(__double2float_rd((double)r.top - 760.0 * (double)temperature), -INFINITY);  // (exp(-746) is 0 in 64 bits)
   d.per_bin = (float)(kBinsPerUnit * inv_t);
 
   uint64_t least = 0;  // the border: places from here on are kept
@@ -915,7 +937,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
         if (exact) break;
         // too close to call (a row in a few hundred): the sum of all weights in 64 bits
         mass = 0.0;
-        r.each([&](float l, int) { mass += r.weight(l); });
+        each_weight(r, [&](double w, float, int) { mass += w; });
         d.give(mass);
         cluster.sync();
         mass = d.taken();
@@ -948,8 +970,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
   const float min_at = r.top + temperature * logf(fmaxf(min_p, 1e-45f)), min_off = (fabsf(r.top) + fabsf(min_at)) * 1e-6f + temperature * 1e-3f;
   const uint32_t border_key = (uint32_t)(least >> 32);
   const float border_logit = least ? logit_of(border_key) : -INFINITY;
-  const float nothing_below = __double2float_rd((double)r.top - 760.0 * (double)temperature);  // (exp(-746) is 0 in 64 bits)
-  const float least_logit = fmaxf(fmaxf(border_logit, nothing_below), min_p > 0.f ? min_at - min_off : -INFINITY);
+  const float least_logit = fmaxf(fmaxf(border_logit, r.lowest), min_p > 0.f ? min_at - min_off : -INFINITY);
   const bool never = isnan(r.plain) || (min_p > 0.f && !(min_at + min_off < INFINITY));
   // kept for certain from here on: above the border's logit
   const float sure = never || border_logit == INFINITY ? __uint_as_float(0x7fc00000u)
