@@ -373,6 +373,14 @@ def test_attention_of_chunks(requests, n_q, n_kv, page, dtype):
     Batch(requests, n_q, n_kv, page, dtype, pad=3).check()
 
 
+@pytest.mark.parametrize("count", [31, 32, 33, 70])
+def test_attention_of_many_chunks(count):
+    """Requests of equal and of different lengths, empty ones and single tokens among them."""
+    requests = [((13 * (i // 3)) % 200, (0, 1, 9, 33, 40, 90)[(5 * i) % 6 if i % 4 else i % 6]) for i in range(count)]
+    Batch(requests, 8, 2, 16, pad=3).check()
+    Batch(requests[::-1], 4, 4, 8, dtype=FP).check(window=40, sinks=3)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 0), (17, 4), (128, 4), (200, 130), (64, 1000), (5000, 3), (2 ** 31 - 1, 2 ** 31 - 1)])
 @pytest.mark.parametrize("requests", [[(700, 1), (0, 1), (15, 1), (129, 1)], [(0, 300), (500, 140), (90, 1)]])
 def test_attention_with_window_and_sinks(requests, window, sinks):
