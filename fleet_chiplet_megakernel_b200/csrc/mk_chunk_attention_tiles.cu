@@ -241,11 +241,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
           load_box3(sq + i * kStageBytes + h * kHalfBytes, &tp.q, q_full, 64 * h, kv_head * p.per_kv, q.q0 + t0 + i * tp.tokens_per_tile);
     }
   }
-  fence_before();
-  __syncthreads();
-  fence_after();
-  uint32_t tm;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tm) : "r"(tm_slot));
+  // The loads wait for nobody: their warp has set the barriers up, and tensor memory they do not use.
+  uint32_t tm = 0;
+  if (warp == kLoadWarp) {
+    asm volatile("barrier.cta.arrive 1, %0;" ::"n"(kTileThreads) : "memory");
+  } else {
+    fence_before();
+    asm volatile("barrier.cta.sync 1, %0;" ::"n"(kTileThreads) : "memory");
+    fence_after();
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tm) : "r"(tm_slot));
+  }
   const uint32_t tm_o = tm + 256;
 
   if (n > 0 && warp == kLoadWarp) {

@@ -30,10 +30,6 @@ template <typename T> struct Raw {
       for (int i = 0; i < 8; ++i) e[i] = p[i];
     }
   }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int k = 0; k < (int)sizeof(T) / 2; ++k) w[k] = make_uint4(0, 0, 0, 0);
-  }
   __device__ __forceinline__ void get(uint64_t (&f)[4]) const {  // as pairs of fp32
 #pragma unroll
     for (int k = 0; k < (int)sizeof(T) / 2; ++k) {

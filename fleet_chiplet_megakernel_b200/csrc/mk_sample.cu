@@ -25,6 +25,8 @@
 // and 8 us, all tokens 13 and 28, top_k = 50 14 and 21, top_p that keeps some thousands 37 and 75; the 64 rows take 6 us of the memory's time.
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "mk_serving.cuh"
 
 namespace cg = cooperative_groups;
@@ -1077,7 +1079,7 @@ template <typename T> cudaError_t launch(const mk_sample_args& a, cudaStream_t s
   cfg.numAttrs = 1;
   // The widest cluster of which the device runs as many at once as there are rows.  (A cluster lies within a group of SMs: 16 rows on
   // clusters of 8, which take 128 of 148 SMs, need two turns: top_k = 50 of 151936 fp32 logits 30 us, 20 on clusters of 4.)
-  static int at_once[64][4] = {};
+  static std::atomic<int> at_once[64][4] = {};
   int dev = 0, ranks = kMaxCluster;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) ranks = 1;
   for (int k = 3; ranks > 1; ranks >>= 1, --k) {
@@ -1086,7 +1088,10 @@ template <typename T> cudaError_t launch(const mk_sample_args& a, cudaStream_t s
     attr[0].val.clusterDim.x = (unsigned)ranks;
     if (at_once[dev][k] == 0) {
       int n = 0;
-      if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<T>, &cfg) != cudaSuccess) n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, sample_kernel<T>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        continue;
+      }
       at_once[dev][k] = n > 0 ? n : -1;
     }
     if (a.requests <= at_once[dev][k]) break;

@@ -6,6 +6,8 @@
 // every CTA works out all the sums for itself in shared memory and then takes its share of the lookups: one launch, no
 // CTA waits for another, no atomics.  What is read and written is about 8 bytes a page and 12 a token; bound by latency:
 // 8 requests 5 us, 512 of up to 8000 tokens on pages of 16, with prompt chunks among them, 7 us.
+#include <atomic>
+
 #include "mk_serving.cuh"
 
 namespace mk_serving {
@@ -177,11 +179,14 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
 }  // namespace
 
 int sm_count() {
-  static int count[64] = {};
-  int dev = 0;
+  static std::atomic<int> count[64] = {};
+  int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  if (count[dev] == 0 && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
-  return count[dev];
+  if ((n = count[dev]) == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    count[dev] = n;
+  }
+  return n;
 }
 char* error_text() {
   static thread_local char text[kErrorBytes];
