@@ -467,6 +467,46 @@ def test_attention_of_strided_tensors():
         b.check()
 
 
+def far_apart(shape, dtype=BF):
+    """Two caches whose pages are 2^30 elements apart, one between the other's."""
+    pages, rest = shape[0], shape[1] * shape[2] * shape[3]
+    pool = torch.empty((pages - 1) * 2 ** 30 + 2 ** 29 + rest, dtype=dtype, device="cuda")
+    stride = (2 ** 30, shape[2] * shape[3], shape[3], 1)
+    return pool.as_strided(shape, stride), pool.as_strided(shape, stride, 2 ** 29)
+
+
+@pytest.mark.parametrize("requests", [[(200, 1), (17, 1)], [(130, 80), (17, 1)]])
+def test_attention_over_a_cache_past_32_bits(requests):
+    b = Batch(requests, 8, 2, 64)
+    k, v = far_apart(b.k.shape)
+    b.k, b.v = k.copy_(b.k), v.copy_(b.v)
+    b.check()
+
+
+def test_rotate_append_into_a_cache_past_32_bits():
+    g = gen(1)
+    kc, vc = far_apart((6, 16, 2, D))
+    kc.zero_(), vc.zero_()
+    x, cos, sin = rnd(g, 40, 8, D), torch.ones(40, D, device="cuda"), torch.zeros(40, D, device="cuda")
+    slots = torch.randperm(96, generator=g, device="cuda")[:40]
+    out = mk.rotate_append(x[:, :4], x[:, 4:6], x[:, 6:], cos, sin, torch.arange(40, device="cuda", dtype=torch.int32), slots, kc, vc)
+    assert torch.equal(out, x[:, :4])  # (no rotation, no norm: as they were)
+    for cache, rows in ((kc, x[:, 4:6]), (vc, x[:, 6:])):
+        want = torch.zeros(96, 2, D, dtype=BF, device="cuda")
+        want[slots] = rows
+        assert torch.equal(cache.reshape(96, 2, D), want)
+
+
+def test_sample_from_rows_past_32_bits():
+    g = gen(2)
+    near = rnd(g, 6, 5000, scale=2.0)
+    pool = torch.empty(5 * 2 ** 30 + 5000, dtype=BF, device="cuda")
+    logits = pool.as_strided((6, 5000), (2 ** 30, 1)).copy_(near)
+    u = torch.rand(6, generator=g, device="cuda")
+    for kw in ({}, {"top_k": 40}, {"top_p": 0.9}):
+        assert torch.equal(mk.sample_tokens(logits, u, **kw), mk.sample_tokens(near, u, **kw))
+
+
 def test_attention_is_the_same_each_time():
     for requests in ([(2000, 1)] * 3, [(700, 200), (9, 1)]):
         b = Batch(requests, 8, 2, 64)
