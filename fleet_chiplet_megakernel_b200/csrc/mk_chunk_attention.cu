@@ -607,7 +607,7 @@ template <typename T, int NT, int RING> int launch_rows(const AttnParams& p, boo
   if constexpr (RING > 2) {
     if (smem > kMostSmem) return launch_rows<T, NT, RING - 1>(p, behind_tiles, s);  // (some hundreds of requests)
   }
-  cudaError_t e = cudaFuncSetAttribute(chunk_attention_rows<T, NT, RING>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  cudaError_t e = allow_shared<chunk_attention_rows<T, NT, RING>>(kMostSmem);
   if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: %s", cudaGetErrorString(e));
   if (behind_tiles) {  // (the two write different rows; the kernel ahead of the tile kernel is done when that one begins)
     e = launch_after((const void*)chunk_attention_rows<T, NT, RING>, dim3(p.row_ctas), kRowThreads, smem, p, s);

@@ -629,7 +629,7 @@ bool encode(CUtensorMap* map, int dtype, int dims, const void* ptr, const cuuint
 
 template <typename T> int launch(const TileParams& tp, cudaStream_t s) {
   const AttnParams& p = tp.p;
-  cudaError_t e = cudaFuncSetAttribute(chunk_attention_tiles<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  cudaError_t e = allow_shared<chunk_attention_tiles<T>>(kSmemBytes);
   if (e != cudaSuccess) return fail(MK_E_CUDA, "chunk_attention: %s", cudaGetErrorString(e));
   const long long slots = p.a.tokens / (2 * tp.tokens_per_tile) + p.a.requests;
   chunk_attention_tiles<T><<<(unsigned)(slots * p.a.kv_heads * p.splits), kTileThreads, kSmemBytes, s>>>(tp);

@@ -25,8 +25,6 @@
 // and 8 us, all tokens 13 and 28, top_k = 50 14 and 21, top_p that keeps some thousands 37 and 75; the 64 rows take 6 us of the memory's time.
 #include <cooperative_groups.h>
 
-#include <atomic>
-
 #include "mk_serving.cuh"
 
 namespace cg = cooperative_groups;

@@ -9,6 +9,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "../../include/b200mk.h"
 
 namespace mk_serving {
@@ -29,6 +31,16 @@ inline int fail(int code, const char* fmt, ...) noexcept {
 inline int launched(const char* what) noexcept {
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "%s: launch failed: %s", what, cudaGetErrorString(e));
+}
+// Lets a kernel have so much dynamic shared memory on the current device, once (a call of the driver takes a microsecond).
+template <auto kernel> cudaError_t allow_shared(int bytes) noexcept {
+  static std::atomic<bool> done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
 }
 // Multiprocessors of the current device (the value of a device does not change).
 int sm_count();

@@ -6,8 +6,6 @@
 // every CTA works out all the sums for itself in shared memory and then takes its share of the lookups: one launch, no
 // CTA waits for another, no atomics.  What is read and written is about 8 bytes a page and 12 a token; bound by latency:
 // 8 requests 5 us, 512 of up to 8000 tokens on pages of 16, with prompt chunks among them, 7 us.
-#include <atomic>
-
 #include "mk_serving.cuh"
 
 namespace mk_serving {
@@ -240,7 +238,7 @@ extern "C" int mk_plan_step(const mk_step_plan_args* args, void* stream) {
     }
   const size_t smem = 4 * (n + 1) * sizeof(int);
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(step_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_shared<step_plan_kernel>(4 * (MK_STEP_MAX_REQUESTS + 1) * (int)sizeof(int));
     if (e != cudaSuccess) return fail(MK_E_CUDA, "plan_step: %s", cudaGetErrorString(e));
   }
   const long long entries = (long long)a.max_indices + a.max_tokens;
