@@ -249,11 +249,18 @@ class MPK:
 
     def sample_tokens(self, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, return_logprobs: bool = False):
         """A token per request from the logits of its last row in the pass before (``serving.sample_tokens``); -1 for requests that
-        were fed nothing.  Needs ``MPKMetadata.logits``."""
+        were fed nothing.  Needs ``MPKMetadata.logits`` and an LM head that is whole on every rank: of a head that is cut by vocabulary
+        rows a rank's logits are its slice, from which no token of the whole can be drawn."""
         if self.metadata.logits is None:
             raise ValueError("sample_tokens needs MPKMetadata.logits")
         if self.metadata.mode == "offline":
             raise ValueError("mode 'offline' takes the largest logit itself; use 'online_notoken'")
+        if not self.with_lm_head:
+            raise ValueError("sample_tokens needs MirageModelConfig.with_lm_head: without it no pass fills MPKMetadata.logits")
+        rows, vocab = self.metadata.logits.shape[-1], self.model_config.vocab_size
+        if self.world_size > 1 and rows != vocab:
+            raise NotImplementedError(f"sample_tokens: this rank's logits are {rows} of {vocab} rows of a sharded LM head; keep it whole "
+                                      "(shard_qwen3_weights with shard_lm_head=False), or gather the logits and call serving.sample_tokens")
         return sample_tokens(self.metadata.logits, u, temperature, top_k, top_p, min_p, qo_indptr=self.qo_indptr_buffer, return_logprobs=return_logprobs)
 
     def finalize(self):
