@@ -37,11 +37,19 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kBins = kThreads;      // one a thread
 constexpr int kCandidates = 2 * kThreads;  // sorted at once, two a thread
 constexpr int kMaxCluster = 8;
-constexpr int kInner = 1024;         // (2^32 / 1024 elements a CTA)
+constexpr int kInner = 1024;         // parts of a bin, at most (inner_parts())
 constexpr double kBinsPerUnit = 32.0;
 constexpr int kSlots = 4;
 constexpr float kNearBins = 64.f;    // bins a unit of (largest logit - logit) / temperature, near the largest
 constexpr float kTopBins = 16.f;     // bins a unit of (largest logit - logit) for the bound of the k-th
+// In how many parts a bin is divided for the sums of how far into it its logits lie: so many that all logits of the row in one bin, over the
+// whole cluster, stay below 2^32.  1024 up to a vocabulary of 2^22, 4 at the largest.
+__host__ __device__ constexpr int inner_parts(int vocab) {
+  int n = kInner;
+  while ((long long)n * vocab > 1ll << 32) n >>= 1;
+  return n;
+}
+static_assert(inner_parts(1 << 22) == kInner && inner_parts(0x3fffffff) == 4, "a largest sum is vocab * (parts - 1)");
 constexpr float kSumError = 1e-5f;   // relative, of a sum of weights in fp32: the argument of exp is off by 2^-22 of itself, at most 23 where weights count
 
 // Larger logits are larger keys; -0 and +0 are equal, NaN counts as minus infinity.
@@ -56,7 +64,7 @@ __device__ __forceinline__ uint64_t place_of(float l, int i) { return ((uint64_t
 
 struct SampleShared {
   uint32_t hist[kBins];
-  uint32_t inner[kBins];            // of linear bins: how far into the bin its logits lie, summed, in units of 1 / kInner
+  uint32_t inner[kBins];            // of linear bins: how far into the bin its logits lie, summed, in units of 1 / inner_parts()
   uint64_t list[kCandidates];       // rank 0's is used
   double weights[kCandidates];      // of the list's
   double power[64];                 // 2^(i / 64)
@@ -258,20 +266,21 @@ template <typename T> struct Sampler {
     return fminf((r.top - l) * per_bin, (float)(kBins - 1));  // (infinite differences too)
   }
   float per_bin;
+  float parts;            // inner_parts()
   uint32_t count;         // of this thread's bin, over the cluster
   uint32_t inner_count;   // how far into it they lie, summed
   double low_w, high_w;   // bounds of the mean weight in it
 
   // exp is convex: the mean weight in a bin is at least the weight at the mean depth and at most the chord's value there.  The depth is
-  // known to 1 / kInner of a bin and to some units of 2^-24 relative.
+  // known to 1 / parts of a bin and to some units of 2^-24 relative.
   __device__ __forceinline__ void mean_bounds(uint32_t inner, float per_unit) {
     low_w = high_w = 0.0;
     const float edge = expf(-(float)threadIdx.x / per_unit);  // (fp32 is off by some 1e-6 here)
     if (threadIdx.x == kBins - 1) {
       high_w = (double)edge * (1.0 + 1e-4);
     } else if (count > 0) {
-      const float f = (float)inner / ((float)count * (float)kInner);
-      low_w = (double)(edge * expf(-(f + 1.f / kInner) / per_unit)) * (1.0 - 1e-5);
+      const float f = (float)inner / ((float)count * parts);
+      low_w = (double)(edge * expf(-(f + 1.f / parts) / per_unit)) * (1.0 - 1e-5);
       high_w = (double)(edge * (1.f - (1.f - expf(-1.f / per_unit)) * f)) * (1.0 + 1e-5);
     }
   }
@@ -282,7 +291,7 @@ template <typename T> struct Sampler {
       const float d = depth(l);
       const int b = (int)d;
       atomicAdd(&s.hist[b], 1u);
-      if (b < kBins - 1) atomicAdd(&s.inner[b], (uint32_t)((d - (float)b) * (float)kInner));
+      if (b < kBins - 1) atomicAdd(&s.inner[b], (uint32_t)((d - (float)b) * parts));
       if (sum) w += r.weight(l);
     });
     if (sum) give(w);
@@ -366,7 +375,7 @@ template <typename T> struct Sampler {
           if (d < (float)(kBins - 1)) {
             const int b = (int)d;
             atomicAdd(&s.hist[b], 1u);
-            atomicAdd(&s.inner[b], (uint32_t)((d - (float)b) * (float)kInner));
+            atomicAdd(&s.inner[b], (uint32_t)((d - (float)b) * parts));
           }
         }
       }
@@ -906,6 +915,7 @@ template <typename T> __global__ void __launch_bounds__(kThreads, 1) sample_kern
   r.plain = r.top == INFINITY ? __uint_as_float(0x7fc00000u) : fmaxf(__double2float_ru((double)r.top - 700.0 * (double)temperature), -3.4028235e38f);
   r.lowest = fmaxf(__double2float_rd((double)r.top - 760.0 * (double)temperature), -INFINITY);  // (exp(-746) is 0 in 64 bits)
   d.per_bin = (float)(kBinsPerUnit * inv_t);
+  d.parts = (float)inner_parts(a.vocab);
 
   uint64_t least = 0;  // the border: places from here on are kept
   const bool cut_k = top_k > 0 && top_k < a.vocab, cut_p = top_p < 1.f;

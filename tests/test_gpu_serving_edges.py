@@ -1,0 +1,25 @@
+"""The serving operators at the edges of what their documentation allows: calls without rows or pages, vocabularies of millions, weights that a
+16-bit type has no value for, positions next to 2^31, tangents, tensors that share memory, waits that run out."""
+import math
+
+import pytest
+import torch
+
+import fleet_chiplet_megakernel_b200 as mk
+from tests.test_gpu_serving import Batch, check_sample, gen, i32, rnd
+
+pytestmark = pytest.mark.gpu
+BF, FP = torch.bfloat16, torch.float16
+D = 128
+
+
+@pytest.mark.parametrize("top_p", [0.3, 0.513, 0.9])
+def test_sample_from_a_vocabulary_of_millions(top_p):
+    """Twelve million logits of two values that are next to each other, and one above them: what is summed over a bin of the histograms does not
+    fit 32 bits in units of 1 / 1024 of a bin."""
+    logits = torch.full((1, 12_000_001), -0.0615, device="cuda")
+    logits[0, 1::2] = -0.0305
+    logits[0, 7_654_320] = 0.0
+    u = torch.tensor([0.0, 0.37, 0.86, 1 - 2.0 ** -24], device="cuda")
+    check_sample(logits.expand(4, -1), u, 1.0, 0, top_p, 0.0)
+    check_sample(logits.expand(4, -1), u, 1.0, 7_000_000, top_p, 0.0)
