@@ -658,8 +658,8 @@ Layout layout_of(const mk_chunk_attention_args& a) {
 }
 
 int check(const mk_chunk_attention_args& a) {
-  if (!a.q || !a.k_cache || !a.v_cache || !a.qo_indptr || !a.kv_indptr || !a.kv_indices || !a.last_page_len || !a.out)
-    return fail(MK_E_INVALID, "chunk_attention: null pointer");
+  if (!a.q || !a.k_cache || !a.v_cache || !a.qo_indptr || !a.kv_indptr || (!a.kv_indices && a.num_indices != 0) || !a.last_page_len || !a.out)
+    return fail(MK_E_INVALID, "chunk_attention: null pointer");  // (an empty tensor has no address)
   if (a.dtype != MK_BF16 && a.dtype != MK_F16) return fail(MK_E_INVALID, "chunk_attention: rows and caches are bf16 or fp16");
   if (a.tokens < 0 || a.q_heads < 1 || a.kv_heads < 1 || a.page_size < 1 || a.pages < 1 || a.num_indices < 0 || a.window < 0 || a.sinks < 0 || a.max_new < 0)
     return fail(MK_E_INVALID, "chunk_attention: negative or zero size");

@@ -23,3 +23,23 @@ def test_sample_from_a_vocabulary_of_millions(top_p):
     u = torch.tensor([0.0, 0.37, 0.86, 1 - 2.0 ** -24], device="cuda")
     check_sample(logits.expand(4, -1), u, 1.0, 0, top_p, 0.0)
     check_sample(logits.expand(4, -1), u, 1.0, 7_000_000, top_p, 0.0)
+
+
+def test_sample_of_a_step_without_rows():
+    """Nothing was granted: no row of logits, and -1 for every request."""
+    logits, u = rnd(gen(0), 4, 50, dtype=torch.float32), torch.rand(3, device="cuda")
+    for none in (logits[:0], torch.empty(0, 50, device="cuda")):
+        tokens, lp = mk.sample_tokens(none, u, 0.8, 5, qo_indptr=i32([0, 0, 0, 0]), return_logprobs=True)
+        assert tokens.tolist() == [-1] * 3 and lp.tolist() == [-math.inf] * 3
+
+
+@pytest.mark.parametrize("rows", [2, 140])
+def test_attention_of_requests_without_pages(rows):
+    """An index without entries: every row sees nothing."""
+    q = rnd(gen(rows), rows + 1, 8, D)
+    cache = torch.full((3, 16, 2, D), math.nan, dtype=BF, device="cuda")
+    out, lse = torch.full_like(q, 7.0), torch.full((rows + 1, 8), 7.0, device="cuda")
+    empty = torch.empty(0, dtype=torch.int32, device="cuda")
+    mk.chunk_attention(q, cache, cache, i32([0, rows, rows]), i32([0, 0, 0]), empty, i32([0, 0]), out=out, lse=lse)
+    assert not out[:rows].any() and bool((lse[:rows] == -math.inf).all())
+    assert bool((out[rows] == 7).all()) and bool((lse[rows] == 7).all())

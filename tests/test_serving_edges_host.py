@@ -1,4 +1,5 @@
 """The serving operators at the edges of what their documentation allows, as far as no GPU is needed."""
+import ctypes as C
 import os
 import socket
 
@@ -7,6 +8,8 @@ import torch
 import torch.multiprocessing as mp
 
 import fleet_chiplet_megakernel_b200 as mk
+from fleet_chiplet_megakernel_b200 import _cabi
+from tests.test_serving_host import filled, refused
 
 NAMES = {"q": "self_attn.q_proj.weight", "k": "self_attn.k_proj.weight", "v": "self_attn.v_proj.weight", "o": "self_attn.o_proj.weight",
          "qn": "self_attn.q_norm.weight", "kn": "self_attn.k_norm.weight", "gate": "mlp.gate_proj.weight", "up": "mlp.up_proj.weight",
@@ -75,3 +78,15 @@ def test_mpk_draws_from_no_logits_that_nothing_fills(native_lib):
     with pytest.raises(ValueError, match="CUDA"):
         m.sample_tokens(torch.zeros(2))
     m.finalize()
+
+
+# ------------------------------------------------------------------------------------
+# arguments of the C entry points
+# ------------------------------------------------------------------------------------
+def test_arrays_without_entries_need_no_address(native_lib):
+    """No rows of logits, no pages: the call goes on to its next check; with one entry an address is needed."""
+    refused(native_lib, "mk_sample_tokens", filled(_cabi.MkSampleArgs, dtype=_cabi.MK_F32, logits=None, rows=0, vocab=0), _cabi.MK_E_INVALID, "sizes")
+    refused(native_lib, "mk_sample_tokens", filled(_cabi.MkSampleArgs, dtype=_cabi.MK_F32, logits=None, rows=1), _cabi.MK_E_INVALID, "null")
+    base = {"dtype": _cabi.MK_BF16, "kv_indices": None, "workspace": None}
+    refused(native_lib, "mk_chunk_attention", filled(_cabi.MkChunkAttentionArgs, **base, num_indices=0), _cabi.MK_E_INVALID, "workspace")
+    refused(native_lib, "mk_chunk_attention", filled(_cabi.MkChunkAttentionArgs, **base, num_indices=1), _cabi.MK_E_INVALID, "null")
