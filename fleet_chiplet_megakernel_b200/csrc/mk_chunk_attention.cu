@@ -165,6 +165,7 @@ template <int NT, int U> struct Joined {
 template <typename T, int NT, int RING> struct RowWarp {
   static constexpr int ROWS = 8 * NT;
   static constexpr int kRing = RING;
+  static constexpr float kLift = __is_same(T, __half) ? 32768.f : 1.f;  // (weights are at most 1 here; hi + lo then reach down to 2^-40)
   static constexpr int kWarpRing = kRing * 2 * kTileBytes;
   static constexpr int kPartsBytes = kRowWarps * part_floats(ROWS) * (int)sizeof(float);
   static int smem_bytes(int requests) { return kRowWarps * kWarpRing + kPartsBytes + (requests + 1) * 8; }
@@ -407,7 +408,7 @@ template <typename T, int NT, int RING> struct RowWarp {
           m[n] = mn;
           float w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = exp2f(sc[n][e] - base);
+          for (int e = 0; e < 4; ++e) w[e] = exp2f(sc[n][e] - base) * kLift;
           l[n] = l[n] * alpha[n] + ((w[0] + w[1]) + (w[2] + w[3]));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -445,6 +446,14 @@ template <typename T, int NT, int RING> struct RowWarp {
       for (int n = 0; n < NT; ++n) {
         l[n] += __shfl_xor_sync(kAll, l[n], 1);
         l[n] += __shfl_xor_sync(kAll, l[n], 2);
+        if constexpr (kLift != 1.f) {
+          l[n] *= 1.f / kLift;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            o[n][i].x *= 1.f / kLift; o[n][i].y *= 1.f / kLift;
+            o[n][i].z *= 1.f / kLift; o[n][i].w *= 1.f / kLift;
+          }
+        }
         bad = bad || !isfinite(l[n]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) bad = bad || !isfinite((o[n][i].x + o[n][i].y) + (o[n][i].z + o[n][i].w));

@@ -15,6 +15,10 @@ namespace mk_serving {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// Weights enter their product with V in 16 bits.  bf16 holds them all with the same relative rounding.  fp16 has fewer and fewer bits below 2^-14
+// and nothing below 2^-25, while a row of some ten thousand positions can consist of such weights; so in fp16 they are carried 2^kLift
+// times as large, up to 2^15 of the 2^16 that the type holds, and the sums divided by it at the end (both exactly).
+
 // Pieces of a group that are to be joined: the warp, or CTA, with the last one (-1: none), and the group's rows.
 struct MergeRecord {
   int last;

@@ -10,8 +10,9 @@
 //                    it lies in the cache); while one row tile is in its softmax the other one's products run
 // Tensor memory: S and O of both row tiles, 4 x 128 columns; P overwrites the S that it comes from, and
 // its product with V begins with the first 64 positions.  O is scaled only when a
-// row's maximum has grown by more than 2^8 over the one in use: until then weights above 1 are as good as any, the sum has them too.
-// P is rounded to the type of V, which adds as much error as the rounding of the output; everything else is fp32.
+// row's maximum has grown by more than 2^8 (fp16: 2^4) over the one in use: until then weights above 1 are as good as any, the sum has them too.
+// P is rounded to the type of V, which adds as much error as the rounding of the output (fp16: weights of less than 2^-25 of the
+// largest are off by 2^-36 of it); everything else is fp32.
 // V rows behind a request's last position are cleared in shared memory (weight 0 times NaN is NaN); pieces whose sums are not
 // finite all the same are done again by exact_row.
 // Few CTAs (short chunks of long requests): every row tile's positions are cut into pieces, and a second kernel merges them.
@@ -32,7 +33,8 @@ constexpr int kStages = 5;
 constexpr int kTileThreads = 320, kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kSmemBytes = 2 * kStageBytes + kStages * kStageBytes + 256;
 constexpr unsigned long long kWaitNs = 2000000000ull;  // a wait that takes longer has lost its partner
-constexpr float kGrow = 8.f;                     // log2 of the weights that a stale maximum may lead to
+template <typename T> constexpr float kGrow = __is_same(T, __half) ? 4.f : 8.f;    // log2 of the weights that a stale maximum may lead to
+template <typename T> constexpr float kLift = __is_same(T, __half) ? 11.f : 0.f;   // log2 of what they are carried larger by
 
 struct TileParams {
   AttnParams p;
@@ -408,7 +410,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       return fmaxf(x, y);
     };
     auto weigh = [&](const uint32_t (&s)[32], int c) {  // the weights of quarter c of a tile
-      const uint64_t base2 = pair(-base, -base);
+      const uint64_t base2 = pair(kLift<T> - base, kLift<T> - base);
       uint32_t w16[16];
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -426,11 +428,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     };
     // the base of a row that has moved; what there is of the row's sums follows
     auto move_base = [&](bool sums) {
-      const bool grow = top > base + kGrow || (unset && top > -INFINITY);
+      const bool grow = top > base + kGrow<T> || (unset && top > -INFINITY);
       if (!__any_sync(kAll, grow)) return;
-      const float alpha = !grow ? 1.f : unset ? 0.f : ex2(base - top);  // (no weight yet: whatever there is, is zero)
+      const float to_base = kLift<T> != 0.f ? ceilf(top) : top;  // (a whole number, so that the lift can be taken from it without rounding)
+      const float alpha = !grow ? 1.f : unset ? 0.f : ex2(base - to_base);  // (no weight yet: whatever there is, is zero)
       if (grow) {
-        base = top;
+        base = to_base;
         unset = false;
       }
       l *= alpha;
@@ -488,6 +491,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       l += both.x + both.y;
       sum[0] = sum[1] = 0;
     }
+    constexpr float kDrop = __is_same(T, __half) ? 0x1p-11f : 1.f;  // 2^-kLift
+    l *= kDrop;
     const float m = l == 0.f ? -INFINITY : base;
     // ---- the rows' outputs
     if (ok && n > 0) ok = bar_wait(o_full + 8 * w, 0, dead);
@@ -504,7 +509,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
 #pragma unroll
     for (int k = 0; k < 4; ++k) rows[k] = reinterpret_cast<T*>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(dst), (lane & ~3) + k));
     bool bad = mine && !isfinite(l);
-    const float inv = !ok ? __uint_as_float(0x7fc00000u) : p.splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+    const float inv = !ok ? __uint_as_float(0x7fc00000u) : p.splits > 1 ? kDrop : l == 0.f ? 0.f : kDrop / l;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
       uint32_t o[32];

@@ -43,3 +43,29 @@ def test_attention_of_requests_without_pages(rows):
     mk.chunk_attention(q, cache, cache, i32([0, rows, rows]), i32([0, 0, 0]), empty, i32([0, 0]), out=out, lse=lse)
     assert not out[:rows].any() and bool((lse[:rows] == -math.inf).all())
     assert bool((out[rows] == 7).all()) and bool((lse[rows] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("gap", [12.0, 15.0, 17.5, 20.0])
+@pytest.mark.parametrize("requests", [[(20000, 1)], [(9000, 3), (20000, 6)], [(20000, 80), (300, 1)]])
+def test_attention_of_many_small_weights(requests, gap, dtype):
+    """One position has a score `gap` above all others, which are what the output consists of: their weights exp(-gap) are small against 2^-14, below
+    which fp16 has fewer bits, and at last against 2^-25, from where on it has none.  On top of what every case may be off by, an fp16 weight
+    may by 2^-36 of the largest (it is carried 2^11 times as large or more, in steps of 2^-24)."""
+    b = Batch(requests, 4, 2, 64, dtype)
+    b.q.zero_(), b.k.zero_()
+    b.q[..., 0] = 16.0
+    b.v.abs_().mul_(500.0)
+    first = b.kv_indices[torch.tensor(b.kv[:-1], device="cuda")].long()
+    b.k[first, 0, :, 0] = gap / (16.0 * D ** -0.5)
+    b.v[first, 0] = 0.0
+    want, lse, tol, lse_tol = b.reference()
+    if dtype == FP:
+        for r, (c, n) in enumerate(requests):
+            v = b.v[b.kv_indices[b.kv[r]:b.kv[r + 1]].long()].flatten(0, 1)[: c + n].double().sum(0).repeat_interleave(2, 0)
+            tol[b.qo[r]:b.qo[r + 1]] += 2.0 ** -36 * v  # (the sum of weights is 1 or more of the largest)
+    b.run()
+    n = b.qo[-1]
+    off = (b.out[:n].double() - want).abs()
+    assert bool((off <= tol).all()), f"off by {float((off / want.abs()).nan_to_num(0).max())} of the value, {float((off / tol).max())} of what is allowed"
+    assert bool(((b.lse[:n].double() - lse).abs() <= lse_tol).all())
