@@ -365,6 +365,7 @@ template <typename T, int NT, int RING> struct RowWarp {
         const int fill = stage == 0 ? kRing - 1 : stage - 1;
         stage = stage == kRing - 1 ? 0 : stage + 1;
         load_next(fill);  // (the stage that the last tile left: every lane is past its reads)
+        __syncwarp();     // (lanes whose position is behind the end have looked no page up; ldmatrix and mma are the warp's together)
         if (c.k >= c.count) continue;
         const int start = c.position(c.k);
         const uint32_t lrow = (uint32_t)((lane & 7) + ((lane >> 4) << 3)), lchunk = (uint32_t)((lane >> 3) & 1);

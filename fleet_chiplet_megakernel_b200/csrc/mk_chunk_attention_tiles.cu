@@ -437,6 +437,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
         unset = false;
       }
       l *= alpha;
+      __syncwarp();  // (loads and stores of tensor memory are a warp's together, here and behind the call)
       if (!sums) return;
 #pragma unroll 1
       for (int c = 0; c < 8; ++c) {
@@ -513,6 +514,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
       uint32_t o[32];
+      __syncwarp();  // (lanes without a row, and those whose sums are not finite, have left the others below)
       if (n > 0 && ok) {
         tm_load(to + 32 * c, o);
         tm_wait_load();
@@ -528,9 +530,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
         f[e] *= inv;
       }
       if (p.splits > 1) {
-        if (!mine) continue;
+        if (mine) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part_o + 32 * c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          for (int e = 0; e < 32; e += 4) *reinterpret_cast<float4*>(part_o + 32 * c + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        }
       } else {
         uint32_t x[4][4];  // 16 bytes of 8 dims each; then of the four rows
 #pragma unroll
