@@ -44,7 +44,7 @@ class MkChunkAttentionArgs(C.Structure):
     _fields_ = [(n, _P) for n in ("q", "k_cache", "v_cache", "qo_indptr", "kv_indptr", "kv_indices", "last_page_len", "out", "lse", "workspace")] + \
         [("workspace_bytes", _L), ("q_stride", _L * 2), ("out_stride", _L * 2), ("lse_stride", _L * 2), ("k_cache_stride", _L * 3),
          ("v_cache_stride", _L * 3), ("scale", _F)] + \
-        [(n, _I) for n in ("dtype", "requests", "tokens", "q_heads", "kv_heads", "page_size", "pages", "num_indices", "window", "sinks", "max_new")]
+        [(n, _I) for n in ("dtype", "requests", "tokens", "q_heads", "kv_heads", "page_size", "pages", "num_indices", "window", "sinks", "max_new")] + [("wait_ns", _L)]
 
 
 class MkSampleArgs(C.Structure):
@@ -89,6 +89,7 @@ SIGNATURES = {
     "mk_tensor_read": (C.c_int, [C.c_void_p, C.c_int, C.c_void_p, C.c_int64]),
     "mk_linear_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "mk_op_error": (C.c_int, [C.c_char_p, C.c_int]),
+    "mk_op_check": (C.c_int, []),
     "mk_plan_step": (C.c_int, [C.POINTER(MkStepPlanArgs), C.c_void_p]),
     "mk_rotate_append": (C.c_int, [C.POINTER(MkRotateAppendArgs), C.c_void_p]),
     "mk_chunk_attention_workspace": (C.c_int64, [C.POINTER(MkChunkAttentionArgs)]),

@@ -28,6 +28,7 @@ struct {
   decltype(&mk_chunk_attention) attention;
   decltype(&mk_sample_tokens) sample;
   decltype(&mk_op_error) error;
+  decltype(&mk_op_check) check;
 } g_lib;
 
 // Texts are put together by std::to_string alone: formatting numbers through a C++ stream of this module ended the process on a
@@ -156,7 +157,7 @@ void count(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK(n == want, "wrong number
 
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  count(n, 6);
+  count(n, 7);
   auto at = [&](int i) { return PyLong_AsVoidPtr(v[i]); };
   g_lib.plan_step = reinterpret_cast<decltype(g_lib.plan_step)>(at(0));
   g_lib.rotate_append = reinterpret_cast<decltype(g_lib.rotate_append)>(at(1));
@@ -164,6 +165,15 @@ PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   g_lib.attention = reinterpret_cast<decltype(g_lib.attention)>(at(3));
   g_lib.sample = reinterpret_cast<decltype(g_lib.sample)>(at(4));
   g_lib.error = reinterpret_cast<decltype(g_lib.error)>(at(5));
+  g_lib.check = reinterpret_cast<decltype(g_lib.check)>(at(6));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* check_waits(PyObject*, PyObject* const*, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  count(n, 0);
+  status(g_lib.check());
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -371,7 +381,7 @@ PyObject* sample_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
 }
 
 #define MK_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
-PyMethodDef g_methods[] = {MK_METHOD(bind), MK_METHOD(plan_step), MK_METHOD(rotate_append), MK_METHOD(chunk_attention), MK_METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
+PyMethodDef g_methods[] = {MK_METHOD(bind), MK_METHOD(check_waits), MK_METHOD(plan_step), MK_METHOD(rotate_append), MK_METHOD(chunk_attention), MK_METHOD(sample_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_serving_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

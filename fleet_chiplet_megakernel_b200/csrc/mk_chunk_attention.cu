@@ -671,7 +671,7 @@ int check(const mk_chunk_attention_args& a) {
   if (!a.q || !a.k_cache || !a.v_cache || !a.qo_indptr || !a.kv_indptr || (!a.kv_indices && a.num_indices != 0) || !a.last_page_len || !a.out)
     return fail(MK_E_INVALID, "chunk_attention: null pointer");  // (an empty tensor has no address)
   if (a.dtype != MK_BF16 && a.dtype != MK_F16) return fail(MK_E_INVALID, "chunk_attention: rows and caches are bf16 or fp16");
-  if (a.tokens < 0 || a.q_heads < 1 || a.kv_heads < 1 || a.page_size < 1 || a.pages < 1 || a.num_indices < 0 || a.window < 0 || a.sinks < 0 || a.max_new < 0)
+  if (a.tokens < 0 || a.q_heads < 1 || a.kv_heads < 1 || a.page_size < 1 || a.pages < 1 || a.num_indices < 0 || a.window < 0 || a.sinks < 0 || a.max_new < 0 || a.wait_ns < 0)
     return fail(MK_E_INVALID, "chunk_attention: negative or zero size");
   if (a.q_heads % a.kv_heads) return fail(MK_E_INVALID, "chunk_attention: %d q heads on %d kv heads", a.q_heads, a.kv_heads);
   if (a.requests < 1 || a.requests > kMaxRequests)
@@ -685,8 +685,40 @@ int check(const mk_chunk_attention_args& a) {
   return 0;
 }
 
+std::atomic<unsigned long long*> g_lost{nullptr};
+
 }  // namespace
+
+unsigned long long* lost_word() {
+  unsigned long long* word = g_lost.load();
+  if (word) return word;
+  // (allowed while a stream is captured: the allocation has no part in the graph)
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+  void* fresh = nullptr;
+  const cudaError_t e = cudaHostAlloc(&fresh, sizeof *word, cudaHostAllocPortable | cudaHostAllocMapped);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return cudaGetLastError(), nullptr;
+  unsigned long long* const made = static_cast<unsigned long long*>(fresh);
+  *made = 0;
+  if (g_lost.compare_exchange_strong(word, made)) return made;
+  cudaFreeHost(fresh);  // (another thread was faster)
+  return word;
+}
+int report_lost_wait() {
+  unsigned long long* word = g_lost.load();
+  if (!word || __atomic_load_n(word, __ATOMIC_RELAXED) == 0) return 0;
+  const unsigned long long said = __atomic_exchange_n(word, 0ull, __ATOMIC_ACQ_REL);
+  if (!said) return 0;
+  static const char* const kNames[] = {"the rows of q", "the last rows of V", "scores", "scores", "weights", "weights", "weights", "weights", "sums", "sums"};
+  const unsigned bar = (unsigned)(said >> 32) & 0xffff;
+  const char* name = bar < sizeof kNames / sizeof *kNames ? kNames[bar] : bar < 15 ? "a tile of K or V" : "a stage to become free";
+  return fail(MK_E_DEVICE, "chunk_attention: in an earlier call the wait for %s ran out (CTA %u): rows of its output may be NaN", name, (unsigned)said);
+}
+
 }  // namespace mk_serving
+
+extern "C" int mk_op_check(void) { return mk_serving::report_lost_wait(); }
 
 extern "C" int64_t mk_chunk_attention_workspace(const mk_chunk_attention_args* args) {
   using namespace mk_serving;
@@ -699,6 +731,7 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   using namespace mk_serving;
   if (!args) return fail(MK_E_INVALID, "chunk_attention: null arguments");
   const mk_chunk_attention_args& a = *args;
+  if (int rc = report_lost_wait()) return rc;
   if (int rc = check(a)) return rc;
   if (a.tokens == 0) return 0;
   const Layout l = layout_of(a);

@@ -127,6 +127,12 @@ __device__ __noinline__ void exact_row(const AttnParams& p, const Request& q, co
     }
 }
 
+// A word of pinned host memory in which a kernel says that a wait has run out (null: there is none to be had): bit 63, which of the tile
+// kernel's barriers in bits 32 on, the CTA below.  One a process, whatever the device.
+unsigned long long* lost_word();
+// Taken out of it and made an error of: 0, or MK_E_DEVICE with its text.
+int report_lost_wait();
+
 // mk_chunk_attention_tiles.cu: whether the tile kernel takes such tensors at all, and its launch
 bool tiles_take(const mk_chunk_attention_args& a);
 int launch_tile_attention(const AttnParams& p, cudaStream_t s);

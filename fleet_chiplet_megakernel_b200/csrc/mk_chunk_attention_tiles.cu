@@ -32,7 +32,8 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr int kStages = 5;
 constexpr int kTileThreads = 320, kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kSmemBytes = 2 * kStageBytes + kStages * kStageBytes + 256;
-constexpr unsigned long long kWaitNs = 2000000000ull;  // a wait that takes longer has lost its partner
+constexpr int kTries = 16;
+constexpr unsigned long long kWaitNs = 2000000000ull;  // a wait that takes longer has lost its partner (where the caller sets no limit)
 template <typename T> constexpr float kGrow = __is_same(T, __half) ? 4.f : 8.f;    // log2 of the weights that a stale maximum may lead to
 template <typename T> constexpr float kLift = __is_same(T, __half) ? 11.f : 0.f;   // log2 of what they are carried larger by
 
@@ -41,6 +42,9 @@ struct TileParams {
   CUtensorMap q, k, v;
   int tokens_per_tile;  // 128 / q heads of a kv head
   int box;              // positions of a box of K or V
+  bool tries;           // whether a wait tries kTries times before it looks at the clock
+  unsigned long long wait_ns;
+  unsigned long long* lost;  // host memory: where a wait has run out
 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -58,25 +62,48 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* dead) {
+// (returns at once; bar_try may sleep for a while)
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// dead: null, or the CTA's word that says which wait has run out (the address of its barrier)
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* dead, unsigned long long limit) {
   unsigned long long t0, t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
   for (;;) {
-    if (bar_try(bar, parity)) return true;
-    if (*dead) return false;
+    if (bar_test(bar, parity)) return true;
+    if (dead && *dead) return false;
     asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    if (t - t0 > kWaitNs) {
-      *dead = 1;
+    if (t - t0 >= limit) {
+      if (dead) *dead = (int)bar;
       return false;
     }
+    __nanosleep(20);
   }
 }
 // False once a wait of this CTA has run out: every role then leaves its loop.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ bool bar_wait(const TileParams& tp, uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (tp.tries) {
 #pragma unroll 1
-  for (int i = 0; i < 16; ++i)
-    if (bar_try(bar, parity)) return true;
-  return bar_wait_slow(bar, parity, dead);
+    for (int i = 0; i < kTries; ++i)
+      if (bar_try(bar, parity)) return true;
+  }
+  return bar_wait_slow(bar, parity, dead, tp.wait_ns);
+}
+// The same by a warp: all of its lanes go on, or none.
+__device__ __forceinline__ bool warp_wait(const TileParams& tp, uint32_t bar, uint32_t parity, volatile int* dead) {
+  return __all_sync(kAll, bar_wait(tp, bar, parity, dead));
+}
+// What is under way already is waited for whatever the caller's limit is, and whether or not another wait has run out.
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+  if (!bar_try(bar, parity)) bar_wait_slow(bar, parity, nullptr, kWaitNs);
+  __syncwarp();
 }
 __device__ __forceinline__ bool elect() {
   uint32_t is;
@@ -211,11 +238,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
   const uint32_t smem = smem_addr(raw);
   const uint32_t sq = smem, skv = smem + 2 * kStageBytes, bars = skv + kStages * kStageBytes;
   const uint32_t q_full = bars, tail_full = bars + 8, s_full = bars + 16, p_full = bars + 32, o_full = bars + 64, kv_full = bars + 80, kv_empty = kv_full + 8 * kStages;
-  const uint32_t tm_slot = kv_empty + 8 * kStages;
+  const uint32_t tm_slot = kv_empty + 8 * kStages, done = tm_slot + 16;
   volatile int* dead = reinterpret_cast<volatile int*>(raw + (tm_slot + 8 - smem));
   if (tid == 32 * kLoadWarp) {
     bar_init(q_full, 1);
     bar_init(tail_full, 1);
+    bar_init(done, 1);
     for (int i = 0; i < 2; ++i) {
       bar_init(s_full + 8 * i, 1);
       bar_init(p_full + 16 * i, kTile);      // the first half of the positions, the second
@@ -260,14 +288,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     const int boxes = kTile / tp.box;           // of a half tile: at most 16
     const int rg = lane % boxes, half = lane / boxes;
     int stage = 0, parity = 1, sent = 0;  // (the first round of empty waits passes)
-    bool ok = true;
+    bool ok = true, cut = false;          // cut: the last tile, whose rows behind the last position are cleared, is under way or there
     for (int i = 0; i < n && ok; ++i) {
       const int start = span.position(k0 + i);
       // a page that does not exist, or a box behind the last position, has coordinate -1: zeros
       int page, in;
       locate(p, q, start + rg * tp.box, &page, &in);
-      for (int v = 0; v < 2 && ok; ++v) {
-        ok = bar_wait(kv_empty + 8 * stage, parity, dead);
+      for (int v = 0; v < 2; ++v) {
+        ok = warp_wait(tp, kv_empty + 8 * stage, parity, dead);
         if (!ok) break;
         // V rows behind the last position but in its box are cleared before anyone sees the tile
         const int rest = q.len - start;
@@ -277,8 +305,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
         __syncwarp();
         if (half < 2) load_box4(dst + half * kHalfBytes + rg * tp.box * 128, v ? &tp.v : &tp.k, bar, 64 * half, kv_head, in, page);
         __syncwarp();
-        if (tail) {
-          ok = bar_wait(tail_full, 0, dead);
+        if (tail) {  // (of the last tile alone)
+          cut = true;
+          ok = warp_wait(tp, tail_full, 0, dead);
+          if (!ok) break;
           const int end = (rest / tp.box + 1) * tp.box;
           for (int e = lane; e < (end - rest) * 16; e += 32) {
             const uint32_t at = dst + (uint32_t)((e & 1) * kHalfBytes + (rest + (e >> 4)) * 128 + ((e >> 1) & 7) * 16);
@@ -287,6 +317,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
           if (elect()) bar_arrive(kv_full + 8 * stage);
+          __syncwarp();
         }
         ++sent;
         if (++stage == kStages) {
@@ -295,18 +326,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
         }
       }
     }
-    if (!ok) {  // a wait ran out: no copy may be in flight when the CTA's shared memory goes to another one
-      int none = 0;
-      bar_wait_slow(q_full, 0, &none);
-      for (int k = max(0, sent - kStages); k < sent; ++k) bar_wait_slow(kv_full + 8 * (k % kStages), (k / kStages) & 1, &none);
-    }
+    // No copy may be in flight when the CTA's shared memory goes to another one.  (Those that nobody has waited for, where a wait has run out; a
+    // stage that was filled again had been read, and a tile that was cut short is behind all others.)
+    bar_drain(q_full, 0);
+    for (int k = max(0, sent - kStages); k < sent; ++k) bar_drain(kv_full + 8 * (k % kStages), (k / kStages) & 1);
+    if (cut) bar_drain(tail_full, 0);
   } else if (n > 0 && warp == kMmaWarp) {
     // ---- products
     constexpr uint32_t type = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1u : 0u;
     constexpr uint32_t qk = (1u << 4) | (type << 7) | (type << 10) | ((kTile >> 3) << 17) | ((kTile >> 4) << 24);
     constexpr uint32_t pv = qk | (1u << 16);  // B with its other dimension contiguous
     int stage = 0, parity = 0;
-    bool ok = bar_wait(q_full, 0, dead);
+    // A lane whose wait has run out goes on beside the others to the end of the round, where all of them agree to leave: agreeing on every wait
+    // takes 3 % of the whole kernel's time.  What the elected lane does not have it does not multiply.
+    bool ok = bar_wait(tp, q_full, 0, dead);
     auto advance = [&]() {
       if (++stage == kStages) {
         stage = 0;
@@ -314,7 +347,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       }
     };
     auto scores = [&](int w, uint32_t k) {  // S_w = Q_w K^T
-      if (elect()) {
+      if (elect() && ok) {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint32_t off = (ks >> 2) * kHalfBytes + (ks & 3) * 32;
@@ -325,7 +358,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       __syncwarp();
     };
     auto sums = [&](int w, uint32_t v, bool add, int half) {  // O_w += P_w V over half of the positions
-      if (elect()) {
+      if (elect() && ok) {
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           const int k = 4 * half + ks;
@@ -335,20 +368,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       __syncwarp();
     };
     auto release = [&](uint32_t bar) {
-      if (elect()) commit(bar);
+      if (elect() && ok) commit(bar);
       __syncwarp();
     };
-    ok = ok && bar_wait(kv_full, 0, dead);
-    if (ok) {
-      fence_after();
-      scores(0, skv);
-      if (two) scores(1, skv);
-      release(kv_empty);
-      advance();
-    }
+    ok = bar_wait(tp, kv_full, 0, dead) && ok;
+    fence_after();
+    scores(0, skv);
+    if (two) scores(1, skv);
+    release(kv_empty);
+    advance();
+    ok = __all_sync(kAll, ok);
     for (int i = 0; i < n && ok; ++i) {
       const uint32_t v = skv + stage * kStageBytes, v_empty = kv_empty + 8 * stage;
-      ok = bar_wait(kv_full + 8 * stage, parity, dead);
+      ok = bar_wait(tp, kv_full + 8 * stage, parity, dead);
       advance();
       const uint32_t k = skv + stage * kStageBytes, k_empty = kv_empty + 8 * stage;
       const bool more = i + 1 < n;
@@ -356,22 +388,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       for (int w = 0; w < 2; ++w) {
         if (w && !two) break;
         for (int half = 0; half < 2; ++half) {
-          ok = ok && bar_wait(p_full + 16 * w + 8 * half, i & 1, dead);
-          if (!ok) break;
+          ok = bar_wait(tp, p_full + 16 * w + 8 * half, i & 1, dead) && ok;
           fence_after();
           sums(w, v, i > 0, half);
         }
-        if (!ok) break;
         if (!more) release(o_full + 8 * w);
-        if (more && w == 0) ok = bar_wait(kv_full + 8 * stage, parity, dead);
-        if (!ok) break;
+        if (more && w == 0) ok = bar_wait(tp, kv_full + 8 * stage, parity, dead) && ok;
         if (w == (two ? 1 : 0)) release(v_empty);
         if (more) scores(w, k);
       }
-      if (ok && more) {
+      if (more) {
         release(k_empty);
         advance();
       }
+      ok = __all_sync(kAll, ok);
     }
   } else if (warp < 8 && (warp < 4 || two)) {
     // ---- softmax: a thread has a row
@@ -450,11 +480,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       }
     };
     for (int i = 0; i < n; ++i) {
-      ok = bar_wait(s_full + 8 * w, i & 1, dead);
-      if (!__all_sync(kAll, ok)) {
-        ok = false;
-        break;
-      }
+      ok = warp_wait(tp, s_full + 8 * w, i & 1, dead);
+      if (!ok) break;
       fence_after();
       const int start = span.position(k0 + i);
       const bool masked = !(start + kTile - 1 <= at0 && (a.window == 0 || start > (long long)at1 - a.window || start + kTile <= a.sinks));
@@ -496,8 +523,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     l *= kDrop;
     const float m = l == 0.f ? -INFINITY : base;
     // ---- the rows' outputs
-    if (ok && n > 0) ok = bar_wait(o_full + 8 * w, 0, dead);
-    ok = __all_sync(kAll, ok);
+    if (ok && n > 0) ok = warp_wait(tp, o_full + 8 * w, 0, dead);
     fence_after();
     const long long token = (long long)q.q0 + t0 + tok;
     const size_t part = ((size_t)split * a.tokens + token) * a.q_heads + head;
@@ -579,6 +605,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
   }
   fence_before();
   __syncthreads();
+  if (*dead) {  // a wait has run out: no product may be under way when tensor memory goes to another CTA
+    if (warp == kMmaWarp) {
+      fence_after();
+      if (elect()) commit(done);
+      __syncwarp();
+      bar_drain(done, 0);
+    }
+    if (tid == 0) {
+      *(volatile unsigned long long*)tp.lost = 1ull << 63 | (unsigned long long)((uint32_t)(*dead - (int)bars) / 8) << 32 | blockIdx.x;
+      __threadfence_system();
+    }
+    __syncthreads();
+  }
   if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm));
@@ -674,6 +713,9 @@ int launch_tile_attention(const AttnParams& p, cudaStream_t s) {
   TileParams tp = {};
   tp.p = p;
   tp.tokens_per_tile = kTile / p.per_kv;
+  tp.wait_ns = a.wait_ns ? (unsigned long long)a.wait_ns : kWaitNs;
+  tp.tries = tp.wait_ns >= 100000;  // (so many take some microseconds)
+  if (!(tp.lost = lost_word())) return fail(MK_E_CUDA, "chunk_attention: no pinned host memory for the kernel's status");
   tp.box = a.page_size & -a.page_size;
   if (tp.box > kTile) tp.box = kTile;
   if (!encode_fn()) return fail(MK_E_CUDA, "chunk_attention: cuTensorMapEncodeTiled is not available from this driver");

@@ -40,9 +40,15 @@ def _load():
         raise RuntimeError("the binding of the serving operators is missing or does not fit this torch: build it with "
                            "`python -m fleet_chiplet_megakernel_b200._build --force`") from e
     native.bind(*(C.cast(getattr(lib, name), C.c_void_p).value for name in
-                  ("mk_plan_step", "mk_rotate_append", "mk_chunk_attention_workspace", "mk_chunk_attention", "mk_sample_tokens", "mk_op_error")))
+                  ("mk_plan_step", "mk_rotate_append", "mk_chunk_attention_workspace", "mk_chunk_attention", "mk_sample_tokens", "mk_op_error", "mk_op_check")))
     _native = native
     return native
+
+
+def check_waits() -> None:
+    """Raises ``RuntimeError`` if a wait inside a kernel has run out (after 2 seconds) in a ``chunk_attention`` call that is done: rows of its output
+    may be NaN.  The next ``chunk_attention`` raises it as well, before it does anything.  Synchronize first, as before reading the output."""
+    (_native or _load()).check_waits()
 
 
 # ------------------------------------------------------------------------------------

@@ -200,11 +200,15 @@ int mk_linear_static(const void* x, const void* w, const void* residual, void* o
 
 /* Operators of a serving step for hosts that keep the paging metadata themselves (mode online_notoken): what stands around the
  * layers, and attention of chunks that are longer than a megakernel iteration.  No handle; every call enqueues its work on `stream`
- * of the current device, allocates nothing and keeps nothing between calls, so calls on different streams and captured ones do not
- * meet (each needs outputs and a workspace of its own).  Structures are read during the call only.  Strides count elements; the
+ * of the current device, allocates nothing (but, once a process, a word of pinned memory for mk_op_check) and keeps nothing between calls, so calls
+ * on different streams and captured ones do not meet (each needs outputs and a workspace of its own).  Structures are read during the call only.  Strides count elements; the
  * last dimension is contiguous.  Returns 0 or MK_E_*; mk_op_error gives the text of this thread's last refused call.  What device arrays
  * say (index pointers, pages, slots) is not visible to the checks: the kernels hold it against the sizes given here. */
 int mk_op_error(char* buf, int n);
+/* Whether a wait inside a kernel has run out in a call that is done: 0, or MK_E_DEVICE once, with its text.  Such a call may leave NaN in rows of
+ * its outputs and everything else intact.  Of the serving operators only mk_chunk_attention waits on more than the barriers of a CTA or cluster;
+ * its next call reports it as well, before it does anything.  Synchronize first: what still runs has not said anything yet. */
+int mk_op_check(void);
 
 #define MK_STEP_MAX_REQUESTS 8192
 
@@ -270,6 +274,7 @@ typedef struct mk_chunk_attention_args {
   float scale;
   int32_t dtype;                                      /* MK_BF16 or MK_F16 */
   int32_t requests, tokens, q_heads, kv_heads, page_size, pages, num_indices, window, sinks, max_new;
+  int64_t wait_ns;                                    /* limit of every wait in the kernel; 0 = default (2 s) */
 } mk_chunk_attention_args;
 int64_t mk_chunk_attention_workspace(const mk_chunk_attention_args* args);
 int mk_chunk_attention(const mk_chunk_attention_args* args, void* stream);

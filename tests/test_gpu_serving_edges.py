@@ -1,11 +1,13 @@
 """The serving operators at the edges of what their documentation allows: calls without rows or pages, vocabularies of millions, weights that a
 16-bit type has no value for, positions next to 2^31, tangents, tensors that share memory, waits that run out."""
+import ctypes as C
 import math
 
 import pytest
 import torch
 
 import fleet_chiplet_megakernel_b200 as mk
+from fleet_chiplet_megakernel_b200 import _cabi
 from tests.test_gpu_serving import Batch, check_sample, gen, i32, rnd
 
 pytestmark = pytest.mark.gpu
@@ -69,3 +71,61 @@ def test_attention_of_many_small_weights(requests, gap, dtype):
     off = (b.out[:n].double() - want).abs()
     assert bool((off <= tol).all()), f"off by {float((off / want.abs()).nan_to_num(0).max())} of the value, {float((off / tol).max())} of what is allowed"
     assert bool(((b.lse[:n].double() - lse).abs() <= lse_tol).all())
+
+
+# ------------------------------------------------------------------------------------
+# waits that run out
+# ------------------------------------------------------------------------------------
+def _call(b, wait_ns):
+    """chunk_attention through its C entry point, which has a limit of the kernel's waits."""
+    lib, a = _cabi.load(), _cabi.MkChunkAttentionArgs()
+    for name, t in (("q", b.q), ("k_cache", b.k), ("v_cache", b.v), ("qo_indptr", b.qo_indptr), ("kv_indptr", b.kv_indptr), ("kv_indices", b.kv_indices),
+                    ("last_page_len", b.last), ("out", b.out), ("lse", b.lse)):
+        setattr(a, name, t.data_ptr())
+    a.q_stride[:], a.out_stride[:], a.lse_stride[:] = b.q.stride()[:2], b.out.stride()[:2], b.lse.stride()
+    a.k_cache_stride[:], a.v_cache_stride[:] = b.k.stride()[:3], b.v.stride()[:3]
+    a.scale, a.dtype, a.requests, a.tokens = D ** -0.5, _cabi.MK_BF16 if b.dtype == BF else _cabi.MK_F16, len(b.requests), b.q.shape[0]
+    a.q_heads, a.kv_heads, a.pages, a.page_size, a.num_indices, a.wait_ns = b.n_q, b.n_kv, b.k.shape[0], b.page, b.kv_indices.numel(), wait_ns
+    a.workspace_bytes = lib.mk_chunk_attention_workspace(C.byref(a))
+    workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device="cuda")
+    a.workspace = workspace.data_ptr()
+    rc = lib.mk_chunk_attention(C.byref(a), torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    return rc
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("requests", [[(0, 300)], [(500, 140), (90, 1), (0, 70)], [(2000, 2100)]])
+def test_attention_whose_waits_run_out(requests, dtype):
+    """A limit below what a copy takes: the kernel ends, says so to the host, and leaves NaN in rows of its tiles; nothing else is lost.  Whatever the limit, a
+    row that is not NaN is right, and the calls behind are."""
+    b = Batch(requests, 8, 2, 16, dtype, pad=3)
+    mk.serving.check_waits()
+    want, _, tol, _ = b.reference()
+    n = b.qo[-1]
+    tiles = torch.cat([torch.full((k,), 4 * k > 32, device="cuda") for _, k in requests])  # rows of the tile kernel, of 4 q heads a kv head
+    for wait_ns in (1, 300, 1000, 2000, 4000, 10000, 30000, 90000):
+        b.out.fill_(7.0), b.lse.fill_(7.0)
+        assert _call(b, wait_ns) == 0
+        lost = b.out[:n].isnan().any(-1)
+        right = ((b.out[:n].double() - want).abs() <= tol).all(-1)
+        assert bool((lost | right).all()) and bool((b.out[n:] == 7).all()) and bool((b.lse[n:] == 7).all())
+        assert torch.equal(lost, b.lse[:n].isnan()) and not bool(lost[~tiles].any())
+        if wait_ns == 1:
+            assert bool(lost[tiles].all())
+        if bool(lost.any()):
+            with pytest.raises(RuntimeError, match=r"wait for .* ran out \(CTA \d+\)"):
+                if wait_ns % 3000 == 0:  # reported by whichever comes first
+                    mk.serving.check_waits()
+                else:
+                    b.run()
+            assert bool((lost == b.out[:n].isnan().any(-1)).all())  # (and that call has done nothing)
+        else:
+            try:  # (a warp whose rows are all behind the last one may have given up)
+                mk.serving.check_waits()
+            except RuntimeError as e:
+                assert "ran out" in str(e)
+        mk.serving.check_waits()
+        assert _call(b, 0) == 0 and bool(((b.out[:n].double() - want).abs() <= tol).all())
+    b.check()
+    mk.serving.check_waits()
