@@ -90,6 +90,7 @@ SIGNATURES = {
     "mk_linear_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "mk_op_error": (C.c_int, [C.c_char_p, C.c_int]),
     "mk_op_check": (C.c_int, []),
+    "mk_debug_share_memory": (C.c_int, [C.POINTER(C.c_int64), C.POINTER(C.c_int64)]),
     "mk_plan_step": (C.c_int, [C.POINTER(MkStepPlanArgs), C.c_void_p]),
     "mk_rotate_append": (C.c_int, [C.POINTER(MkRotateAppendArgs), C.c_void_p]),
     "mk_chunk_attention_workspace": (C.c_int64, [C.POINTER(MkChunkAttentionArgs)]),

@@ -737,6 +737,18 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   const Layout l = layout_of(a);
   if (!a.workspace || a.workspace_bytes < (int64_t)l.bytes || (((uintptr_t)a.workspace) & 15))
     return fail(MK_E_INVALID, "chunk_attention: a workspace of %lld bytes, 16-byte aligned, is needed", (long long)l.bytes);
+  // Outputs are written while others are worked out, so they may share memory with nothing else of the call.
+  auto rows = [&](const char* name, const void* at, const int64_t* stride, int bytes, int n) -> Memory {
+    return {name, at, (long long)n * bytes, 2, {a.tokens, a.q_heads}, {bytes * stride[0], bytes * stride[1]}};
+  };
+  auto cache = [&](const char* name, const void* at, const int64_t* stride) -> Memory {
+    return {name, at, 2 * kHeadDim, 3, {a.pages, a.page_size, a.kv_heads}, {2 * stride[0], 2 * stride[1], 2 * stride[2]}};
+  };
+  const Memory used[] = {rows("out", a.out, a.out_stride, 2, kHeadDim), rows("lse", a.lse, a.lse_stride, 4, 1), list_of("workspace", a.workspace, (long long)l.bytes, 1),
+                         rows("q", a.q, a.q_stride, 2, kHeadDim), cache("k_cache", a.k_cache, a.k_cache_stride), cache("v_cache", a.v_cache, a.v_cache_stride),
+                         list_of("qo_indptr", a.qo_indptr, a.requests + 1ll, 4), list_of("kv_indptr", a.kv_indptr, a.requests + 1ll, 4),
+                         list_of("kv_indices", a.kv_indices, a.num_indices, 4), list_of("last_page_len", a.last_page_len, a.requests, 4)};
+  if (int rc = refuse_shared("chunk_attention", used, 3, sizeof used / sizeof *used)) return rc;
   AttnParams p = {};
   p.a = a;
   p.per_kv = a.q_heads / a.kv_heads;

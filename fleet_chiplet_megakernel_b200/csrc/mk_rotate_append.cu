@@ -200,8 +200,24 @@ extern "C" int mk_rotate_append(const mk_rotate_append_args* args, void* stream)
               aligned16(a.v_cache) && aligned16(a.out) && aligned16(a.q_norm) && aligned16(a.k_norm);
   for (int i = 0; i < 2; ++i) wide = wide && !((a.q_stride[i] | a.k_stride[i] | a.v_stride[i] | a.out_stride[i] | a.table_stride[i]) & 7);
   for (int i = 0; i < 3; ++i) wide = wide && !((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7);
-  const cudaStream_t s = (cudaStream_t)stream;
   const bool f32 = a.table_dtype == MK_F32;
+  // Rows are written while others are read, so what is written may share memory with nothing else of the call.  (out may be q: the lanes
+  // that write a row have read it, and no others do.)
+  const bool in_place = a.out == a.q && (a.tokens == 1 || a.out_stride[0] == a.q_stride[0]) && (a.q_heads == 1 || a.out_stride[1] == a.q_stride[1]);
+  const long long row = 2 * kHeadDim, entry = f32 ? 4 : 2;
+  auto rows = [&](const char* name, const void* at, int heads, const int64_t* stride) -> Memory {
+    return {name, at, row, 2, {a.tokens, heads}, {2 * stride[0], 2 * stride[1]}};
+  };
+  auto cache = [&](const char* name, const void* at, const int64_t* stride) -> Memory {
+    return {name, at, row, 3, {a.pages, a.page_size, a.kv_heads}, {2 * stride[0], 2 * stride[1], 2 * stride[2]}};
+  };
+  auto table = [&](const char* name, const void* at, int64_t stride) -> Memory { return {name, at, entry * kHeadDim, 1, {a.table_rows}, {entry * stride}}; };
+  const Memory used[] = {cache("k_cache", a.k_cache, a.k_cache_stride), cache("v_cache", a.v_cache, a.v_cache_stride), rows("out", a.out, a.q_heads, a.out_stride),
+                         rows("k", a.k, a.kv_heads, a.k_stride), rows("v", a.v, a.kv_heads, a.v_stride), table("cos", a.cos, a.table_stride[0]),
+                         table("sin", a.sin, a.table_stride[1]), list_of("positions", a.positions, a.tokens, 4), list_of("slots", a.slots, a.tokens, 8),
+                         list_of("q_norm", a.q_norm, kHeadDim, 2), list_of("k_norm", a.k_norm, kHeadDim, 2), rows("q", in_place ? nullptr : a.q, a.q_heads, a.q_stride)};
+  if (int rc = refuse_shared("rotate_append", used, 3, sizeof used / sizeof *used)) return rc;
+  const cudaStream_t s = (cudaStream_t)stream;
   if (a.dtype == MK_BF16) return f32 ? launch<__nv_bfloat16, float>(a, wide, s) : launch<__nv_bfloat16, __nv_bfloat16>(a, wide, s);
   return f32 ? launch<__half, float>(a, wide, s) : launch<__half, __half>(a, wide, s);
 }

@@ -1122,6 +1122,13 @@ extern "C" int mk_sample_tokens(const mk_sample_args* args, void* stream) {
   if (a.requests > 0x7fffffff / kMaxCluster) return fail(MK_E_TOO_LARGE, "sample_tokens: %d requests", a.requests);
   if (!a.qo_indptr && a.rows < a.requests) return fail(MK_E_INVALID, "sample_tokens: %d rows of logits for %d requests", a.rows, a.requests);
   if (a.requests == 0) return 0;
+  // A request's token is written while others are drawn, so it may share memory with nothing that they read.
+  const int size = a.dtype == MK_F32 ? 4 : 2;
+  const Memory used[] = {list_of("out", a.tokens, a.requests, 8), list_of("logprobs", a.logprobs, a.requests, 4),
+                         {"logits", a.logits, (long long)a.vocab * size, 1, {a.rows}, {a.row_stride * size}}, list_of("u", a.u, a.requests, 4),
+                         list_of("temperature", a.temperature, a.requests, 4), list_of("top_k", a.top_k, a.requests, 4), list_of("top_p", a.top_p, a.requests, 4),
+                         list_of("min_p", a.min_p, a.requests, 4), list_of("qo_indptr", a.qo_indptr, a.requests + 1ll, 4)};
+  if (int rc = refuse_shared("sample_tokens", used, 2, sizeof used / sizeof *used)) return rc;
   const cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = a.dtype == MK_F32 ? launch<float>(a, st) : a.dtype == MK_BF16 ? launch<__nv_bfloat16>(a, st) : launch<__half>(a, st);
   return e == cudaSuccess ? 0 : fail(MK_E_CUDA, "sample_tokens: launch failed: %s", cudaGetErrorString(e));

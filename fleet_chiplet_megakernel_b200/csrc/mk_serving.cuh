@@ -45,6 +45,21 @@ template <auto kernel> cudaError_t allow_shared(int bytes) noexcept {
 // Multiprocessors of the current device (the value of a device does not change).
 int sm_count();
 
+// What a call reads or writes of one tensor: entries of `reach` bytes, at `at` plus multiples of the strides (bytes), size[i] of each.
+struct Memory {
+  const char* name;
+  const void* at;
+  long long reach;
+  int dims;
+  long long size[3], stride[3];
+};
+inline Memory list_of(const char* name, const void* at, long long n, int bytes) { return {name, at, n * bytes, 0, {}, {}}; }
+// Whether two of them have a byte in common.  Exactly, where the strides nest as those of slices and permutations of a tensor do; where
+// the search would take long, true.
+bool share_memory(const Memory& a, const Memory& b);
+// The first pair of the `n` that shares memory, the first `written` of them with any other: an error that names them (0: none).
+int refuse_shared(const char* what, const Memory* m, int written, int n);
+
 inline bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
 
 // ---- 16-bit types

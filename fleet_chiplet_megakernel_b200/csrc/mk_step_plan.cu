@@ -186,6 +186,80 @@ int sm_count() {
   }
   return n;
 }
+namespace {
+using Wide = __int128;  // (sizes and strides of a C caller may be anything)
+struct Term {  // count * stride, count between lo and hi
+  Wide stride, lo, hi;
+};
+// Whether offset + sum of the terms k.. can be above -below and below above.  steps: what the search may still take.
+bool reaches(const Term* t, int n, int k, Wide offset, Wide below, Wide above, int* steps) {
+  Wide least = 0, most = 0;  // of the terms behind k
+  for (int i = k + 1; i < n; ++i) least += t[i].lo * t[i].stride, most += t[i].hi * t[i].stride;
+  if (k == n) return offset > -below && offset < above;
+  if (--*steps < 0) return true;
+  // counts with offset + count * stride + most > -below and offset + count * stride + least < above
+  auto floor_div = [](Wide x, Wide y) { return x / y - (x % y < 0 ? 1 : 0); };
+  Wide lo = floor_div(-below - offset - most, t[k].stride) + 1, hi = floor_div(above - 1 - offset - least, t[k].stride);
+  if (lo < t[k].lo) lo = t[k].lo;
+  if (hi > t[k].hi) hi = t[k].hi;
+  for (Wide c = lo; c <= hi; ++c)
+    if (reaches(t, n, k + 1, offset + c * t[k].stride, below, above, steps)) return true;
+  return false;
+}
+}  // namespace
+bool share_memory(const Memory& a, const Memory& b) {
+  if (!a.at || !b.at || a.reach <= 0 || b.reach <= 0) return false;
+  Term t[6];
+  int n = 0;
+  auto add = [&](long long size, long long stride, bool of_a) {  // entries of b count upwards from those of a
+    if (size <= 1 || stride == 0) return;
+    Wide lo = of_a ? 1 - (Wide)size : 0, hi = of_a ? 0 : (Wide)size - 1;
+    Wide s = stride;
+    if (s < 0) {
+      s = -s;
+      const Wide x = -lo;
+      lo = -hi;
+      hi = x;
+    }
+    int k = 0;
+    while (k < n && t[k].stride > s) ++k;
+    if (k < n && t[k].stride == s) {
+      t[k].lo += lo;
+      t[k].hi += hi;
+      return;
+    }
+    for (int i = n++; i > k; --i) t[i] = t[i - 1];
+    t[k] = {s, lo, hi};
+  };
+  for (int i = 0; i < a.dims; ++i) {
+    if (a.size[i] <= 0) return false;
+    add(a.size[i], a.stride[i], true);
+  }
+  for (int i = 0; i < b.dims; ++i) {
+    if (b.size[i] <= 0) return false;
+    add(b.size[i], b.stride[i], false);
+  }
+  int steps = 2000;
+  return reaches(t, n, 0, (Wide)(intptr_t)b.at - (Wide)(intptr_t)a.at, b.reach, a.reach, &steps);
+}
+int refuse_shared(const char* what, const Memory* m, int written, int n) {  // (n <= 16)
+  // (most are apart as a whole: a fraction of a microsecond, a microsecond without)
+  struct {
+    Wide first, last;  // last: behind the last byte
+  } at[16];
+  for (int i = 0; i < n; ++i) {
+    at[i].first = (Wide)(intptr_t)m[i].at;
+    at[i].last = at[i].first + m[i].reach;
+    for (int k = 0; k < m[i].dims; ++k) {
+      const Wide far = m[i].size[k] > 1 ? (Wide)(m[i].size[k] - 1) * m[i].stride[k] : 0;
+      (far < 0 ? at[i].first : at[i].last) += far;
+    }
+  }
+  for (int i = 0; i < written; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (at[i].first < at[j].last && at[j].first < at[i].last && share_memory(m[i], m[j])) return fail(MK_E_INVALID, "%s: %s and %s share memory", what, m[i].name, m[j].name);
+  return 0;
+}
 char* error_text() {
   static thread_local char text[kErrorBytes];
   return text;
@@ -197,6 +271,20 @@ extern "C" int mk_op_error(char* buf, int n) {
   if (!buf || n <= 0) return MK_E_INVALID;
   snprintf(buf, n, "%s", mk_serving::error_text());
   return 0;
+}
+
+extern "C" int mk_debug_share_memory(const int64_t* memory, const int64_t* other) {
+  using namespace mk_serving;
+  Memory m[2] = {};
+  for (int k = 0; k < 2; ++k) {
+    const int64_t* v = k ? other : memory;
+    if (!v || v[2] < 0 || v[2] > 3) return MK_E_INVALID;
+    m[k].at = (const void*)(intptr_t)v[0];
+    m[k].reach = v[1];
+    m[k].dims = (int)v[2];
+    for (int i = 0; i < 3; ++i) m[k].size[i] = v[3 + i], m[k].stride[i] = v[6 + i];
+  }
+  return share_memory(m[0], m[1]) ? 1 : 0;
 }
 
 extern "C" int mk_plan_step(const mk_step_plan_args* args, void* stream) {

@@ -210,6 +210,10 @@ int mk_op_error(char* buf, int n);
  * its next call reports it as well, before it does anything.  Synchronize first: what still runs has not said anything yet. */
 int mk_op_check(void);
 
+/* Test hook: whether entries of `reach` bytes at `at` and multiples of the strides (bytes) have a byte in common with those of another tensor, as the
+ * operators check what they write.  memory: {at, reach, dims (0 to 3), sizes[3], strides[3]}.  1, 0, or MK_E_INVALID. */
+int mk_debug_share_memory(const int64_t* memory, const int64_t* other);
+
 #define MK_STEP_MAX_REQUESTS 8192
 
 /* Page allocation, block tables, index pointers and slot map of a step.  Request r has lengths[r] tokens in the cache, on the pages

@@ -129,3 +129,53 @@ def test_attention_whose_waits_run_out(requests, dtype):
         assert _call(b, 0) == 0 and bool(((b.out[:n].double() - want).abs() <= tol).all())
     b.check()
     mk.serving.check_waits()
+
+
+# ------------------------------------------------------------------------------------
+# tensors that share memory
+# ------------------------------------------------------------------------------------
+def test_tensors_that_share_memory_are_refused_and_slices_beside_each_other_are_not():
+    b = Batch([(200, 2), (0, 50)], 8, 2, 16)
+    rows = b.qo[-1]
+    b.check()
+    joint = torch.zeros(rows + 1, 16, D, dtype=BF, device="cuda")
+    joint[1:, :8] = b.q
+    b.q, kept = joint[1:, :8], b.out
+    for out in (joint[:-1, :8], joint[1:, 1:9], b.k.view(-1)[: rows * 8 * D].view(rows, 8, D)):
+        b.out = out
+        with pytest.raises(ValueError, match="out and (q|k_cache) share memory"):
+            b.run()
+    b.out = joint[1:, 8:]
+    b.check()
+    b.out, lse = kept, b.lse
+    b.lse = kept.view(torch.float32).view(-1)[: rows * 8].view(rows, 8)
+    with pytest.raises(ValueError, match="out and lse share memory"):
+        b.run()
+    b.lse = lse
+    assert torch.equal(joint[1:, :8], b.q) and not joint[0].any()
+
+    g = gen(0)
+    x = rnd(g, 6, 8, D)
+    q, k, v = x[:, :4], x[:, 4:6], x[:, 6:]
+    cos, sin = torch.ones(6, D, device="cuda"), torch.zeros(6, D, device="cuda")
+    kv = torch.zeros(4, 2, 4, 2, D, dtype=BF, device="cuda")
+    flat = kv.view(-1)
+    args = dict(q=q, k=k, v=v, cos=cos, sin=sin, positions=torch.arange(6, dtype=torch.int32, device="cuda"), slots=torch.arange(6, device="cuda"),
+                k_cache=kv[:3, 0], v_cache=kv[:3, 1])
+    row_later = flat.as_strided((3, 4, 2, D), kv[:3, 0].stride(), 2 * D)
+    for change, text in ((dict(v_cache=row_later), "k_cache and v_cache"), (dict(out=x[:, 2:6]), "out and (k|q)"), (dict(out=kv[0, 0].reshape(-1)[: 6 * D].view(6, 1, D).expand(6, 4, D)), "share memory"),
+                         (dict(out=flat[: 6 * 4 * D].view(6, 4, D)), "k_cache and out"), (dict(k=kv[:2].view(-1, 2, D)[:6]), "k_cache and k")):
+        with pytest.raises(ValueError, match=text):
+            mk.rotate_append(**{**args, **change})
+    assert not kv.any()
+    out = mk.rotate_append(**args, out=q)
+    assert torch.equal(out, q) and torch.equal(kv[:3, 0].reshape(12, 2, D)[:6], k) and torch.equal(kv[:3, 1].reshape(12, 2, D)[:6], v)
+
+    logits, buf = rnd(g, 4, 50, dtype=torch.float32), torch.ones(8, dtype=torch.float32, device="cuda")
+    for kw in (dict(u=buf[:4]), dict(u=buf[4:]), dict(u=torch.rand(4, device="cuda"), temperature=buf[2:6]), dict(u=torch.rand(4, device="cuda"), top_k=buf.view(torch.int32)[:4])):
+        with pytest.raises(ValueError, match="out and .* share memory"):
+            mk.sample_tokens(logits, out=buf.view(torch.int64), **kw)
+    with pytest.raises(ValueError, match="out and logits share memory"):
+        mk.sample_tokens(logits, torch.rand(4, device="cuda"), out=logits.view(-1)[:8].view(torch.int64))
+    with pytest.raises(ValueError, match="out and qo_indptr"):
+        mk.sample_tokens(logits, torch.rand(3, device="cuda"), qo_indptr=buf.view(torch.int32)[:4], out=buf.view(torch.int64)[:3])

@@ -1,6 +1,7 @@
 """The serving operators at the edges of what their documentation allows, as far as no GPU is needed."""
 import ctypes as C
 import os
+import random
 import socket
 
 import pytest
@@ -9,7 +10,7 @@ import torch.multiprocessing as mp
 
 import fleet_chiplet_megakernel_b200 as mk
 from fleet_chiplet_megakernel_b200 import _cabi
-from tests.test_serving_host import filled, refused
+from tests.test_serving_host import FAKE, filled, refused
 
 NAMES = {"q": "self_attn.q_proj.weight", "k": "self_attn.k_proj.weight", "v": "self_attn.v_proj.weight", "o": "self_attn.o_proj.weight",
          "qn": "self_attn.q_norm.weight", "kn": "self_attn.k_norm.weight", "gate": "mlp.gate_proj.weight", "up": "mlp.up_proj.weight",
@@ -90,3 +91,85 @@ def test_arrays_without_entries_need_no_address(native_lib):
     base = {"dtype": _cabi.MK_BF16, "kv_indices": None, "workspace": None}
     refused(native_lib, "mk_chunk_attention", filled(_cabi.MkChunkAttentionArgs, **base, num_indices=0), _cabi.MK_E_INVALID, "workspace")
     refused(native_lib, "mk_chunk_attention", filled(_cabi.MkChunkAttentionArgs, **base, num_indices=1), _cabi.MK_E_INVALID, "null")
+
+
+# ------------------------------------------------------------------------------------
+# tensors that share memory
+# ------------------------------------------------------------------------------------
+def _memory(at, reach, sizes, strides):
+    v = [at, reach, len(sizes)] + (list(sizes) + [1] * 3)[:3] + (list(strides) + [0] * 3)[:3]
+    return (C.c_int64 * 9)(*v)
+
+
+def _bytes(at, reach, sizes, strides):
+    starts = [at]
+    for n, s in zip(sizes, strides):
+        starts = [x + i * s for x in starts for i in range(n)]
+    return {x + k for x in starts for k in range(reach)}
+
+
+def test_shared_memory_is_found_exactly(native_lib):
+    """Against the sets of bytes: slices, permutations and views of other shapes of one buffer, broadcast and empty ones."""
+    rng = random.Random(5)
+    seen = [0, 0]
+    for _ in range(4000):
+        def one():
+            dims = rng.randint(0, 3)
+            strides, at = [], 1
+            for _ in range(dims):  # nested, with gaps or without; some of them broadcast
+                at *= rng.choice([1, 2, 3, 4, 5, 8])
+                strides.append(0 if rng.random() < 0.05 else 4 * at)
+            sizes = [rng.choice([0, 1, 2, 3, 4]) if rng.random() < 0.9 else 7 for _ in range(dims)]
+            rng.shuffle(strides)
+            return 4096 + 4 * rng.randint(0, 60), rng.choice([4, 8, 16]), sizes, strides
+        a, b = one(), one()
+        if rng.random() < 0.4:  # the same strides, another slice
+            b = (b[0], b[1], b[2][: len(a[2])] + [1] * (len(a[2]) - len(b[2])), a[3])
+        want = bool(_bytes(*a) & _bytes(*b))
+        assert native_lib.mk_debug_share_memory(_memory(*a), _memory(*b)) == want, (a, b)
+        assert native_lib.mk_debug_share_memory(_memory(*b), _memory(*a)) == want, (a, b)
+        seen[want] += 1
+    assert min(seen) > 500
+
+
+def test_shared_memory_of_real_layouts(native_lib):
+    meet = lambda a, b: native_lib.mk_debug_share_memory(_memory(*a), _memory(*b))  # noqa: E731
+    T, row = 4096, 256
+    base = 0x7f0000000000
+    part = lambda first, heads: (base + first * row, row, (T, heads), (48 * row, row))  # noqa: E731 (slices of one projection)
+    assert [meet(part(0, 32), part(32, 8)), meet(part(0, 32), part(40, 8)), meet(part(0, 33), part(32, 8)), meet(part(0, 32), part(31, 1))] == [0, 0, 1, 1]
+    # K and V interleaved by page, by row and by head; one page, row or head too many
+    for strides, gap in (((2 * 64 * 8 * row, 8 * row, row), 64 * 8 * row), ((64 * 16 * row, 16 * row, row), 8 * row), ((64 * 16 * row, 16 * row, 2 * row), row)):
+        k, v = (base, row, (1000, 64, 8), strides), (base + gap, row, (1000, 64, 8), strides)
+        assert meet(k, v) == 0 and meet(k, (base + gap - 2, row, (1000, 64, 8), strides)) == 1
+        assert meet(k, (base + strides[0], row, (1000, 64, 8), strides)) == 1
+    # two caches whose pages are 2 GB apart, an output inside the gap and one that is not
+    far = (base, row, (6, 16, 2), (1 << 31, 2 * row, row))
+    assert meet(far, (base + (1 << 30), row, (6, 16, 2), far[3])) == 0
+    assert meet(far, (base + 32 * row, row, (1000, 32), (32 * row, row))) == 0 and meet(far, (base + 31 * row, row, (1000, 32), (32 * row, row))) == 1
+    # strides that no address has
+    assert meet((base, row, (1 << 31, 1 << 31), (1 << 62, 1 << 62)), (base - row, row, (), ())) == 0
+
+
+def test_operators_refuse_what_shares_memory(native_lib):
+    """Every tensor that is written with every other of the call, at one element past its beginning (all other tensors are apart)."""
+    for cls, fn, written, more in (
+            (_cabi.MkRotateAppendArgs, "mk_rotate_append", ("out", "k_cache", "v_cache"),
+             dict(dtype=_cabi.MK_BF16, table_dtype=_cabi.MK_F32, q_stride=(128, 128), k_stride=(128, 128), v_stride=(128, 128), out_stride=(128, 128), table_stride=(128, 128),
+                  k_cache_stride=(128, 128, 128), v_cache_stride=(128, 128, 128), tokens=8)),
+            (_cabi.MkChunkAttentionArgs, "mk_chunk_attention", ("out", "lse", "workspace"),
+             dict(dtype=_cabi.MK_BF16, q_stride=(128, 128), out_stride=(128, 128), lse_stride=(1, 1), k_cache_stride=(128, 128, 128), v_cache_stride=(128, 128, 128),
+                  workspace_bytes=1 << 40, tokens=8, requests=8, num_indices=8)),
+            (_cabi.MkSampleArgs, "mk_sample_tokens", ("tokens", "logprobs"), dict(dtype=_cabi.MK_F32, rows=8, requests=8, vocab=8, row_stride=8))):
+        names = [n for n, kind in cls._fields_ if kind is C.c_void_p]
+        apart = {n: FAKE + (k << 26) for k, n in enumerate(names)}
+        for name in written:
+            for other in names:
+                if other == name or (name, other) == ("out", "q") and cls is _cabi.MkRotateAppendArgs:
+                    continue
+                refused(native_lib, fn, filled(cls, **{**apart, **more, other: apart[name] + 16}), _cabi.MK_E_INVALID, "share memory")
+    # out may be q, but not q moved by a row
+    base = dict(dtype=_cabi.MK_BF16, table_dtype=_cabi.MK_F32, q_stride=(128, 128), out_stride=(128, 128), tokens=8)
+    names = [n for n, kind in _cabi.MkRotateAppendArgs._fields_ if kind is C.c_void_p]
+    apart = {n: FAKE + (k << 26) for k, n in enumerate(names)}
+    refused(native_lib, "mk_rotate_append", filled(_cabi.MkRotateAppendArgs, **{**apart, **base, "out": apart["q"] + 256}), _cabi.MK_E_INVALID, "out and q share")
