@@ -94,6 +94,7 @@ struct Checks {
   }
   static void no_gradient(const at::Tensor& t, const char* what) {
     need(!t.requires_grad() || !c10::GradMode::is_enabled(), what, " requires a gradient and the serving operators have none: call them under torch.no_grad()");
+    need(!t._fw_grad(0).defined(), what, " carries a forward-mode tangent and the serving operators have no derivative: pass torch.autograd.forward_ad.unpack_dual(x).primal");
   }
   void here(const at::Tensor& t, const char* what) const {
     REFUSE_IF(t.device() != device, what, " is on ", t.device(), ", the first tensor on ", device);

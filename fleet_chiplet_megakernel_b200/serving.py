@@ -12,10 +12,10 @@ stream, allocates no more than its outputs and a workspace from torch's allocato
 
 The caches have the layout of the attention layers, ``[pages, page_size, kv_heads, 128]``, so the megakernel goes on from what these
 calls leave in them.  Tensors may be on any CUDA device (all of a call on one); wrong types, shapes and strides raise ``ValueError``,
-sizes beyond what a kernel takes ``NotImplementedError``.  So does a tensor that is written and shares memory with another one of the call
-(``ValueError``; slices beside each other in one buffer share none).  None of them has a gradient: a tensor that requires one is refused while
-gradients are recorded.  What index tensors hold is on the device and is not checked here: the
-kernels stay inside the tensors whatever it is.
+sizes beyond what a kernel takes ``NotImplementedError``.  A tensor that is written and shares memory with another one of the call is refused as well
+(slices beside each other in one buffer share none).  None of them has a derivative: a tensor that requires a gradient is refused while gradients are
+recorded, one with a forward-mode tangent always.  What index tensors hold is on the device and is not checked here: the kernels stay
+inside the tensors whatever it is.
 """
 from __future__ import annotations
 

@@ -179,3 +179,26 @@ def test_tensors_that_share_memory_are_refused_and_slices_beside_each_other_are_
         mk.sample_tokens(logits, torch.rand(4, device="cuda"), out=logits.view(-1)[:8].view(torch.int64))
     with pytest.raises(ValueError, match="out and qo_indptr"):
         mk.sample_tokens(logits, torch.rand(3, device="cuda"), qo_indptr=buf.view(torch.int32)[:4], out=buf.view(torch.int64)[:3])
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fw
+    b = Batch([(40, 2)], 8, 2, 16)
+    logits, u = rnd(gen(0), 2, 50, dtype=torch.float32), torch.rand(2, device="cuda")
+    cos = torch.ones(4, D, device="cuda")
+    x = rnd(gen(1), 2, 4, D)
+    caches = [torch.zeros(1, 4, 2, D, dtype=BF, device="cuda") for _ in range(2)]
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        with pytest.raises(ValueError, match="q carries a forward-mode tangent"):
+            mk.chunk_attention(dual(b.q), b.k, b.v, b.qo_indptr, b.kv_indptr, b.kv_indices, b.last)
+        with pytest.raises(ValueError, match="v_cache carries"), torch.no_grad():
+            mk.chunk_attention(b.q, b.k, dual(b.v), b.qo_indptr, b.kv_indptr, b.kv_indices, b.last)
+        with pytest.raises(ValueError, match="sin carries"):
+            mk.rotate_append(x, x[:, :2], x[:, 2:], cos, dual(cos), i32([0, 1]), torch.arange(2, device="cuda"), *caches)
+        with pytest.raises(ValueError, match="logits carries"):
+            mk.sample_tokens(dual(logits), u)
+        with pytest.raises(ValueError, match="temperature carries"):
+            mk.sample_tokens(logits, u, dual(torch.ones(2, device="cuda")))
+        mk.sample_tokens(fw.unpack_dual(dual(logits)).primal, u)
+    mk.sample_tokens(logits, u)
