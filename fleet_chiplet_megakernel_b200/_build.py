@@ -63,7 +63,9 @@ def check_registers(instances):
 
 
 def binding_command():
-    """The binding is compiled against the torch that runs it (its headers, its C++ ABI) and linked with torch alone."""
+    """The binding is compiled against the torch that runs it (its headers, its C++ ABI) and linked with torch alone.  The C++ runtime is
+    named: it has to be the process's shared one.  Some installations of g++ link a static one where no other is named, and with two of them a C++ stream
+    in the module (torch's macros format their errors through one) ends the process at the first number."""
     import torch
     root = os.path.dirname(torch.__file__)
     lib = os.path.join(root, "lib")
@@ -71,7 +73,7 @@ def binding_command():
                os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
     return ([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"] +
             [f"-I{i}" for i in include] + [os.path.join(CSRC, BINDING_SOURCE), "-o", BINDING, f"-L{lib}"] +
-            [f"-l{n}" for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python")])
+            [f"-l{n}" for n in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python", ":libstdc++.so.6")])
 
 
 def build(force=False, verbose=False):

@@ -31,8 +31,7 @@ struct {
   decltype(&mk_op_check) check;
 } g_lib;
 
-// Texts are put together by std::to_string alone: formatting numbers through a C++ stream of this module ended the process on a
-// machine with a GPU, where more libraries are loaded than here.
+// The texts of refusals.
 void put(std::string& s, const char* t) { s += t; }
 void put(std::string& s, const std::string& t) { s += t; }
 void put(std::string& s, int64_t v) { s += std::to_string(v); }
@@ -154,7 +153,7 @@ at::ScalarType row_type(const at::Tensor& t, const char* what) {
 }
 int code(at::ScalarType t) { return t == at::kBFloat16 ? MK_BF16 : t == at::kHalf ? MK_F16 : MK_F32; }
 at::Tensor new_rows(int64_t tokens, int64_t heads, const at::Tensor& like) { return at::zeros({tokens, heads, kHeadDim}, like.options().requires_grad(false)); }
-void count(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK(n == want, "wrong number of arguments"); }
+void count(Py_ssize_t n, Py_ssize_t want) { TORCH_CHECK(n == want, n, " arguments, ", want, " are needed"); }
 
 PyObject* bind(PyObject*, PyObject* const* v, Py_ssize_t n) {
   HANDLE_TH_ERRORS

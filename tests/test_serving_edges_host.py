@@ -3,6 +3,8 @@ import ctypes as C
 import os
 import random
 import socket
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -10,6 +12,7 @@ import torch.multiprocessing as mp
 
 import fleet_chiplet_megakernel_b200 as mk
 from fleet_chiplet_megakernel_b200 import _cabi
+from tests.conftest import ROOT
 from tests.test_serving_host import FAKE, filled, refused
 
 NAMES = {"q": "self_attn.q_proj.weight", "k": "self_attn.k_proj.weight", "v": "self_attn.v_proj.weight", "o": "self_attn.o_proj.weight",
@@ -173,3 +176,13 @@ def test_operators_refuse_what_shares_memory(native_lib):
     names = [n for n, kind in _cabi.MkRotateAppendArgs._fields_ if kind is C.c_void_p]
     apart = {n: FAKE + (k << 26) for k, n in enumerate(names)}
     refused(native_lib, "mk_rotate_append", filled(_cabi.MkRotateAppendArgs, **{**apart, **base, "out": apart["q"] + 256}), _cabi.MK_E_INVALID, "out and q share")
+
+
+# ------------------------------------------------------------------------------------
+# the binding
+# ------------------------------------------------------------------------------------
+def test_the_binding_shares_the_process_c_plus_plus_runtime(native_lib):
+    """torch's macros format numbers through a C++ stream in the module; with a runtime of its own (linked statically) that ends the process."""
+    code = "import torch, fleet_chiplet_megakernel_b200.serving as s\ntry: s._load().plan_step(1, 2, 3)\nexcept RuntimeError as e: print(e)"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0 and "3 arguments, 14 are needed" in r.stdout, (r.returncode, r.stdout, r.stderr)
