@@ -358,7 +358,9 @@ PyObject* sample_tokens(PyObject*, PyObject* const* v, Py_ssize_t n) {
   const c10::cuda::CUDAGuard guard(c.device);
   at::Tensor out = v[7] == Py_None ? at::empty({R}, logits.options().dtype(at::kLong).requires_grad(false)) : tensor(v[7], "out");
   a.tokens = c.list<int64_t>(out, "out", at::kLong, R);
-  const bool with_logprobs = v[8] == Py_True;
+  const int asked = PyObject_IsTrue(v[8]);
+  if (asked < 0) throw python_error();
+  const bool with_logprobs = asked != 0;
   at::Tensor logprobs;
   if (with_logprobs) {
     logprobs = at::empty({R}, logits.options().dtype(at::kFloat).requires_grad(false));

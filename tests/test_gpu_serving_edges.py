@@ -202,3 +202,14 @@ def test_forward_mode_tangents_are_refused():
             mk.sample_tokens(logits, u, dual(torch.ones(2, device="cuda")))
         mk.sample_tokens(fw.unpack_dual(dual(logits)).primal, u)
     mk.sample_tokens(logits, u)
+
+
+def test_logprobs_are_asked_for_by_any_true_value():
+    import numpy as np
+    logits, u = rnd(gen(0), 2, 50, dtype=torch.float32), torch.rand(2, device="cuda")
+    want = mk.sample_tokens(logits, u, return_logprobs=True)
+    for yes in (1, np.True_, "yes"):
+        got = mk.sample_tokens(logits, u, return_logprobs=yes)
+        assert isinstance(got, tuple) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    for no in (0, np.False_, None):
+        assert torch.equal(mk.sample_tokens(logits, u, return_logprobs=no), want[0])
