@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const __grid_co
     const int r = r0 + threadIdx.x;
     const int len = r < R ? length_of(r) : 0, want = r < R ? __ldg(a.new_tokens + r) : 0;
     const int held = pages_of(len), after = pages_of((unsigned)len + (unsigned)max(0, want));
-    const bool valid = want > 0 && after <= a.table_width;
+    const bool valid = want > 0 && after <= a.table_width && (unsigned)len + (unsigned)want <= 0x7fffffffu;  // (positions are ints)
     const int need = valid ? after - held : 0;
     long long v[3] = {need, 0, 0};
     scan(v, total, 1);

@@ -219,8 +219,8 @@ int mk_debug_share_memory(const int64_t* memory, const int64_t* other);
 /* Page allocation, block tables, index pointers and slot map of a step.  Request r has lengths[r] tokens in the cache, on the pages
  * block_table[r, 0 .. ceil(length / page)), and is to be fed new_tokens[r]: 0 idle, -1 ended (its pages go back behind the ring's
  * tail, first of all).  Free pages are free_pages[i % ring_size] for free_range[0] <= i < free_range[1].  Requests take pages and
- * token rows in their order; one that cannot get all of them, or whose row of the table is too short, is granted nothing, and
- * those behind it that need pages (or rows) neither.  Written: granted[r] (new tokens or 0), new pages into block_table, the
+ * token rows in their order; one that cannot get all of them is granted nothing, and those behind it that need pages (or rows) neither.
+ * One whose row of the table is too short, or that would pass 2^31 - 1 tokens, is granted nothing and holds up nobody.  Written: granted[r] (new tokens or 0), new pages into block_table, the
  * index pointers, pages and last page lengths as the attention layers read them, cache slot (page * page_size + row) and
  * position of every token row (-1 and 0 behind the last), and the free range behind the step.  lengths, new_tokens and
  * free_range_in are left as they are: the same call again gives the same step. */

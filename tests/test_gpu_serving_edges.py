@@ -213,3 +213,18 @@ def test_logprobs_are_asked_for_by_any_true_value():
         assert isinstance(got, tuple) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     for no in (0, np.False_, None):
         assert torch.equal(mk.sample_tokens(logits, u, return_logprobs=no), want[0])
+
+
+def test_plan_grants_no_position_past_32_bits():
+    """A request may grow to 2^31 - 1 tokens; one token more, and its positions (and its length) would not fit their type."""
+    page, top = 1 << 20, 2 ** 31 - 1
+    for more in (3, 4):
+        table = torch.full((2, 2100), -7, dtype=torch.int32, device="cuda")
+        table[0, :2048] = torch.arange(2048, dtype=torch.int32, device="cuda")
+        plan = mk.StepPlan.empty(2, 8, 2200)
+        mk.plan_step(i32([top - 3, 0]), i32([more, 2]), table, i32([2050, 2051]), torch.tensor([0, 2], device="cuda"), page, plan)
+        granted = 3 if more == 3 else 0
+        assert plan.granted.tolist() == [granted, 2]
+        own = [(2047 * page + page - 4 + i, top - 3 + i) for i in range(granted)]
+        assert list(zip(plan.slots.tolist(), plan.positions.tolist()))[: granted + 2] == own + [(2050 * page, 0), (2050 * page + 1, 1)]
+        assert plan.last_page_len.tolist() == [page - 4 + granted, 2]
