@@ -667,9 +667,13 @@ Layout layout_of(const mk_chunk_attention_args& a) {
   return l;
 }
 
-int check(const mk_chunk_attention_args& a) {
+int check_pointers(const mk_chunk_attention_args& a) {
   if (!a.q || !a.k_cache || !a.v_cache || !a.qo_indptr || !a.kv_indptr || (!a.kv_indices && a.num_indices != 0) || !a.last_page_len || !a.out)
     return fail(MK_E_INVALID, "chunk_attention: null pointer");  // (an empty tensor has no address)
+  if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out)) return fail(MK_E_INVALID, "chunk_attention: pointers must be 16-byte aligned");
+  return 0;
+}
+int check_sizes(const mk_chunk_attention_args& a) {
   if (a.dtype != MK_BF16 && a.dtype != MK_F16) return fail(MK_E_INVALID, "chunk_attention: rows and caches are bf16 or fp16");
   if (a.tokens < 0 || a.q_heads < 1 || a.kv_heads < 1 || a.page_size < 1 || a.pages < 1 || a.num_indices < 0 || a.window < 0 || a.sinks < 0 || a.max_new < 0 || a.wait_ns < 0)
     return fail(MK_E_INVALID, "chunk_attention: negative or zero size");
@@ -677,7 +681,6 @@ int check(const mk_chunk_attention_args& a) {
   if (a.requests < 1 || a.requests > kMaxRequests)
     return fail(a.requests < 1 ? MK_E_INVALID : MK_E_TOO_LARGE, "chunk_attention: %d requests (1 to %d)", a.requests, kMaxRequests);
   if ((long long)a.tokens * a.q_heads > 0x3fffffffll || (long long)a.requests * a.kv_heads > 0x3fffffffll || a.kv_heads > 65535) return fail(MK_E_TOO_LARGE, "chunk_attention: too many rows");
-  if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out)) return fail(MK_E_INVALID, "chunk_attention: pointers must be 16-byte aligned");
   for (int i = 0; i < 3; ++i)
     if ((a.k_cache_stride[i] | a.v_cache_stride[i]) & 7) return fail(MK_E_INVALID, "chunk_attention: rows of the caches must start at multiples of 16 bytes");
   for (int i = 0; i < 2; ++i)
@@ -723,7 +726,7 @@ extern "C" int mk_op_check(void) { return mk_serving::report_lost_wait(); }
 extern "C" int64_t mk_chunk_attention_workspace(const mk_chunk_attention_args* args) {
   using namespace mk_serving;
   if (!args) return fail(MK_E_INVALID, "chunk_attention: null arguments");
-  if (int rc = check(*args)) return rc;
+  if (int rc = check_sizes(*args)) return rc;
   return (int64_t)layout_of(*args).bytes;
 }
 
@@ -732,7 +735,8 @@ extern "C" int mk_chunk_attention(const mk_chunk_attention_args* args, void* str
   if (!args) return fail(MK_E_INVALID, "chunk_attention: null arguments");
   const mk_chunk_attention_args& a = *args;
   if (int rc = report_lost_wait()) return rc;
-  if (int rc = check(a)) return rc;
+  if (int rc = check_pointers(a)) return rc;
+  if (int rc = check_sizes(a)) return rc;
   if (a.tokens == 0) return 0;
   const Layout l = layout_of(a);
   if (!a.workspace || a.workspace_bytes < (int64_t)l.bytes || (((uintptr_t)a.workspace) & 15))

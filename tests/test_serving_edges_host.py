@@ -186,3 +186,27 @@ def test_the_binding_shares_the_process_c_plus_plus_runtime(native_lib):
     code = "import torch, fleet_chiplet_megakernel_b200.serving as s\ntry: s._load().plan_step(1, 2, 3)\nexcept RuntimeError as e: print(e)"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
     assert r.returncode == 0 and "3 arguments, 14 are needed" in r.stdout, (r.returncode, r.stdout, r.stderr)
+
+
+# ------------------------------------------------------------------------------------
+# the workspace of chunk_attention
+# ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("page,max_new", [(64, 0), (64, 1), (12, 0)])
+def test_workspace_follows_from_the_shapes_alone(native_lib, page, max_new):
+    """It may be asked for before there is any memory, and has to be asked for every shape: chunks of few rows are cut into pieces, longer ones are not."""
+    row = 8 * 128
+    need = {}
+    for tokens in (1, 8, 64, 512, 4096):
+        a = filled(_cabi.MkChunkAttentionArgs, dtype=_cabi.MK_BF16, tokens=tokens, q_heads=32, kv_heads=8, page_size=page, pages=100, requests=1, max_new=max_new, scale=0.1, window=0, sinks=0,
+                   q_stride=(32 * 128, 128), out_stride=(32 * 128, 128), k_cache_stride=(page * row, row, 128), v_cache_stride=(page * row, row, 128))
+        need[tokens] = native_lib.mk_chunk_attention_workspace(C.byref(a))
+        assert need[tokens] > 0
+        for name, kind in _cabi.MkChunkAttentionArgs._fields_:
+            if kind is C.c_void_p:
+                setattr(a, name, None)
+        assert native_lib.mk_chunk_attention_workspace(C.byref(a)) == need[tokens]
+    if page == 64 and max_new == 0:
+        tile = lambda tokens, splits: splits * tokens * 32 * 130 * 4  # noqa: E731 (as many pieces as there are SMs for, of 64 tokens and a kv head each)
+        assert need[64] == tile(64, 16) and need[512] == tile(512, 2) and need[4096] == 16 and need[8] < need[64] > need[4096]
+    else:
+        assert len(set(need.values())) <= 2  # of the kernel for few rows: a share per SM
