@@ -671,7 +671,8 @@ int check_pointers(const mk_chunk_attention_args& a) {
   if (!a.q || !a.k_cache || !a.v_cache || !a.qo_indptr || !a.kv_indptr || (!a.kv_indices && a.num_indices != 0) || !a.last_page_len || !a.out)
     return fail(MK_E_INVALID, "chunk_attention: null pointer");  // (an empty tensor has no address)
   if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out)) return fail(MK_E_INVALID, "chunk_attention: pointers must be 16-byte aligned");
-  return 0;
+  return refuse_misaligned("chunk_attention", {{"lse", a.lse, 4}, {"qo_indptr", a.qo_indptr, 4}, {"kv_indptr", a.kv_indptr, 4}, {"kv_indices", a.kv_indices, 4},
+                                               {"last_page_len", a.last_page_len, 4}});
 }
 int check_sizes(const mk_chunk_attention_args& a) {
   if (a.dtype != MK_BF16 && a.dtype != MK_F16) return fail(MK_E_INVALID, "chunk_attention: rows and caches are bf16 or fp16");

@@ -216,6 +216,10 @@ extern "C" int mk_rotate_append(const mk_rotate_append_args* args, void* stream)
                          rows("k", a.k, a.kv_heads, a.k_stride), rows("v", a.v, a.kv_heads, a.v_stride), table("cos", a.cos, a.table_stride[0]),
                          table("sin", a.sin, a.table_stride[1]), list_of("positions", a.positions, a.tokens, 4), list_of("slots", a.slots, a.tokens, 8),
                          list_of("q_norm", a.q_norm, kHeadDim, 2), list_of("k_norm", a.k_norm, kHeadDim, 2), rows("q", in_place ? nullptr : a.q, a.q_heads, a.q_stride)};
+  if (int rc = refuse_misaligned("rotate_append", {{"q", a.q, 2}, {"k", a.k, 2}, {"v", a.v, 2}, {"cos", a.cos, (int)entry}, {"sin", a.sin, (int)entry}, {"positions", a.positions, 4},
+                                                   {"slots", a.slots, 8}, {"k_cache", a.k_cache, 2}, {"v_cache", a.v_cache, 2}, {"q_norm", a.q_norm, 2}, {"k_norm", a.k_norm, 2},
+                                                   {"out", a.out, 2}}))
+    return rc;
   if (int rc = refuse_shared("rotate_append", used, 3, sizeof used / sizeof *used)) return rc;
   const cudaStream_t s = (cudaStream_t)stream;
   if (a.dtype == MK_BF16) return f32 ? launch<__nv_bfloat16, float>(a, wide, s) : launch<__nv_bfloat16, __nv_bfloat16>(a, wide, s);

@@ -1128,6 +1128,9 @@ extern "C" int mk_sample_tokens(const mk_sample_args* args, void* stream) {
                          {"logits", a.logits, (long long)a.vocab * size, 1, {a.rows}, {a.row_stride * size}}, list_of("u", a.u, a.requests, 4),
                          list_of("temperature", a.temperature, a.requests, 4), list_of("top_k", a.top_k, a.requests, 4), list_of("top_p", a.top_p, a.requests, 4),
                          list_of("min_p", a.min_p, a.requests, 4), list_of("qo_indptr", a.qo_indptr, a.requests + 1ll, 4)};
+  if (int rc = refuse_misaligned("sample_tokens", {{"out", a.tokens, 8}, {"logprobs", a.logprobs, 4}, {"logits", a.logits, size}, {"u", a.u, 4}, {"temperature", a.temperature, 4},
+                                                   {"top_k", a.top_k, 4}, {"top_p", a.top_p, 4}, {"min_p", a.min_p, 4}, {"qo_indptr", a.qo_indptr, 4}}))
+    return rc;
   if (int rc = refuse_shared("sample_tokens", used, 2, sizeof used / sizeof *used)) return rc;
   const cudaStream_t st = (cudaStream_t)stream;
   const cudaError_t e = a.dtype == MK_F32 ? launch<float>(a, st) : a.dtype == MK_BF16 ? launch<__nv_bfloat16>(a, st) : launch<__half>(a, st);

@@ -10,6 +10,7 @@
 #include <stdio.h>
 
 #include <atomic>
+#include <initializer_list>
 
 #include "../../include/b200mk.h"
 
@@ -59,6 +60,14 @@ inline Memory list_of(const char* name, const void* at, long long n, int bytes) 
 bool share_memory(const Memory& a, const Memory& b);
 // The first pair of the `n` that shares memory, the first `written` of them with any other: an error that names them (0: none).
 int refuse_shared(const char* what, const Memory* m, int written, int n);
+
+// An address that is no multiple of its element's size: an error that names it (0: none).  torch's own tensors have none, an address from elsewhere may.
+struct Address {
+  const char* name;
+  const void* at;
+  int bytes;
+};
+int refuse_misaligned(const char* what, std::initializer_list<Address> all);
 
 inline bool aligned16(const void* p) { return (((uintptr_t)p) & 15) == 0; }
 

@@ -260,6 +260,11 @@ int refuse_shared(const char* what, const Memory* m, int written, int n) {  // (
       if (at[i].first < at[j].last && at[j].first < at[i].last && share_memory(m[i], m[j])) return fail(MK_E_INVALID, "%s: %s and %s share memory", what, m[i].name, m[j].name);
   return 0;
 }
+int refuse_misaligned(const char* what, std::initializer_list<Address> all) {
+  for (const Address& a : all)
+    if ((uintptr_t)a.at % (unsigned)a.bytes) return fail(MK_E_INVALID, "%s: %s must be a multiple of %d bytes", what, a.name, a.bytes);
+  return 0;
+}
 char* error_text() {
   static thread_local char text[kErrorBytes];
   return text;
@@ -324,6 +329,11 @@ extern "C" int mk_plan_step(const mk_step_plan_args* args, void* stream) {
       const uintptr_t x = (uintptr_t)arrays[i].at, y = (uintptr_t)arrays[j].at;
       if (x < y + arrays[j].bytes && y < x + arrays[i].bytes) return fail(MK_E_INVALID, "plan_step: %s and %s share memory", arrays[i].name, arrays[j].name);
     }
+  if (int rc = refuse_misaligned("plan_step", {{"lengths", a.lengths, 4}, {"new_tokens", a.new_tokens, 4}, {"block_table", a.block_table, 4}, {"free_pages", a.free_pages, 4},
+                                               {"free_range", a.free_range_in, 8}, {"qo_indptr", a.qo_indptr, 4}, {"kv_indptr", a.kv_indptr, 4}, {"kv_indices", a.kv_indices, 4},
+                                               {"last_page_len", a.last_page_len, 4}, {"slots", a.slots, 8}, {"positions", a.positions, 4}, {"granted", a.granted, 4},
+                                               {"free_range", a.free_range_out, 8}}))
+    return rc;
   const size_t smem = 4 * (n + 1) * sizeof(int);
   if (smem > 48 * 1024) {
     const cudaError_t e = allow_shared<step_plan_kernel>(4 * (MK_STEP_MAX_REQUESTS + 1) * (int)sizeof(int));

@@ -210,3 +210,15 @@ def test_workspace_follows_from_the_shapes_alone(native_lib, page, max_new):
         assert need[64] == tile(64, 16) and need[512] == tile(512, 2) and need[4096] == 16 and need[8] < need[64] > need[4096]
     else:
         assert len(set(need.values())) <= 2  # of the kernel for few rows: a share per SM
+
+
+def test_operators_refuse_addresses_between_elements(native_lib):
+    """Every pointer of every call, one byte on (all tensors are apart): the kernels' loads want whole elements."""
+    for cls, fn, more in ((_cabi.MkStepPlanArgs, "mk_plan_step", dict(table_stride=1)),
+                          (_cabi.MkRotateAppendArgs, "mk_rotate_append", dict(dtype=_cabi.MK_BF16, table_dtype=_cabi.MK_F32)),
+                          (_cabi.MkChunkAttentionArgs, "mk_chunk_attention", dict(dtype=_cabi.MK_BF16, workspace_bytes=1 << 40)),
+                          (_cabi.MkSampleArgs, "mk_sample_tokens", dict(dtype=_cabi.MK_BF16))):
+        names = [n for n, kind in cls._fields_ if kind is C.c_void_p]
+        apart = {n: FAKE + (k << 26) for k, n in enumerate(names)}
+        for name in names:
+            refused(native_lib, fn, filled(cls, **{**apart, **more, name: apart[name] + 1}), _cabi.MK_E_INVALID, "aligned" if name in ("q", "out", "k_cache", "v_cache", "workspace") and cls is _cabi.MkChunkAttentionArgs else "multiple of")
