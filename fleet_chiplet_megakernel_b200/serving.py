@@ -117,7 +117,10 @@ def chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, last_
     last positions.  One new token each (decode), chunks, or both in one batch.  ``window`` > 0: a row at position p sees positions above
     p - window and the first ``sinks``.  ``scale``: 1/sqrt(128) if None.  Rows behind the last request are left as they were; a row that
     sees nothing is zero.  ``lse`` [tokens, q_heads] fp32, if given, takes the natural logarithm of each row's sum of weights.
-    ``max_new``: the largest number of new tokens of a request, if the caller knows it; it chooses kernels, nothing else depends on it.
+    ``max_new``: the largest number of new tokens of a request, if the caller knows it (0: no); say it for a batch of single tokens, which then need not
+    pass by the kernel for chunks.  It only chooses kernels and may be wrong.  Both kernels hold scores, weights' sums and outputs in fp32.  Requests of up to
+    32 rows (new tokens x q heads of a kv head) enter the product with V with weights of two 16-bit parts, longer chunks with weights rounded to the
+    cache's type, which adds about as much error as the rounding of ``out``; so the last bits of a row depend on the kernel that takes it.
     Returns ``out`` [tokens, q_heads, 128], which may not share memory with q."""
     return (_native or _load()).chunk_attention(q, k_cache, v_cache, qo_indptr, kv_indptr, kv_indices, last_page_len, scale, window, sinks, out, lse, max_new)
 

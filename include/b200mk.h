@@ -264,7 +264,8 @@ int mk_rotate_append(const mk_rotate_append_args* args, void* stream);
  * among them, as the last positions), head dimension 128.  window > 0: a row at position p sees positions above p - window and the
  * first `sinks`.  Rows behind the last request are left as they are; a row that sees nothing is zero with lse minus infinity.
  * lse (natural logarithm of the sum of weights) may be NULL.  max_new, if not 0, is the largest number of new tokens of a
- * request as far as the host knows it: it chooses kernels, results do not depend on it.  mk_chunk_attention_workspace gives the
+ * request as far as the host knows it: it chooses kernels.  The one for chunks (more than 32 rows, new tokens x q heads of a kv head) rounds weights to the
+ * cache's type ahead of their product with V, the one for few rows has them in two parts; otherwise results do not depend on it, nor on its being right.  mk_chunk_attention_workspace gives the
  * bytes of the workspace of such a call from its sizes, types, strides and scale, whatever its pointers are, or MK_E_*.  It is asked for every
  * shape: the bytes do not grow with the batch (pieces of rows are kept where there are few). */
 typedef struct mk_chunk_attention_args {

@@ -228,3 +228,10 @@ def test_plan_grants_no_position_past_32_bits():
         own = [(2047 * page + page - 4 + i, top - 3 + i) for i in range(granted)]
         assert list(zip(plan.slots.tolist(), plan.positions.tolist()))[: granted + 2] == own + [(2050 * page, 0), (2050 * page + 1, 1)]
         assert plan.last_page_len.tolist() == [page - 4 + granted, 2]
+
+
+@pytest.mark.parametrize("max_new", [1, 2, 9, 100, 10 ** 6, 2 ** 31 - 1])
+def test_attention_whatever_the_caller_says_of_its_longest_chunk(max_new):
+    """max_new chooses kernels; one that is too small or too large leaves the results within what every case is allowed."""
+    Batch([(300, 1), (64, 90), (0, 33), (700, 7), (5, 0)], 8, 2, 16, pad=2).check(max_new=max_new)
+    Batch([(200, 40)], 14, 2, 8, dtype=FP).check(max_new=max_new, window=50, sinks=2)
