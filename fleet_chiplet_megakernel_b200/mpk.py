@@ -77,8 +77,8 @@ class MPKMetadata:
     spec_decode_config: Optional[object] = None
     use_cutlass_kernel: bool = True
     eos_token_id: int = -1
-    logits: Optional[torch.Tensor] = None  # [max_num_batched_tokens, vocab] bf16: filled by every pass (extension; sample_tokens reads it)
     extra: dict = field(default_factory=dict)  # further PersistentKernel arguments (numerics, max_iterations, ...)
+    logits: Optional[torch.Tensor] = None  # [max_num_batched_tokens, vocab] bf16: filled by every pass (extension; sample_tokens reads it)
 
     def check_valid(self):
         if self.weight_from_model:

@@ -1,5 +1,6 @@
 """The serving operators at the edges of what their documentation allows, as far as no GPU is needed."""
 import ctypes as C
+import dataclasses
 import os
 import random
 import socket
@@ -222,3 +223,12 @@ def test_operators_refuse_addresses_between_elements(native_lib):
         apart = {n: FAKE + (k << 26) for k, n in enumerate(names)}
         for name in names:
             refused(native_lib, fn, filled(cls, **{**apart, **more, name: apart[name] + 1}), _cabi.MK_E_INVALID, "aligned" if name in ("q", "out", "k_cache", "v_cache", "workspace") and cls is _cabi.MkChunkAttentionArgs else "multiple of")
+
+
+def test_mpk_metadata_keeps_the_order_of_its_fields():
+    """By position, the fields that were there before stand where they stood: what is new comes last."""
+    names = [f.name for f in dataclasses.fields(mk.MPKMetadata)]
+    assert names[-4:] == ["use_cutlass_kernel", "eos_token_id", "extra", "logits"]
+    values = [None] * (len(names) - 1)
+    values[-1] = {"numerics": "mpk"}
+    assert mk.MPKMetadata(*values).extra == {"numerics": "mpk"} and mk.MPKMetadata(*values).logits is None
