@@ -1118,7 +1118,8 @@ extern "C" int mk_sample_tokens(const mk_sample_args* args, void* stream) {
   const mk_sample_args& a = *args;
   if ((!a.logits && a.rows != 0) || !a.u || !a.tokens) return fail(MK_E_INVALID, "sample_tokens: null pointer");  // (an empty tensor has no address)
   if (a.dtype != MK_BF16 && a.dtype != MK_F16 && a.dtype != MK_F32) return fail(MK_E_INVALID, "sample_tokens: logits are bf16, fp16 or fp32");
-  if (a.requests < 0 || a.rows < 0 || a.vocab < 1 || a.vocab > 0x3fffffff) return fail(MK_E_INVALID, "sample_tokens: bad sizes");
+  if (a.requests < 0 || a.rows < 0 || a.vocab < 1) return fail(MK_E_INVALID, "sample_tokens: bad sizes");
+  if (a.vocab > 0x3fffffff) return fail(MK_E_TOO_LARGE, "sample_tokens: a vocabulary of %d (up to 2^30 - 1)", a.vocab);
   if (a.requests > 0x7fffffff / kMaxCluster) return fail(MK_E_TOO_LARGE, "sample_tokens: %d requests", a.requests);
   if (!a.qo_indptr && a.rows < a.requests) return fail(MK_E_INVALID, "sample_tokens: %d rows of logits for %d requests", a.rows, a.requests);
   if (a.requests == 0) return 0;

@@ -232,3 +232,7 @@ def test_mpk_metadata_keeps_the_order_of_its_fields():
     values = [None] * (len(names) - 1)
     values[-1] = {"numerics": "mpk"}
     assert mk.MPKMetadata(*values).extra == {"numerics": "mpk"} and mk.MPKMetadata(*values).logits is None
+
+
+def test_a_vocabulary_beyond_the_counters_is_a_limit_and_no_mistake(native_lib):
+    refused(native_lib, "mk_sample_tokens", filled(_cabi.MkSampleArgs, dtype=_cabi.MK_F32, vocab=1 << 30), _cabi.MK_E_TOO_LARGE, "vocabulary")
