@@ -89,6 +89,10 @@ struct Checks {
   c10::Device device;
   explicit Checks(const at::Tensor& t, const char* what) : device(t.device()) {
     need(t.is_cuda(), what, " must be a CUDA tensor; there is no CPU fallback");
+    plain(t, what);
+  }
+  static void plain(const at::Tensor& t, const char* what) {
+    need(!t.is_neg(), what, " is negated lazily: pass x.resolve_neg()");
     no_gradient(t, what);
   }
   static void no_gradient(const at::Tensor& t, const char* what) {
@@ -98,7 +102,7 @@ struct Checks {
   void here(const at::Tensor& t, const char* what) const {
     REFUSE_IF(t.device() != device, what, " is on ", t.device(), ", the first tensor on ", device);
     need(t.layout() == at::kStrided, what, ": a strided tensor is needed");
-    no_gradient(t, what);
+    plain(t, what);
   }
   void type(const at::Tensor& t, const char* what, at::ScalarType dt) const {
     here(t, what);

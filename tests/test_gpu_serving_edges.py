@@ -235,3 +235,15 @@ def test_attention_whatever_the_caller_says_of_its_longest_chunk(max_new):
     """max_new chooses kernels; one that is too small or too large leaves the results within what every case is allowed."""
     Batch([(300, 1), (64, 90), (0, 33), (700, 7), (5, 0)], 8, 2, 16, pad=2).check(max_new=max_new)
     Batch([(200, 40)], 14, 2, 8, dtype=FP).check(max_new=max_new, window=50, sinks=2)
+
+
+def test_tensors_that_are_negated_lazily_are_refused():
+    """A view that only records a sign (of the imaginary part of a conjugate, for instance) holds other numbers than its memory."""
+    b = Batch([(40, 2)], 8, 2, 16)
+    logits, u = rnd(gen(0), 2, 50, dtype=torch.float32), torch.rand(2, device="cuda")
+    b.q = torch._neg_view(b.q)
+    with pytest.raises(ValueError, match="q is negated"):
+        b.run()
+    with pytest.raises(ValueError, match="logits is negated"):
+        mk.sample_tokens(torch._neg_view(logits), u)
+    assert torch.equal(mk.sample_tokens(torch._neg_view(logits).resolve_neg(), u), mk.sample_tokens(-logits, u))
