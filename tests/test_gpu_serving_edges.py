@@ -2,12 +2,15 @@
 16-bit type has no value for, positions next to 2^31, tangents, tensors that share memory, waits that run out."""
 import ctypes as C
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
 
 import fleet_chiplet_megakernel_b200 as mk
 from fleet_chiplet_megakernel_b200 import _cabi
+from tests.conftest import ROOT
 from tests.test_gpu_serving import Batch, check_sample, gen, i32, rnd
 
 pytestmark = pytest.mark.gpu
@@ -235,6 +238,30 @@ def test_attention_whatever_the_caller_says_of_its_longest_chunk(max_new):
     """max_new chooses kernels; one that is too small or too large leaves the results within what every case is allowed."""
     Batch([(300, 1), (64, 90), (0, 33), (700, 7), (5, 0)], 8, 2, 16, pad=2).check(max_new=max_new)
     Batch([(200, 40)], 14, 2, 8, dtype=FP).check(max_new=max_new, window=50, sinks=2)
+
+
+def test_the_first_call_of_a_process_may_be_a_captured_one():
+    """What a process sets up once (shared memory of the kernels, tensor maps, the word that waits report to) is no part of the graph."""
+    code = """
+import torch, fleet_chiplet_megakernel_b200 as mk
+from tests.test_gpu_serving import Batch
+b = Batch([(40, 2), (0, 300), (9, 1)], 8, 2, 16)
+logits, u = torch.randn(3, 5000, device="cuda"), torch.rand(3, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    b.run()
+    tokens = mk.sample_tokens(logits, u, 0.9, 0, 0.9)
+g.replay()
+torch.cuda.synchronize()
+got = b.out.clone()
+b.check()
+assert torch.equal(got, b.out) and torch.equal(tokens, mk.sample_tokens(logits, u, 0.9, 0, 0.9))
+mk.serving.check_waits()
+print("captured first")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=ROOT)
+    assert r.returncode == 0 and "captured first" in r.stdout, (r.returncode, r.stdout, r.stderr[-2000:])
 
 
 def test_tensors_that_are_negated_lazily_are_refused():
