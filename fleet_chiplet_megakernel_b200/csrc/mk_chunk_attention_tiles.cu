@@ -469,14 +469,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       l *= alpha;
       __syncwarp();  // (loads and stores of tensor memory are a warp's together, here and behind the call)
       if (!sums) return;
-#pragma unroll 1
-      for (int c = 0; c < 8; ++c) {
-        uint32_t o[16];
-        tm_load16(to + 16 * c, o);
-        tm_wait_load();
+      // The next columns come while these are scaled.  (fp16 rows move their base more often than bf16 ones, within a window after its first tile
+      // above all, which has few positions: windows of 1024 over 7100 rows 202 us without, 196 so; 183 if it moved after 2^8, which leaves 2^7 for the lift.)
+      uint32_t o[2][16];
+      tm_load16(to, o[0]);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-        tm_store16(to + 16 * c, o);
+      for (int c = 0; c < 8; ++c) {
+        tm_wait_load();
+        if (c < 7) tm_load16(to + 16 * (c + 1), o[(c + 1) & 1]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[c & 1][e] = __float_as_uint(__uint_as_float(o[c & 1][e]) * alpha);
+        tm_store16(to + 16 * c, o[c & 1]);
       }
     };
     for (int i = 0; i < n; ++i) {
