@@ -8,7 +8,7 @@
 // range writes its outputs; pieces of a group are joined in shared memory by the CTA when its warps are done, and what is left of groups
 // that several CTAs have worked on by a second kernel, both in the order of the positions.  K and V tiles come by 16-byte
 // cp.async into a ring of the warp's own, two tiles ahead of the sums and across the border between two groups.
-// 64 requests of 90 to 2200 positions, 8 kv heads: 57 us, 5.3 TB/s of 6.5 that a copy reaches; 4 of 20000 to 32700, 4 kv heads: 43 us, 5.0
+// 64 requests of 90 to 2200 positions, 8 kv heads: 57 us, 5.3 TB/s of 6.5 that a copy reaches; 4 of 20000 to 32700, 4 kv heads: 44 us, 4.9
 // TB/s.  A bare cp.async stream of this shape reaches 6.0 to 6.2; the rest is the ring's filling, the last CTA and the merge.
 // (CTAs taking a group's tiles with all warps in turn, joined after every group: 46 us like this for long contexts, but twice the
 // time for short ones, 123 and 62 us, where what begins and ends a group is longer than the ring covers.)
@@ -634,6 +634,8 @@ template <typename T, int NT, int RING> int launch_rows(const AttnParams& p, boo
 // Requests of up to 32 rows a kv head (new tokens x its q heads) are the row kernel's.  (24 requests of 6 tokens and a chunk of 200, 4 q heads a
 // kv head: 79 us, with 16 as the limit 69; but 8 x 6 tokens alone 36 and 57, 64 x 6 84 and 90.  With 64 as the limit: 8 x 12 tokens 50
 // instead of 59, 64 x 12 143 instead of 90.)
+// A caller that gives no max_new has a grid of the tile kernel's launched ahead, whose CTAs find nothing to do in a batch of single tokens: 64 of 90 to
+// 2200 positions, 32 q and 8 kv heads: 66 us, 57 with max_new; 4 of 20000 to 32700: 48 and 44.
 constexpr int kFewRows = 32;
 struct Layout {
   bool rows, tiles;

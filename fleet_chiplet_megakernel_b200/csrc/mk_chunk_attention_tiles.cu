@@ -16,9 +16,10 @@
 // V rows behind a request's last position are cleared in shared memory (weight 0 times NaN is NaN); pieces whose sums are not
 // finite all the same are done again by exact_row.
 // Few CTAs (short chunks of long requests): every row tile's positions are cut into pieces, and a second kernel merges them.
-// 2048 tokens behind 6111, 32 q and 8 kv heads: 230 us in bf16 (1040 TFLOP/s), 256 in fp16, the products alone 172 (256 items take two turns of
+// 2048 tokens behind 6111, 32 q and 8 kv heads: 230 us in bf16 (1040 TFLOP/s), 250 in fp16, the products alone 172 (256 items take two turns of
 // 148 CTAs).  A pair of tiles takes 2.0 us, the products 1.1 of it, the exponentials as much; a CTA 10 us to begin and to end, which bounds
-// short walks (windows of 1024 over 7100 rows: 174 us).
+// short walks (windows of 1024 over 7100 rows: 172 us, 196 in fp16).
+// Every wait has a limit; what gives up is reported (lost_word), and nothing is under way when the CTA ends.
 #include <cuda.h>
 
 #include "mk_chunk_attention.cuh"
@@ -198,8 +199,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the row kernel takes the SMs as they become free
   // The CTA's rows.  CTAs that begin late should have little to do: of up to 32 requests the one with most positions comes first, else the last
-  // of the batch, and of its rows the last (6 chunks of 90 to 333 tokens behind 330 to 1900 cached: 59 us, 63 in the
-  // order of the batch).
+  // of the batch (a warp's lanes hold the requests), and of its rows the last (6 chunks of 90 to 333 tokens behind 330 to 1900 cached: 59 us, 63 in the
+  // order of the batch; more than 32 requests have not been tried).
   const int pieces = a.kv_heads * p.splits, tokens = 2 * tp.tokens_per_tile;
   const int slot = (int)(blockIdx.x / pieces), piece = blockIdx.x % pieces;
   const int kv_head = piece % a.kv_heads, split = piece / a.kv_heads;

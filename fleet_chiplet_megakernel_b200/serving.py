@@ -82,8 +82,8 @@ def plan_step(lengths, new_tokens, block_table, free_pages, free_range, page_siz
     Free pages are ``free_pages[i % len(free_pages)]`` for ``free_range[0] <= i < free_range[1]``.  Requests take pages and token rows in their
     order; one that cannot have all of them is granted nothing, nor are those behind it that need any.  One whose row of the table is too short, or that
     would pass 2^31 - 1 tokens, is granted nothing and holds up nobody.  Pages of ended requests go behind the ring's tail first and can be taken
-    in the same step.  ``block_table`` and ``free_pages`` are brought up to date in place; the step counts once the caller takes ``plan.free_range`` and ``lengths + plan.granted`` (0 for ended requests) into its next one:
-    until then the same call gives the same plan."""
+    in the same step.  ``block_table`` and ``free_pages`` are brought up to date in place; the step counts once the caller takes ``plan.free_range`` and
+    ``lengths + plan.granted`` (0 for ended requests) into its next one: until then the same call gives the same plan."""
     if not isinstance(plan, StepPlan):
         raise ValueError("plan: a StepPlan is needed")
     (_native or _load()).plan_step(lengths, new_tokens, block_table, free_pages, free_range, page_size, plan.qo_indptr, plan.kv_indptr, plan.kv_indices,
