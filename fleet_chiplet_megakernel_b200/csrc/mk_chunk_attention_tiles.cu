@@ -462,7 +462,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
       const bool grow = top > base + kGrow<T> || (unset && top > -INFINITY);
       if (!__any_sync(kAll, grow)) return;
       const float to_base = kLift<T> != 0.f ? ceilf(top) : top;  // (a whole number, so that the lift can be taken from it without rounding)
-      const float alpha = !grow ? 1.f : unset ? 0.f : ex2(base - to_base);  // (no weight yet: whatever there is, is zero)
+      // (no weight yet: whatever there is, is zero.  exp2f and not ex2, which has no numbers below 2^-126: a weight of 2^127 is what the row may
+      // consist of.)
+      const float alpha = !grow ? 1.f : unset ? 0.f : exp2f(base - to_base);
       if (grow) {
         base = to_base;
         unset = false;
@@ -539,7 +541,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) chunk_attention_tiles(const _
     T* rows[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) rows[k] = reinterpret_cast<T*>(__shfl_sync(kAll, reinterpret_cast<unsigned long long>(dst), (lane & ~3) + k));
-    bool bad = mine && !isfinite(l);
+    bool bad = mine && !(l < 0x1p100f);  // (sums that are not finite, or with those of other pieces might not be)
     const float inv = !ok ? __uint_as_float(0x7fc00000u) : p.splits > 1 ? kDrop : l == 0.f ? 0.f : kDrop / l;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {

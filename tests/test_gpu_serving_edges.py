@@ -274,3 +274,21 @@ def test_tensors_that_are_negated_lazily_are_refused():
     with pytest.raises(ValueError, match="logits is negated"):
         mk.sample_tokens(torch._neg_view(logits), u)
     assert torch.equal(mk.sample_tokens(torch._neg_view(logits).resolve_neg(), u), mk.sample_tokens(-logits, u))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("at", [200, 130, 400, 470])
+@pytest.mark.parametrize("requests,heads", [([(420, 60)] * 11, (32, 8)), ([(5000, 60)], (8, 2))])
+def test_attention_whose_scores_grow_by_the_range_of_a_float(requests, heads, at, dtype):
+    """All scores are 0 but one position's, which lie 120 to 134 above in base 2, row by row: in the bf16 tiles its weight is next to the largest float, or beyond
+    it, until the base of the row follows (it never does behind the last tile), and what the weights are scaled by then is next to the smallest."""
+    b = Batch(requests, *heads, 64, dtype, spoil=False)
+    per_log2 = 1 / (D ** -0.5 * math.log2(math.e))
+    b.k.zero_(), b.q.zero_()
+    b.q[..., 0] = 1.0
+    b.q[..., 1] = torch.linspace(-1, 1, b.q.shape[0] * b.n_q, device="cuda").view(b.q.shape[0], b.n_q).to(dtype)
+    for r, (c, n) in enumerate(requests):
+        p = c + n - 480 + at  # (a position that the cache has)
+        page = b.kv_indices[b.kv[r] + p // 64].long()
+        b.k[page, p % 64, :, 0], b.k[page, p % 64, :, 1] = round(127 * per_log2 / 4) * 4, round(7 * per_log2)
+    b.check()
