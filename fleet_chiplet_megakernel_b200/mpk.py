@@ -258,7 +258,7 @@ class MPK:
         if not self.with_lm_head:
             raise ValueError("sample_tokens needs MirageModelConfig.with_lm_head: without it no pass fills MPKMetadata.logits")
         rows, vocab = self.metadata.logits.shape[-1], self.model_config.vocab_size
-        if self.world_size > 1 and rows != vocab:
+        if self.world_size > 1 and rows < vocab:  # (a head that is whole may be padded)
             raise NotImplementedError(f"sample_tokens: this rank's logits are {rows} of {vocab} rows of a sharded LM head; keep it whole "
                                       "(shard_qwen3_weights with shard_lm_head=False), or gather the logits and call serving.sample_tokens")
         return sample_tokens(self.metadata.logits, u, temperature, top_k, top_p, min_p, qo_indptr=self.qo_indptr_buffer, return_logprobs=return_logprobs)

@@ -24,11 +24,11 @@ NAMES = {"q": "self_attn.q_proj.weight", "k": "self_attn.k_proj.weight", "v": "s
 # ------------------------------------------------------------------------------------
 # MPK.sample_tokens
 # ------------------------------------------------------------------------------------
-def _wrapper(world_size=1, rank=0, shard_lm_head=True, with_lm_head=True, vocab=2048):
+def _wrapper(world_size=1, rank=0, shard_lm_head=True, with_lm_head=True, vocab=2048, padded=0):
     """MPK in mode online_notoken over this rank's shard, built (without a GPU nothing can be compiled)."""
     H, L, n_q, n_kv, mlp = 512, 1, 4, 2, 1024
     z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
-    w = {"embed": z(vocab, H), "norm": z(H), "lm_head": z(vocab, H)}
+    w = {"embed": z(vocab, H), "norm": z(H), "lm_head": z(padded or vocab, H)}
     for s, shape in {"q": (n_q * 128, H), "k": (n_kv * 128, H), "v": (n_kv * 128, H), "o": (H, n_q * 128), "qn": (128,), "kn": (128,), "gate": (mlp, H), "up": (mlp, H),
                      "down": (H, mlp), "ln1": (H,), "ln2": (H,)}.items():
         w[f"l0.{s}"] = z(*shape)
@@ -49,8 +49,8 @@ def _rank(rank, ws, port, ret):
     os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
     torch.distributed.init_process_group("gloo", rank=rank, world_size=ws)
     said = []
-    for shard in (True, False):
-        m = _wrapper(shard_lm_head=shard, world_size=ws, rank=rank)
+    for shard, padded in ((True, 0), (False, 0), (False, 2304)):
+        m = _wrapper(shard_lm_head=shard, world_size=ws, rank=rank, padded=padded)
         try:
             m.sample_tokens(torch.zeros(2))
         except (ValueError, NotImplementedError) as e:
@@ -62,16 +62,16 @@ def _rank(rank, ws, port, ret):
 
 
 def test_mpk_draws_from_no_slice_of_the_logits(native_lib):
-    """Two ranks: with the head cut by vocabulary rows every rank refuses; with the head whole the call goes on to the operator (which wants a GPU)."""
+    """Two ranks: with the head cut by vocabulary rows every rank refuses; with the head whole, padded or not, the call goes on to the operator (which wants a GPU)."""
     with socket.socket() as s:
         s.bind(("127.0.0.1", 0))
         port = s.getsockname()[1]
     ret = mp.Manager().dict()
     mp.spawn(_rank, args=(2, port, ret), nprocs=2, join=True)
     for rank in (0, 1):
-        (kind, text), (kind_whole, text_whole) = ret[rank]
+        (kind, text), *whole = ret[rank]
         assert kind == "NotImplementedError" and "1024 of 2048" in text and "sharded" in text
-        assert kind_whole == "ValueError" and "CUDA" in text_whole
+        assert len(whole) == 2 and all(k == "ValueError" and "CUDA" in t for k, t in whole)
 
 
 def test_mpk_draws_from_no_logits_that_nothing_fills(native_lib):
